@@ -257,7 +257,8 @@ def run(state):
                             state["v_cache"], state["slots"], need_kv=c["kv"])
     return (q, k, v, state["k_cache"], state["v_cache"]) if c["kv"] else (q, state["k_cache"], state["v_cache"])
   if op == "verify":
-    return S.verify_draft(state["target"], state["tokens"], state["u"], state["starts"], state["lens"], state["draft"])
+    return S.verify_draft(state["target"], state["tokens"], state["u"], state["starts"], state["lens"], state["draft"],
+                          out=torch.empty_like(state["tokens"], dtype=torch.int32))
   if op == "shared":
     return S.shared_prefix_decode(state["q"], state["k_cache"], state["v_cache"], state["tables"], state["ctx"], c["prefix"],
                                   state["sinks"], state["scale"], c["window"])
