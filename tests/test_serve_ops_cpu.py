@@ -1,0 +1,102 @@
+"""Operators of a serving step on CPU tensors: the plain statements against 64-bit definitions, and what is refused."""
+import pytest
+import torch
+
+from nmoe_b200.serve import ops as S
+from serve_oracle import attend, paged, rope, verify
+
+
+def i32(x):
+  return torch.tensor(x, dtype=torch.int32)
+
+
+def _attention_case(window=0, dtype=torch.float32):
+  g = torch.Generator().manual_seed(window)
+  lens, ctx, starts = [1, 3, 0, 9], [5, 3, 40, 30], [9, 10, 13, 0]
+  k, v, tables = paged(ctx, 8, 2, 16, g, dtype=dtype)
+  q = torch.randn(15, 6, 16, generator=g).to(dtype)
+  return q, k, v, tables, ctx, starts, lens, torch.randn(6, generator=g)
+
+
+@pytest.mark.parametrize("window", [0, 4])
+def test_paged_extend_plain(window):
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case(window)
+  want, _, owned = attend(q, k, v, tables, ctx, starts, lens, sinks, 0.25, window)
+  out = S.paged_extend(q, k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, window)
+  # fp32 throughout: a few hundred roundings of 2^-24 on values of order one
+  assert (out.double() - want).abs().max() < 1e-5 and (out[~owned] == 0).all()
+  keep = torch.full_like(q, 2.0)
+  S.paged_extend(q, k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, window, out=keep)
+  assert torch.equal(keep[owned], out[owned]) and (keep[~owned] == 2.0).all()
+
+
+def test_shared_prefix_decode_plain_equals_paged_decode():
+  g = torch.Generator().manual_seed(0)
+  ctx = [21, 40, 0, 33, 12]
+  k, v, tables = paged([max(c, 20) for c in ctx], 8, 2, 16, g, shared=20, dtype=torch.float32)
+  q, sinks = torch.randn(5, 6, 16, generator=g), torch.randn(6, generator=g)
+  out = S.shared_prefix_decode(q, k, v, tables, i32(ctx), 20, sinks, 0.25)
+  ref = S.paged_decode(q, k, v, tables, i32(ctx), sinks, 0.25)
+  assert torch.allclose(out, ref, atol=1e-5) and (out[2] == 0).all()
+
+
+def test_rope_append_plain():
+  g = torch.Generator().manual_seed(0)
+  qkv, pos = torch.randn(7, 8 * 16, generator=g), torch.randint(0, 10_000_000, (7,), generator=g)
+  inv = 10000.0 ** (-torch.arange(0, 16, 2).float() / 16)
+  y, _, vv = rope(qkv, pos, inv, 1.2, 4, 2)
+  kc, vc = torch.zeros(3, 4, 2, 16), torch.zeros(3, 4, 2, 16)
+  q, k, v = S.rope_append(qkv, pos, inv, 1.2, 4, 2, kc, vc, i32([3, -1, 0, 11, -1, 5, 6]), need_kv=True)
+  assert (torch.cat((q, k), 1).double() - y).abs().max() < 1e-5 and torch.equal(v.double(), vv)
+  assert torch.equal(kc.view(-1, 2, 16)[[3, 0, 11, 5, 6]], k[[0, 2, 3, 5, 6]]) and int((vc.view(-1, 32) != 0).any(-1).sum()) == 5
+  assert S.rope_append(qkv, pos, inv, 1.2, 4, 2)[1:] == (None, None)
+
+
+@pytest.mark.parametrize("dist", [False, True])
+def test_verify_draft_plain(dist):
+  g = torch.Generator().manual_seed(4)
+  lens = [1, 4, 0, 2, 6, 3] * 20
+  N, V = sum(lens), 30
+  starts = [sum(lens[:b]) for b in range(len(lens))]
+  target, draft = torch.softmax(torch.randn(N, V, generator=g), -1), torch.softmax(torch.randn(N, V, generator=g), -1)
+  tokens, u = torch.multinomial(draft, 1, generator=g).squeeze(1), torch.rand(N, generator=g)
+  want, count = verify(target.tolist(), tokens.tolist(), u.double().tolist(), starts, lens, draft.tolist() if dist else None)
+  out, n = S.verify_draft(target, tokens, u, i32(starts), i32(lens), draft if dist else None)
+  assert out.tolist() == want and n.tolist() == count and 1 < max(count)
+
+
+def test_refusals():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  ok = dict(q=q, k_cache=k, v_cache=v, block_tables=tables, context_lens=i32(ctx), q_starts=i32(starts), q_lens=i32(lens), sinks=sinks,
+            scale=0.25)
+  S.paged_extend(**ok)
+  for bad in (dict(q=q[0]), dict(q=q[:, :5]), dict(k_cache=k[:, :, :1]), dict(k_cache=k.transpose(1, 2)), dict(v_cache=v.half()),
+              dict(block_tables=tables.long()), dict(block_tables=tables[:2]), dict(context_lens=torch.tensor(ctx)), dict(sinks=sinks[:3]),
+              dict(q_starts=torch.tensor(starts)), dict(q_lens=i32(lens[:2])), dict(window=-1), dict(max_q_len=-1),
+              dict(out=torch.zeros(3, 6, 16)), dict(out=q.transpose(0, 1).contiguous().transpose(0, 1))):
+    with pytest.raises(ValueError):
+      S.paged_extend(**{**ok, **bad})
+  qd = q[:4]
+  ok = dict(q=qd, k_cache=k, v_cache=v, block_tables=tables, context_lens=i32(ctx), prefix_len=0, sinks=None, scale=0.25)
+  S.shared_prefix_decode(**ok)
+  for bad in (dict(q=q), dict(prefix_len=-1), dict(prefix_len=10_000), dict(window=-3), dict(context_lens=i32(ctx[:3]))):
+    with pytest.raises(ValueError):
+      S.shared_prefix_decode(**{**ok, **bad})
+  qkv, pos, inv = torch.randn(3, 8 * 16), torch.arange(3), torch.ones(8)
+  kc = torch.zeros(2, 4, 2, 16)
+  ok = dict(qkv=qkv, positions=pos, inv_freq=inv, conc=1.0, n_heads=4, n_kv_heads=2, k_cache=kc, v_cache=kc.clone(), slots=i32([0, 1, -1]))
+  S.rope_append(**ok)
+  for bad in (dict(qkv=qkv[0]), dict(n_heads=5), dict(n_heads=0), dict(positions=pos.float()), dict(positions=pos[:2]), dict(inv_freq=inv[:4]),
+              dict(inv_freq=inv.double()), dict(slots=None), dict(v_cache=None), dict(slots=torch.tensor([0, 1, 2])), dict(slots=i32([0])),
+              dict(k_cache=kc.bfloat16(), v_cache=kc.bfloat16())):
+    with pytest.raises(ValueError):
+      S.rope_append(**{**ok, **bad})
+  t = torch.rand(4, 9)
+  ok = dict(target_probs=t, tokens=torch.zeros(4, dtype=torch.long), uniforms=torch.rand(4), q_starts=i32([0]), q_lens=i32([4]))
+  S.verify_draft(**ok)
+  for bad in (dict(target_probs=t[0]), dict(target_probs=t.double()), dict(target_probs=t[:, :0]), dict(tokens=torch.zeros(4)),
+              dict(tokens=torch.zeros(3, dtype=torch.long)), dict(uniforms=torch.rand(4).double()), dict(uniforms=torch.rand(5)),
+              dict(q_starts=torch.tensor([0])), dict(q_lens=i32([4, 1])), dict(draft_probs=t[:2]), dict(draft_probs=t.half()),
+              dict(out=torch.zeros(4)), dict(out=i32([0, 0]))):
+    with pytest.raises(ValueError):
+      S.verify_draft(**{**ok, **bad})

@@ -1,0 +1,357 @@
+"""Operators of a serving step on the GPU against their definitions in 64 bits."""
+import pytest
+import torch
+
+from serve_oracle import attend, paged, rope, verify
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def i32(x):
+  return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def within(got, want, bound, what=""):
+  off = (got.double().cpu() - want).abs()
+  bad = off > bound
+  assert torch.isfinite(got).all(), what
+  assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / bound).max()):.2f} bounds"
+
+
+# ------------------------------------------------------------------------------------------------ rotate and append
+@pytest.mark.parametrize("N,hq,hkv,D,bs,far,pos_dtype", [
+  (1, 64, 8, 64, 16, 100, torch.int64), (5, 8, 2, 64, 8, 4096, torch.int32), (37, 14, 2, 64, 12, 200_000, torch.int64),
+  (130, 32, 4, 128, 16, 2_000_000_000, torch.int64), (3, 1, 1, 16, 1, 50, torch.int32), (9, 3, 1, 80, 5, 1000, torch.int64),
+  (600, 16, 16, 128, 64, 9000, torch.int64), (2500, 8, 2, 64, 16, 40000, torch.int64), (7, 2, 1, 512, 4, 70, torch.int32)])
+def test_rope_append(N, hq, hkv, D, bs, far, pos_dtype):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(N)
+  qkv = torch.randn(N, (hq + 2 * hkv) * D, generator=g).bfloat16()
+  pos = torch.randint(0, far, (N,), generator=g).to(pos_dtype)
+  inv = (150000.0 ** (-torch.arange(0, D, 2).float() / D)).contiguous()
+  blocks = (N + bs - 1) // bs + 2
+  kc, vc = torch.randn(blocks, bs, hkv, D, generator=g).bfloat16(), torch.randn(blocks, bs, hkv, D, generator=g).bfloat16()
+  slots = torch.randperm(blocks * bs, generator=g)[:N].int()
+  slots[::3] = -1
+  y, bound, v = rope(qkv, pos, inv, 1.3, hq, hkv)
+  kd, vd = kc.to(DEV), vc.to(DEV)
+  q, k, vo = S.rope_append(qkv.to(DEV), pos.to(DEV), inv.to(DEV), 1.3, hq, hkv, kd, vd, slots.to(DEV), need_kv=True)
+  within(q, y[:, :hq], bound[:, :hq], "q")
+  within(k, y[:, hq:], bound[:, hq:], "k")
+  assert torch.equal(vo.cpu().double(), v)
+  # the cache: live slots hold exactly the dense rows, every other slot what it held
+  ek, ev = kc.view(-1, hkv, D).clone(), vc.view(-1, hkv, D).clone()
+  live = slots >= 0
+  ek[slots[live].long()], ev[slots[live].long()] = k.cpu()[live], vo.cpu()[live]
+  assert torch.equal(kd.cpu().view(-1, hkv, D), ek) and torch.equal(vd.cpu().view(-1, hkv, D), ev)
+  # no dense K/V wanted: the same q and the same cache
+  kd2, vd2 = kc.to(DEV), vc.to(DEV)
+  q2, k2, v2 = S.rope_append(qkv.to(DEV), pos.to(DEV), inv.to(DEV), 1.3, hq, hkv, kd2, vd2, slots.to(DEV))
+  assert k2 is None and v2 is None and torch.equal(q2, q) and torch.equal(kd2, kd) and torch.equal(vd2, vd)
+  # no cache at all, strided and misaligned rows
+  wide = torch.zeros(N, qkv.size(1) + 24, dtype=torch.bfloat16, device=DEV)
+  for off in (8, 3):
+    wide[:, off:off + qkv.size(1)] = qkv.to(DEV)
+    q3, k3, _ = S.rope_append(wide[:, off:off + qkv.size(1)], pos.to(DEV), inv.to(DEV), 1.3, hq, hkv, need_kv=True)
+    assert torch.equal(q3, q) and torch.equal(k3, k)
+
+
+def test_rope_append_skips_and_reports_a_slot_past_the_cache():
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  from nmoe_b200.serve import ops as S
+  G.check_status()
+  qkv = torch.randn(3, 4 * 64, device=DEV).bfloat16()
+  kc = torch.zeros(2, 4, 1, 64, device=DEV, dtype=torch.bfloat16)
+  vc = torch.zeros_like(kc)
+  S.rope_append(qkv, torch.arange(3, device=DEV), torch.ones(32, device=DEV), 1.0, 2, 1, kc, vc, i32([7, 8, 2]))
+  with pytest.raises(NativeLibraryError, match="code=2 where=1000"):
+    G.check_status()
+  assert int((vc != 0).any(-1).sum()) == 2
+
+
+# ------------------------------------------------------------------------------------------------ attention
+SHAPES = [(64, 8, 64, 16), (8, 2, 64, 8), (14, 2, 64, 12), (16, 16, 128, 16), (32, 4, 128, 64), (16, 1, 128, 5), (1, 1, 64, 1),
+          (129, 1, 64, 16)]
+
+
+@pytest.mark.parametrize("hq,hkv,D,bs", SHAPES)
+@pytest.mark.parametrize("window,use_sinks", [(0, False), (0, True), (37, True), (1, False)])
+def test_paged_extend(hq, hkv, D, bs, window, use_sinks):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(hq * 1000 + window)
+  lens = [1, 3, 0, 70, 2, 17, 1, 5]
+  ctx = [1, 3, 40, 70, 1, 300, 129, 64]            # one new token alone, a whole prompt, none, more new tokens than context, ...
+  if hq == 129:
+    lens, ctx = lens[:3], ctx[:3]
+  k, v, tables = paged(ctx, bs, hkv, D, g)
+  # rows in an order of their own, with gaps
+  starts, at = [0] * len(lens), 3
+  for b in reversed(range(len(lens))):
+    starts[b] = at
+    at += lens[b] + b % 2
+  N = at + 4
+  q = torch.randn(N, hq, D, generator=g).bfloat16()
+  sinks = torch.randn(hq, generator=g).bfloat16() if use_sinks else None
+  want, bound, owned = attend(q, k, v, tables, ctx, starts, lens, sinks, D ** -0.5, window)
+  args = (q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None if sinks is None else sinks.to(DEV),
+          D ** -0.5, window)
+  out = S.paged_extend(*args, max_q_len=max(lens))
+  within(out.cpu()[owned], want[owned], bound[owned])
+  assert (out.cpu()[~owned] == 0).all()
+  keep = torch.full((N, hq, D), 3.0, dtype=torch.bfloat16, device=DEV)
+  S.paged_extend(*args, out=keep)                   # no bound of the lengths: the same bits; rows of no sequence stay
+  assert torch.equal(keep.cpu()[owned], out.cpu()[owned]) and (keep.cpu()[~owned] == 3.0).all()
+
+
+@pytest.mark.parametrize("D,hq,hkv", [(64, 8, 1), (128, 4, 2)])
+def test_paged_extend_long_context_and_prefill(D, hq, hkv):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(D)
+  lens, ctx = [1, 5, 333], [5003, 2500, 700]
+  k, v, tables = paged(ctx, 16, hkv, D, g)
+  starts = [0, 1, 6]
+  q = (2 * torch.randn(339, hq, D, generator=g)).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, starts, lens, None, D ** -0.5, 0)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, D ** -0.5)
+  within(out, want, bound)
+
+
+@pytest.mark.parametrize("what", ["beyond", "before"])
+def test_paged_extend_ignores_what_lies_outside(what):
+  """NaN in the slots that no token may see: behind the context in its last page, before every window."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(5)
+  lens, ctx, window = [3, 1], [90, 201], 20 if what == "before" else 0
+  k, v, tables = paged(ctx, 16, 2, 64, g)
+  clean = k.clone(), v.clone()
+  for b in range(2):
+    for t in (range(ctx[b], (ctx[b] + 15) // 16 * 16) if what == "beyond" else range(0, ctx[b] - lens[b] - window + 1)):
+      k[tables[b, t // 16].long(), t % 16] = float("nan")
+      v[tables[b, t // 16].long(), t % 16] = float("inf")
+  q = torch.randn(4, 8, 64, generator=g).bfloat16()
+  want, bound, _ = attend(q, *clean, tables, ctx, [0, 3], lens, None, 0.125, window)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, 3]), i32(lens), None, 0.125, window)
+  within(out, want, bound)
+
+
+def test_paged_extend_large_scores_and_extreme_sinks():
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(6)
+  lens, ctx = [4, 40], [400, 40]
+  k, v, tables = paged(ctx, 16, 1, 64, g)
+  k = (k.float() * 30).bfloat16()                   # scores of some hundreds that grow and fall along the context
+  q = (torch.randn(44, 4, 64, generator=g) * 4).bfloat16()
+  sinks = torch.tensor([float("-inf"), -1e30, 60.0, 3000.0])
+  want, bound, _ = attend(q, k, v, tables, ctx, [0, 4], lens, sinks, 0.125, 0)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, 4]), i32(lens), sinks.to(DEV), 0.125)
+  within(out, want, bound)
+
+
+def test_paged_extend_reports_bad_pages_and_lengths():
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  from nmoe_b200.serve import ops as S
+  G.check_status()
+  g = torch.Generator().manual_seed(7)
+  ctx = [40, 40, 40]
+  k, v, tables = paged(ctx, 16, 2, 64, g)
+  q = torch.randn(6, 8, 64, generator=g).bfloat16()
+  args = lambda t, c, s, n: S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), t.to(DEV), i32(c), i32(s), i32(n), None, 0.125, max_q_len=2)
+  good = args(tables, ctx, [0, 2, 4], [2, 2, 2])
+  G.check_status()
+  bad = tables.clone()
+  bad[1, 1] = 1 << 20
+  for t, c, s, n, where in ((bad, ctx, [0, 2, 4], [2, 2, 2], 1022), (tables, [40, 1000, 40], [0, 2, 4], [2, 2, 2], 1021),
+                            (tables, ctx, [0, 5, 4], [2, 2, 2], 1020), (tables, ctx, [0, -1, 4], [2, 2, 2], 1020),
+                            (tables, ctx, [0, 2, 4], [2, 3, 2], 1020)):
+    out = args(t, c, s, n)
+    with pytest.raises(NativeLibraryError, match="code=2 where="):
+      G.check_status()
+    assert torch.equal(out[:2], good[:2]) and torch.equal(out[5:], good[5:])      # the other sequences are not touched
+
+
+@pytest.mark.parametrize("hq,hkv,D,bs", SHAPES)
+@pytest.mark.parametrize("prefix,window,use_sinks", [(0, 0, True), (100, 0, False), (128, 0, True), (129, 60, True), (257, 200, False)])
+def test_shared_prefix_decode(hq, hkv, D, bs, prefix, window, use_sinks):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(hq + prefix)
+  ctx = [prefix + n for n in (1, 2, 70, 16, 33)]
+  k, v, tables = paged(ctx, bs, hkv, D, g, shared=prefix)
+  q = torch.randn(len(ctx), hq, D, generator=g).bfloat16()
+  sinks = torch.randn(hq, generator=g) if use_sinks else None
+  want, bound, _ = attend(q, k, v, tables, ctx, list(range(len(ctx))), [1] * len(ctx), sinks, D ** -0.5, window)
+  out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix,
+                               None if sinks is None else sinks.to(DEV), D ** -0.5, window)
+  within(out, want, bound)
+
+
+def test_shared_prefix_decode_many_rows_and_odd_contexts():
+  """More rows than one tile, padding rows (context 0), sequences shorter than the prefix."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(9)
+  prefix, hq, hkv, D = 700, 16, 2, 64
+  ctx = [prefix + 1 + (7 * b) % 90 for b in range(70)]
+  ctx[3], ctx[20], ctx[69], ctx[40] = 0, 5, 700, 650
+  k, v, tables = paged([max(c, prefix) for c in ctx], 16, hkv, D, g, shared=prefix)
+  q = torch.randn(70, hq, D, generator=g).bfloat16()
+  sinks = torch.randn(hq, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, list(range(70)), [1 if c else 0 for c in ctx], sinks, 0.125, 0)
+  out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix, sinks.to(DEV), 0.125)
+  within(out, want, bound + 1e-30)
+
+
+# ------------------------------------------------------------------------------------------------ drafted tokens
+def _verify_case(B, V, lens, dist, seed, dyadic=False):
+  g = torch.Generator().manual_seed(seed)
+  N = sum(lens)
+  starts = [sum(lens[:b]) for b in range(B)]
+  if dyadic:      # multiples of 1/16: sums are exact in every order, and uniforms fall on borders
+    target = torch.randint(0, 4, (N, V), generator=g).float() / 16
+    draft = torch.randint(0, 4, (N, V), generator=g).float() / 16
+    u = torch.randint(0, 16, (N,), generator=g).float() / 16
+  else:
+    target = torch.softmax(2 * torch.randn(N, V, generator=g), -1)
+    draft = torch.softmax(2 * target.roll(1, 0).log().mul(0.4) + torch.randn(N, V, generator=g) * 0.3, -1)
+    u = torch.rand(N, generator=g)
+  tokens = torch.multinomial(draft + 1e-9, 1, generator=g).squeeze(1)
+  return target, tokens, u, starts, draft if dist else None
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 100, 4096, 50_001])
+@pytest.mark.parametrize("dist", [False, True])
+@pytest.mark.parametrize("dyadic", [False, True])
+def test_verify_draft(V, dist, dyadic):
+  from nmoe_b200.serve import ops as S
+  lens = [1, 5, 2, 0, 3, 9, 1, 4, 6] * (1 if V > 5000 else 5)
+  target, tokens, u, starts, draft = _verify_case(len(lens), V, lens, dist, V, dyadic)
+  want, count = verify(target.tolist(), tokens.tolist(), u.double().tolist(), starts, lens, None if draft is None else draft.tolist())
+  for tok in (tokens, tokens.int()):
+    out, n = S.verify_draft(target.to(DEV), tok.to(DEV), u.to(DEV), i32(starts), i32(lens), None if draft is None else draft.to(DEV))
+    assert n.tolist() == count and out.tolist() == want
+
+
+def test_verify_draft_strided_rows_gaps_and_degenerate_rows():
+  from nmoe_b200.serve import ops as S
+  V, lens = 1003, [3, 3, 3, 2, 1, 2]
+  target, tokens, u, _, draft = _verify_case(6, V, lens, True, 3)
+  starts = [9, 0, 3, 6, 13, 15]                     # any order, gaps at 8, 12 and 14
+  N = 18
+  pad = lambda t: torch.cat((t, t[:N - t.size(0)]), 0)
+  target, tokens, u, draft = pad(target), pad(tokens), pad(u), pad(draft)
+  draft[1] = target[0]                              # the two agree: nothing to redraw from if it failed
+  tokens[1], target[0, tokens[1]] = int(target[0].argmin()), 0.0
+  draft[1, tokens[1]] = 0.0                         # 0 < 0 fails, the difference is empty: drawn from the target
+  target[14], target[15] = 0.0, 0.0
+  target[13] = 0.0                                  # a row without a positive entry
+  u[6] = 0.99999994                                 # the largest number below 1
+  u[3] = 0.0
+  want, count = verify(target.tolist(), tokens.tolist(), u.double().tolist(), starts, lens, draft.tolist())
+  wide = torch.zeros(N, V + 5, device=DEV)
+  wide[:, 2:V + 2] = target.to(DEV)
+  keep = torch.full((N,), 77, dtype=torch.int32, device=DEV)
+  out, n = S.verify_draft(wide[:, 2:V + 2], tokens.to(DEV), u.to(DEV), i32(starts), i32(lens), draft.to(DEV), out=keep)
+  assert n.tolist() == count and out.tolist() == [77 if x is None else x for x in want]
+  out2, _ = S.verify_draft(wide[:, 2:V + 2], tokens.to(DEV), u.to(DEV), i32(starts), i32(lens), draft.to(DEV))
+  assert out2.tolist() == [-1 if x is None else x for x in want]
+
+
+def test_verify_draft_emits_the_target_distribution():
+  """Tokens drawn from the draft and verified are distributed as the target: every frequency within 5.5 standard deviations
+  (24 of them, chance of a false alarm below 1e-6)."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(1)
+  V, B = 24, 200_000
+  p, q = torch.softmax(torch.randn(V, generator=g), -1), torch.softmax(torch.randn(V, generator=g), -1)
+  tokens = torch.multinomial(q, 2 * B, replacement=True, generator=g)
+  u = torch.rand(2 * B, generator=g)
+  starts = torch.arange(B, dtype=torch.int32) * 2
+  out, n = S.verify_draft(p.expand(2 * B, V).contiguous().to(DEV), tokens.to(DEV), u.to(DEV), starts.to(DEV),
+                          torch.full((B,), 2, dtype=torch.int32, device=DEV), q.expand(2 * B, V).contiguous().to(DEV))
+  freq = torch.bincount(out[0::2].cpu().long(), minlength=V).double() / B
+  sd = (p.double() * (1 - p.double()) / B).sqrt()
+  assert ((freq - p.double()).abs() < 5.5 * sd).all()
+
+
+def test_verify_draft_reports_a_token_outside_the_vocabulary():
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  from nmoe_b200.serve import ops as S
+  G.check_status()
+  target = torch.full((3, 8), 0.125, device=DEV)
+  out, n = S.verify_draft(target, torch.tensor([0, 8, 1], device=DEV), torch.zeros(3, device=DEV), i32([0]), i32([3]))
+  with pytest.raises(NativeLibraryError, match="code=2 where=1011"):
+    G.check_status()
+  assert n.tolist() == [1] and out.tolist() == [0, -1, -1]
+  S.verify_draft(target, torch.tensor([0, 1, 1], device=DEV), torch.zeros(3, device=DEV), i32([1]), i32([3]))
+  with pytest.raises(NativeLibraryError, match="code=2 where=1010"):
+    G.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ streams and graphs
+def test_a_captured_step_replays_with_new_inputs_on_another_stream():
+  """append -> attend -> verify captured on a side stream; two graphs, replayed in turn, share nothing."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(2)
+  hq, hkv, D, bs, V = 8, 2, 64, 16, 333
+  lens, ctx = [3, 1, 4], [50, 17, 200]
+  k, v, tables = paged(ctx, bs, hkv, D, g, shared=16)
+  starts, N = [0, 3, 4], 8
+  inv = (10000.0 ** (-torch.arange(0, D, 2).float() / D)).to(DEV)
+  slots, pos = [], []
+  for b in range(3):
+    for t in range(ctx[b] - lens[b], ctx[b]):
+      pos.append(t)
+      slots.append(int(tables[b, t // bs]) * bs + t % bs)
+  pos, slots = torch.tensor(pos, device=DEV), i32(slots)
+  ints = i32(ctx), i32(starts), i32(lens)
+  probs = torch.softmax(torch.randn(N, V, generator=g) * 2, -1).to(DEV)
+  tables = tables.to(DEV)
+
+  def step(s):
+    q, _, _ = S.rope_append(s["qkv"], pos, inv, 1.0, hq, hkv, s["k"], s["v"], slots)
+    o = S.paged_extend(q, s["k"], s["v"], tables, *ints, None, 0.125, max_q_len=4)
+    d = S.shared_prefix_decode(q[:3], s["k"], s["v"], tables, ints[0], 16, None, 0.125)
+    return (o, d) + S.verify_draft(probs, s["tok"], s["u"], *ints[1:])
+
+  def inputs(seed):
+    gg = torch.Generator().manual_seed(seed)
+    return dict(qkv=torch.randn(N, (hq + 2 * hkv) * D, generator=gg).bfloat16().to(DEV), k=k.to(DEV), v=v.to(DEV),
+                tok=torch.randint(0, V, (N,), generator=gg).to(DEV), u=torch.rand(N, generator=gg).to(DEV))
+
+  side = torch.cuda.Stream()
+  states, graphs, outs = [inputs(0), inputs(1)], [], []
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    for s in states:
+      step(s)
+      graph = torch.cuda.CUDAGraph()
+      with torch.cuda.graph(graph, stream=side):
+        outs.append(step(s))
+      graphs.append(graph)
+  torch.cuda.synchronize()
+  for round_ in range(2):
+    fresh = [inputs(10 + round_), inputs(20 + round_)]
+    for s, f in zip(states, fresh):
+      for key in s:
+        s[key].copy_(f[key])
+    for gr in graphs:
+      gr.replay()
+    torch.cuda.synchronize()
+    for o, f in zip(outs, fresh):
+      for a, b in zip(o, step(f)):
+        assert torch.equal(a, b)
+
+
+def test_results_do_not_change_between_runs():
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(3)
+  ctx, lens = [3000, 900, 2047], [4, 1, 3]
+  k, v, tables = paged(ctx, 16, 2, 64, g)
+  q = torch.randn(8, 16, 64, generator=g).bfloat16().to(DEV)
+  args = (q, k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, 4, 5]), i32(lens), None, 0.125)
+  first = S.paged_extend(*args)
+  for _ in range(20):
+    assert torch.equal(S.paged_extend(*args), first)
