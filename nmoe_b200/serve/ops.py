@@ -218,7 +218,7 @@ def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_st
   return out
 
 
-def _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, window):
+def _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window):
   _need(q.dim() == 3, "q must be [N, Hq, D]")
   _need(k_cache.dim() == 4, "k_cache and v_cache must be [num_blocks, block_size, Hkv, D]")
   Hq, D, Hkv, B = q.size(1), q.size(2), k_cache.size(2), context_lens.numel()
@@ -228,6 +228,7 @@ def _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, win
   _need(block_tables.dim() == 2 and block_tables.size(0) == B and context_lens.dim() == 1, "block_tables must be [B, n], context_lens [B]")
   _need(sinks is None or (sinks.shape == (Hq,) and sinks.device == q.device), "sinks must be [Hq] on q's device")
   _need(window >= 0, "window must not be negative")
+  _need(scale > 0, "scale must be positive")
 
 
 def _attention_args(q, k_cache, v_cache, block_tables, sinks):
@@ -255,7 +256,7 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   key gives zeros.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.
   Lengths or pages outside their tensors are skipped and show up in ``check_status``."""
-  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, window)
+  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
   N, Hq, D = q.shape
   B = context_lens.numel()
   _check_ints(q.device, q_starts=q_starts, q_lens=q_lens)
@@ -271,11 +272,11 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   with _on(q.device):
     out = torch.zeros(N, Hq, D, dtype=q.dtype, device=q.device) if out is None else out
     _need(_aligned(out), "out must start on a 16-byte boundary")
-    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifpp")(
+    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifippp")(
       _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), _p(q_starts),
       _p(q_lens), _p(sinks), int(sinks is not None and sinks.dtype == torch.float32), _p(out), N, B, Hq, k_cache.size(2), D,
-      k_cache.size(1), k_cache.size(0), block_tables.size(1), min(max_q_len, N), window, scale, _p(status_buffer(q.device)),
-      _stream()), "paged_extend")
+      k_cache.size(1), k_cache.size(0), block_tables.size(1), min(max_q_len, N), window, scale, 0, 0,
+      _p(status_buffer(q.device)), _stream()), "paged_extend")
   return out
 
 
@@ -289,7 +290,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
   q [B, Hq, D] -> [B, Hq, D]; block_tables [B, n] hold every sequence's whole table (prefix pages included; where the prefix
   ends inside a page, each table may have its own copy of that page).  ``context_lens`` counts the current token; a sequence
   with a context of 0 (a padding row) gives zeros, one shorter than the prefix sees its part of it."""
-  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, window)
+  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
   B, Hq, D = q.shape
   _need(context_lens.numel() == B, "q must hold one token per sequence")
   _need(0 <= prefix_len <= block_tables.size(1) * k_cache.size(1), "prefix_len must lie within the block tables")
@@ -301,10 +302,13 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
   context_lens = context_lens.contiguous()
   with _on(q.device):
     out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifpp")(
+    # (O, m, l) of every row over the prefix
+    work = torch.empty(B * Hq * (D + 2), dtype=torch.float32, device=q.device) if prefix_len > 0 else None
+    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifippp")(
       _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), 0, 0, _p(sinks),
       int(sinks is not None and sinks.dtype == torch.float32), _p(out), B, B, Hq, k_cache.size(2), D, k_cache.size(1),
-      k_cache.size(0), block_tables.size(1), 1, window, scale, _p(status_buffer(q.device)), _stream()), "shared_prefix_decode")
+      k_cache.size(0), block_tables.size(1), 1, window, scale, prefix_len, _p(work),
+      _p(status_buffer(q.device)), _stream()), "shared_prefix_decode", 2 if prefix_len > 0 else 1)
   return out
 
 

@@ -72,7 +72,7 @@ def test_refusals():
   S.paged_extend(**ok)
   for bad in (dict(q=q[0]), dict(q=q[:, :5]), dict(k_cache=k[:, :, :1]), dict(k_cache=k.transpose(1, 2)), dict(v_cache=v.half()),
               dict(block_tables=tables.long()), dict(block_tables=tables[:2]), dict(context_lens=torch.tensor(ctx)), dict(sinks=sinks[:3]),
-              dict(q_starts=torch.tensor(starts)), dict(q_lens=i32(lens[:2])), dict(window=-1), dict(max_q_len=-1),
+              dict(q_starts=torch.tensor(starts)), dict(q_lens=i32(lens[:2])), dict(window=-1), dict(max_q_len=-1), dict(scale=0.0),
               dict(out=torch.zeros(3, 6, 16)), dict(out=q.transpose(0, 1).contiguous().transpose(0, 1))):
     with pytest.raises(ValueError):
       S.paged_extend(**{**ok, **bad})
