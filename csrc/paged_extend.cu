@@ -135,7 +135,8 @@ k_paged_extend(const ExtendParams p) {
   uint64_t* s_full = kv_empty + kStages;     // [tile][buf]
   uint64_t* p_full = s_full + 2 * TILES;     // [tile][buf]
   uint64_t* pv_done = p_full + 2 * TILES;    // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + TILES);
+  uint64_t* o_full = pv_done + TILES;        // [tile]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_range = reinterpret_cast<int*>(tmem_slot + 2);          // [2] first key, end of keys
 
@@ -182,6 +183,7 @@ k_paged_extend(const ExtendParams p) {
       const int warps = rows > 0 ? (rows + 31) / 32 : 1;
       for (int i = 0; i < 2; ++i) { mbar_init(&s_full[2 * t + i], 1); mbar_init(&p_full[2 * t + i], warps); }
       mbar_init(&pv_done[t], 1);
+      mbar_init(&o_full[t], 1);
     }
     s_range[0] = 0x7fffffff;
     s_range[1] = 0;
@@ -327,7 +329,7 @@ k_paged_extend(const ExtendParams p) {
           for (int j = 0; j < PX_BN / 16; ++j)
             px_mma_ts(tmem_base + kTmemO + t * D, a_t + j * 8, make_smem_desc(va + j * 2048, PX_BN * 128, 1024, kSwizzle128B),
                       idesc_pv, (i | j) != 0 ? 1u : 0u);
-          mma_commit(&pv_done[t]);
+          mma_commit(i + 1 < n_blk ? &pv_done[t] : &o_full[t]);
         }
         mma_commit(&kv_empty[st]);
       }
@@ -407,11 +409,10 @@ k_paged_extend(const ExtendParams p) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[tile * 2 + bf]);
     }
-    // S of the last block was issued before P V of the one before, so that one may still be running: a wait on the
-    // last phase alone would pass on the parity of the phase two earlier
-    if (ok && n_blk > 1) ok = px_wait(&pv_done[tile], (n_blk - 2) & 1, abort_flag);
-    if (n_blk > 0) {
-      if (ok) ok = px_wait(&pv_done[tile], (n_blk - 1) & 1, abort_flag);
+    // The end of the last P V has a barrier of its own: pv_done alternates its parity with every block, and when a
+    // warp gets here it may still be two phases behind (P V of the block before runs after S of the last one) or done.
+    if (ok && n_blk > 0) {
+      ok = px_wait(&o_full[tile], 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1035, 0, tile); *abort_flag = 1; }
     }

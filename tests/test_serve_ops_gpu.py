@@ -345,13 +345,23 @@ def test_a_captured_step_replays_with_new_inputs_on_another_stream():
         assert torch.equal(a, b)
 
 
-def test_results_do_not_change_between_runs():
+@pytest.mark.parametrize("window", [0, 128])
+@pytest.mark.parametrize("D,hq,hkv", [(64, 64, 8), (128, 32, 4)])
+def test_results_do_not_change_between_runs(window, D, hq, hkv):
+  """Enough CTAs to fill every SM several times over: a wait that passes too early shows as a bit that changes."""
+  from nmoe_b200.ops import tc_gemm as G
   from nmoe_b200.serve import ops as S
   g = torch.Generator().manual_seed(3)
-  ctx, lens = [3000, 900, 2047], [4, 1, 3]
-  k, v, tables = paged(ctx, 16, 2, 64, g)
-  q = torch.randn(8, 16, 64, generator=g).bfloat16().to(DEV)
-  args = (q, k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, 4, 5]), i32(lens), None, 0.125)
-  first = S.paged_extend(*args)
-  for _ in range(20):
+  lens = [1 + b % 5 for b in range(40)] + [300, 290]
+  ctx = [200 + 37 * b for b in range(40)] + [900, 290]
+  starts = [sum(lens[:b]) for b in range(len(lens))]
+  k, v, tables = paged(ctx, 16, hkv, D, g)
+  k, v, tables = k.to(DEV), v.to(DEV), tables.to(DEV)
+  q = torch.randn(sum(lens), hq, D, generator=g).bfloat16().to(DEV)
+  args = (q, k, v, tables, i32(ctx), i32(starts), i32(lens), None, D ** -0.5, window)
+  one = (q[:40], k, v, tables[:1].expand(40, -1).contiguous(), i32([200] * 40), 150, None, D ** -0.5, window)
+  first, shared = S.paged_extend(*args), S.shared_prefix_decode(*one)
+  for _ in range(200):
     assert torch.equal(S.paged_extend(*args), first)
+    assert torch.equal(S.shared_prefix_decode(*one), shared)
+  G.check_status()
