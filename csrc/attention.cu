@@ -132,7 +132,9 @@ k_attn_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
   uint64_t* s_full = bars + 9;        // [tile][buf]
   uint64_t* p_full = bars + 13;       // [tile][buf]
   uint64_t* pv_done = bars + 17;      // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* o_full = bars + 19;       // [tile] the tile's last P V is done: pv_done alone is ambiguous there, a warp may reach
+                                      // the epilogue with its parity two phases behind
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -154,6 +156,8 @@ k_attn_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
     mbar_init(&pv_done[0], 1);
     mbar_init(&pv_done[1], 1);
+    mbar_init(&o_full[0], 1);
+    mbar_init(&o_full[1], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -245,7 +249,7 @@ k_attn_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           for (int j = 0; j < ATT_BN / 16; ++j)
             mma_f16_ts(tmem_base + 256 + t * 128, a_t + j * 8, make_smem_desc(va + j * 2048, ATT_BN * 128, 1024, kSwizzle128B),
                        idesc_pv, (li | j) != 0 ? 1u : 0u);
-          mma_commit(&pv_done[t]);
+          mma_commit(i + 1 < trs[t].kb_end ? &pv_done[t] : &o_full[t]);
         }
         mma_commit(&v_empty[st]);
       }
@@ -342,7 +346,7 @@ k_attn_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     }
     // epilogue
     if (ok && n_blocks > 0) {
-      ok = attn_wait(&pv_done[tile], (n_blocks - 1) & 1, abort_flag);
+      ok = attn_wait(&o_full[tile], 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 722, 0, tile); *abort_flag = 1; }
     }
