@@ -483,7 +483,7 @@ def cmd_hydra_oracle_label(a) -> int:
   with open(a.output, "a" if n_done else "w", encoding="utf-8") as f:
     for i0 in range(0, len(texts), a.flush_every):
       res = grade_prompts(eng, tok, texts[i0:i0 + a.flush_every], max_new=a.max_new, max_ctx=a.max_ctx,
-                          stop_tokens=[getattr(tok, "eot", -1)])
+                          stop_tokens=[getattr(tok, "eot", -1)], draft_tokens=a.draft_tokens)
       for did, g in zip(ids[i0:i0 + a.flush_every], res):
         f.write(json.dumps({"doc_id": did, "id": did, "ok": g["scores"] is not None, **g}) + "\n")
         parsed += int(g["scores"] is not None)
@@ -733,6 +733,7 @@ def build_parser() -> argparse.ArgumentParser:
   p.add_argument("--subdir", default=""); p.add_argument("--min-tokens", type=int, default=0); p.add_argument("--fraction", type=float, default=1.0)
   p.add_argument("--seed", type=int, default=0); p.add_argument("--limit", type=int)
   p = sub.add_parser("hydra-oracle-label"); p.set_defaults(fn=cmd_hydra_oracle_label); model_args(p, optional_io=True); p.add_argument("--max-new", type=int, default=256)
+  p.add_argument("--draft-tokens", type=int, default=0, help="tokens per step that an answer may look up in its own text and have verified")
   p.add_argument("--input-docids"); p.add_argument("--data-root"); p.add_argument("--resume", action="store_true"); p.add_argument("--flush-every", type=int, default=1024)
   p = sub.add_parser("hydra-train"); p.set_defaults(fn=cmd_hydra_train); model_args(p, heads=True)
   p.add_argument("--phase", choices=["A", "B", "C"], required=True); p.add_argument("--steps", type=int, default=1000); p.add_argument("--lr", type=float, default=1e-3)

@@ -115,11 +115,12 @@ def compute_aggregated_code(scores: Dict[str, float]) -> float:
 
 def grade_prompts(engine, tok: Tokenizer, texts: Sequence[str], *, is_code: Optional[Sequence[bool]] = None,
                   max_new: int = 256, max_ctx: int = 4096, stop_tokens: Iterable[int] = (),
-                  fmt: Optional[ChatFormat] = None) -> List[dict]:
-  """Rows ``{scores, aggregated, raw}`` in input order; ``scores`` is None when no valid JSON came back."""
+                  fmt: Optional[ChatFormat] = None, draft_tokens: int = 0) -> List[dict]:
+  """Rows ``{scores, aggregated, raw}`` in input order; ``scores`` is None when no valid JSON came back.
+  ``draft_tokens`` is the engine's: the answers' keys and braces are soon found in the rubric and in the answer itself."""
   code = list(is_code) if is_code is not None else [False] * len(texts)
   prompts = [right_trim(tok, t, is_code=c, max_ctx=max_ctx, max_new=max_new, fmt=fmt) for t, c in zip(texts, code)]
-  outs = engine.generate(prompts, max_new_tokens=max_new, stop_tokens=stop_tokens)
+  outs = engine.generate(prompts, max_new_tokens=max_new, stop_tokens=stop_tokens, draft_tokens=draft_tokens)
   rows = []
   for o, c in zip(outs, code):
     raw = tok.decode(o)

@@ -19,7 +19,8 @@ def status_buffer(device: torch.device) -> torch.Tensor:
   """Per-device int32[4] status record that kernels write when a bounded wait runs out."""
   buf = _STATUS.get(device)
   if buf is None:
-    buf = torch.zeros(4, dtype=torch.int32, device=device)
+    with torch.inference_mode(False):      # check_status resets it, also outside the inference mode that first asked for it
+      buf = torch.zeros(4, dtype=torch.int32, device=device)
     _STATUS[device] = buf
   return buf
 

@@ -13,6 +13,13 @@ prompts are prefilled together, minus any prefix already in the cache) or advanc
 sequence by one token.  ``generate`` wraps the loop for greedy / top-k sampling; ``hidden_states``
 runs prompts through the first layers only (the probe / judge taps of the curation stack).
 
+Two things shorten decoding.  Blocks that every running sequence has in common (a grading rubric, a
+few-shot header) are attended to once per step for the whole batch.  And with ``draft_tokens`` > 0
+``generate`` lets each sequence propose that many tokens per step by looking its last tokens up in
+its own text (answers that quote their prompt, structured output); one pass scores them all and
+those that fit are kept.  Greedy output is what it would be without drafts, sampled output has the
+same distribution.
+
 Behavioural counterpart: ``BatchedGenerator`` (nmoe/data/model.py:650-790).  Differences: prefix
 blocks found in the cache are really attended to during prefill, the host-side batch assembly is
 vectorised, and a request that cannot get a cache block is preempted back to the queue instead of
@@ -23,10 +30,37 @@ from __future__ import annotations
 from collections import deque
 from typing import Callable, Deque, Dict, Iterable, List, Optional, Sequence as Seq, Tuple
 
+import numpy as np
 import torch
 
+from . import ops as sops
 from .kv import BlockPool, SeqStatus, Sequence
 from .model import CacheView, Transformer
+
+
+# A shared prefix of fewer tokens is left to the per-sequence decode kernel.
+MIN_SHARED_TOKENS = 64
+
+
+class LookupDraft:
+  """Proposes the continuation of the last earlier place where a sequence had its current last 3 (else 2) tokens."""
+
+  def __init__(self):
+    self.known = 0                                  # tokens of the last call
+    self.seen: Dict[tuple, int] = {}                # n-gram -> index of the token behind its last occurrence
+
+  def propose(self, tokens: List[int], k: int) -> List[int]:
+    """``tokens``: the sequence so far; successive calls only append to it."""
+    for end in range(max(2, self.known), len(tokens)):       # n-grams that end before tokens[end]
+      for n in (2, 3):
+        if end >= n:
+          self.seen[tuple(tokens[end - n:end])] = end
+    self.known = len(tokens)
+    for n in (3, 2):
+      at = self.seen.get(tuple(tokens[-n:])) if len(tokens) >= n else None
+      if at is not None:
+        return tokens[at:at + k]
+    return []
 
 
 class Engine:
@@ -46,7 +80,8 @@ class Engine:
     self.waiting: Deque[Sequence] = deque()
     self.running: List[Sequence] = []
     self.finished: Dict[int, Sequence] = {}
-    self.steps = {"prefill": 0, "decode": 0, "prefill_tokens": 0, "cached_tokens": 0, "preempted": 0}
+    self.drafts: Dict[int, LookupDraft] = {}
+    self.steps = {"prefill": 0, "decode": 0, "prefill_tokens": 0, "cached_tokens": 0, "preempted": 0, "drafted": 0, "accepted": 0}
 
   # ------------------------------------------------------------------ requests
   def add(self, tokens: Seq[int], max_new_tokens: Optional[int] = None) -> int:
@@ -140,14 +175,106 @@ class Engine:
     ids = torch.tensor([s.tokens[-1] for s in seqs], dtype=torch.long)
     pos = torch.tensor([len(s) - 1 for s in seqs], dtype=torch.long)
     ctx = torch.tensor([len(s) for s in seqs], dtype=torch.int32)
-    max_blocks = max(len(s.block_table) for s in seqs)
-    tables = torch.zeros(len(seqs), max_blocks, dtype=torch.int32)
-    for i, s in enumerate(seqs):
-      tables[i, :len(s.block_table)] = torch.tensor(s.block_table, dtype=torch.int32)
-    cache = CacheView(self.k_cache, self.v_cache, slots.to(dev), block_tables=tables.to(dev), context_lens=ctx.to(dev),
-                      block_size=self.block_size)
+    tables = self._tables(seqs)
+    cache = CacheView(self.k_cache, self.v_cache, slots.to(dev), block_tables=torch.from_numpy(tables).to(dev), context_lens=ctx.to(dev),
+                      block_size=self.block_size, shared_len=self._shared_len(tables, int(ctx.min())))
     self.steps["decode"] += 1
     return self.model(ids.to(dev), pos.to(dev), cache=cache, is_prefill=False)
+
+  @staticmethod
+  def _tables(seqs: List[Sequence]) -> np.ndarray:
+    tables = np.zeros((len(seqs), max(len(s.block_table) for s in seqs)), dtype=np.int32)
+    for i, s in enumerate(seqs):
+      tables[i, :len(s.block_table)] = s.block_table
+    return tables
+
+  def _shared_len(self, tables: np.ndarray, shortest: int) -> int:
+    """Leading tokens whose blocks are the same in every table, where that is enough to be worth a pass of its own."""
+    if len(tables) < 2:
+      return 0
+    n_blocks = min(tables.shape[1], (shortest - 1) // self.block_size)        # the block being written is nobody else's
+    same = (tables[:, :n_blocks] == tables[:1, :n_blocks]).all(0)
+    n = (n_blocks if same.all() else int(same.argmin())) * self.block_size
+    return n if n >= MIN_SHARED_TOKENS else 0
+
+  # ------------------------------------------------------------------ several tokens per step
+  def _decode_drafts(self, seqs: List[Sequence], k: int) -> Tuple[torch.Tensor, torch.Tensor, CacheView, List[int]]:
+    """One pass over the last token of every sequence and up to ``k`` looked-up ones behind it: (logits [N, vocab], the packed
+    input tokens [N], the step's cache view, rows per sequence).  A sequence gets fewer where its budget, its context or the
+    free blocks end."""
+    dev, bs = self.device, self.block_size
+    for s in seqs:
+      self.pool.append_slot(s)                        # the step itself comes before anybody's drafts
+    ids, pos, slots, lens = [], [], [], []
+    for s in seqs:
+      room = min(k, s.max_new_tokens - s.n_generated - 1, self.max_seq_len - len(s) - 1)
+      draft = self.drafts.setdefault(s.seq_id, LookupDraft()).propose(s.tokens, room) if room > 0 else []
+      if draft:
+        draft = draft[:self.pool.reserve(s, len(draft))]
+      first = len(s) - 1
+      ids += [s.tokens[-1]] + draft
+      pos += range(first, first + 1 + len(draft))
+      slots += [self.pool.slot(s, p) for p in range(first, first + 1 + len(draft))]
+      lens.append(1 + len(draft))
+      self.steps["drafted"] += len(draft)
+    starts = [0]
+    for n in lens[:-1]:
+      starts.append(starts[-1] + n)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(dev)
+    tokens = torch.tensor(ids, dtype=torch.long).to(dev)
+    cache = CacheView(self.k_cache, self.v_cache, i32(slots), block_tables=torch.from_numpy(self._tables(seqs)).to(dev),
+                      context_lens=i32([len(s) - 1 + n for s, n in zip(seqs, lens)]), block_size=bs, q_starts=i32(starts), q_lens=i32(lens),
+                      max_q_len=max(lens))
+    self.steps["decode"] += 1
+    return self.model(tokens, torch.tensor(pos, dtype=torch.long).to(dev), cache=cache, is_prefill=False), tokens, cache, lens
+
+  @torch.inference_mode()
+  def step_drafts(self, k: int, *, temperature: float = 0.0, top_k: int = 0, generator: Optional[torch.Generator] = None
+                  ) -> Optional[List[Tuple[int, List[int]]]]:
+    """``step`` with up to ``k`` looked-up tokens per running sequence, sampling included: (sequence id, emitted tokens) of
+    every sequence that moved, at least one token each.  The caller hands them to ``update`` one by one."""
+    batch = self._admit()
+    if batch:
+      self.running.extend(batch)
+      logits = self._prefill(batch)
+      nxt = self._probs(logits, temperature, top_k)
+      nxt = logits.argmax(-1) if nxt is None else torch.multinomial(nxt, 1, generator=generator).squeeze(-1)
+      return [(s.seq_id, [t]) for s, t in zip(batch, nxt.tolist())]
+    if not self.running:
+      return None
+    self._preempt_for_space()
+    seqs = list(self.running)
+    logits, tokens, cache, lens = self._decode_drafts(seqs, k)
+    probs = self._probs(logits, temperature, top_k)
+    out, row = [], 0
+    if probs is None:                                 # greedy: a drafted token passes where it is the likeliest one
+      nxt, ids = logits.argmax(-1).tolist(), tokens.tolist()
+      for s, n in zip(seqs, lens):
+        j = 1
+        while j < n and ids[row + j] == nxt[row + j - 1]:
+          j += 1
+        out.append((s.seq_id, nxt[row:row + j]))
+        row += n
+    else:
+      u = torch.rand(tokens.numel(), device=generator.device if generator is not None else self.device, generator=generator).to(self.device)
+      emitted, count = sops.verify_draft(probs, tokens, u, cache.q_starts, cache.q_lens, out=torch.empty_like(tokens, dtype=torch.int32))
+      emitted = emitted.tolist()
+      for s, n, j in zip(seqs, lens, count.tolist()):
+        out.append((s.seq_id, emitted[row:row + j]))
+        row += n
+    self.steps["accepted"] += sum(len(t) - 1 for _, t in out)
+    return out
+
+  @staticmethod
+  def _probs(logits: torch.Tensor, temperature: float, top_k: int) -> Optional[torch.Tensor]:
+    """Sampling probabilities, None for greedy."""
+    if temperature <= 0:
+      return None
+    lg = logits / temperature
+    if top_k > 0:
+      kth = lg.topk(min(top_k, lg.size(-1)), dim=-1).values[:, -1:]
+      lg = lg.masked_fill(lg < kth, float("-inf"))
+    return torch.softmax(lg, -1)
 
   def update(self, seq_id: int, token: int, finished: bool = False) -> None:
     for i, s in enumerate(self.running):
@@ -159,33 +286,40 @@ class Engine:
           self.pool.release(s)
           self.running.pop(i)
           self.finished[s.seq_id] = s
+          self.drafts.pop(s.seq_id, None)
         return
     raise KeyError(f"sequence {seq_id} is not running")
 
   # ------------------------------------------------------------------ conveniences
   def generate(self, prompts: Iterable[Seq[int]], *, max_new_tokens: int = 64, stop_tokens: Iterable[int] = (),
                temperature: float = 0.0, top_k: int = 0, generator: Optional[torch.Generator] = None,
-               on_token: Optional[Callable[[int, int], None]] = None) -> List[List[int]]:
-    """Greedy (temperature 0) or top-k sampled completions, in the order of ``prompts``."""
+               on_token: Optional[Callable[[int, int], None]] = None, draft_tokens: int = 0) -> List[List[int]]:
+    """Greedy (temperature 0) or top-k sampled completions, in the order of ``prompts``.  ``draft_tokens``: tokens that every
+    sequence may look up in its own text and have scored in one step (see the module's first lines)."""
+    if draft_tokens < 0:
+      raise ValueError("draft_tokens must not be negative")
     stop = set(int(t) for t in stop_tokens)
     order = [self.add(p, max_new_tokens) for p in prompts]
     while not self.idle:
-      res = self.step()
-      if res is None:
-        break
-      logits, ids = res
-      if temperature <= 0:
-        nxt = logits.argmax(-1)
+      if draft_tokens > 0:
+        moved = self.step_drafts(draft_tokens, temperature=temperature, top_k=top_k, generator=generator)
+        if moved is None:
+          break
       else:
-        lg = logits / temperature
-        if top_k > 0:
-          kth = lg.topk(min(top_k, lg.size(-1)), dim=-1).values[:, -1:]
-          lg = lg.masked_fill(lg < kth, float("-inf"))
-        nxt = torch.multinomial(torch.softmax(lg, -1), 1, generator=generator).squeeze(-1)
-      for sid, tok in zip(ids, nxt.tolist()):
-        if on_token is not None:
-          on_token(sid, tok)
-        self.update(sid, tok, finished=tok in stop)
+        res = self.step()
+        if res is None:
+          break
+        logits, ids = res
+        probs = self._probs(logits, temperature, top_k)
+        nxt = logits.argmax(-1) if probs is None else torch.multinomial(probs, 1, generator=generator).squeeze(-1)
+        moved = [(sid, [tok]) for sid, tok in zip(ids, nxt.tolist())]
+      for sid, toks in moved:
+        for tok in toks:
+          if on_token is not None:
+            on_token(sid, tok)
+          self.update(sid, tok, finished=tok in stop)
+          if sid in self.finished:                    # what was drafted behind the end is dropped
+            break
     return [self.finished[sid].tokens[self.finished[sid].prompt_len:] for sid in order]
 
   @torch.inference_mode()

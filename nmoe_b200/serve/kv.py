@@ -154,6 +154,16 @@ class BlockPool:
       seq.block_table.append(bid)
     return seq.block_table[bi] * self.block_size + pos % self.block_size
 
+  def reserve(self, seq: Sequence, n_extra: int) -> int:
+    """Blocks for up to ``n_extra`` tokens behind the last one (whose own slot exists); returns how many tokens fit without
+    taking from other sequences.  Blocks that stay unused hold the sequence's next tokens."""
+    last = len(seq) - 1
+    while (last + n_extra) // self.block_size >= len(seq.block_table) and self.free:
+      bid = self._take()
+      self.ref[bid] = 1
+      seq.block_table.append(bid)
+    return min(n_extra, len(seq.block_table) * self.block_size - 1 - last)
+
   def slot(self, seq: Sequence, pos: int) -> int:
     return seq.block_table[pos // self.block_size] * self.block_size + pos % self.block_size
 

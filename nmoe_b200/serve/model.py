@@ -1,15 +1,18 @@
 """The grading / rephrasing model of the curation stack: a gpt-oss-shaped decoder (GQA attention
 with learned sinks, sliding window on even layers, YaRN rotary; top-k MoE MLP with biases and a
-clamped SwiGLU) with the two execution modes a serving engine needs:
+clamped SwiGLU) with the execution modes a serving engine needs:
 
   prefill   whole (padded) prompts, K/V written to the paged cache as they are produced
-  decode    one token per running sequence, attention over the paged cache
+  decode    one token per running sequence, attention over the paged cache; a prefix that the whole
+            batch shares is attended to once
+  extend    a few tokens per running sequence (its last one and drafted ones), rows packed
 
 and hidden-state taps for the probe / judge heads (``return_hidden_states`` / ``up_to_layer`` /
 ``from_layer``: early exit and resume between layers).
 
-CUDA path: dense projections and prefill attention on the tcgen05 kernels of this package, decode
-attention and the cache scatter in ``csrc/paged_attention.cu``, experts on the block-scaled
+CUDA path: dense projections and attention on the tcgen05 kernels of this package, rotary and cache
+append in one pass (``csrc/rope_append.cu``), decode attention in ``csrc/paged_attention.cu``, attention
+of several tokens and of shared prefixes in ``csrc/paged_extend.cu``, experts on the block-scaled
 grouped GEMM (tokens are placed and quantised to MXFP8 by the RDEP placement kernel; expert
 weights ship as MXFP4 in the checkpoint and are widened once, exactly, to E4M3 with the same E8M0
 scales).  CPU tensors run the same maths in plain PyTorch.
@@ -88,12 +91,25 @@ def clamped_swiglu(h: torch.Tensor, limit: float, alpha: float = 1.702) -> torch
 class CacheView:
   """What a forward pass needs to know about the paged cache for one step."""
 
-  def __init__(self, k_cache, v_cache, slots, *, block_tables=None, context_lens=None, prefix_lens=None, block_size=16):
+  def __init__(self, k_cache, v_cache, slots, *, block_tables=None, context_lens=None, prefix_lens=None, block_size=16,
+               q_starts=None, q_lens=None, max_q_len=None, shared_len=0):
     self.k_cache, self.v_cache = k_cache, v_cache          # [L, num_blocks, block_size, Hkv, D]
-    self.slots = slots                                      # prefill: [B, S] int32 (-1 = padding), decode: [B]
+    self.slots = slots                                      # prefill: [B, S] int32 (-1 = padding), decode: [B], extend: [N]
     self.block_tables, self.context_lens = block_tables, context_lens
     self.prefix_lens = prefix_lens                          # prefill: cached tokens per sequence (host list) or None
     self.block_size = block_size
+    self.q_starts, self.q_lens, self.max_q_len = q_starts, q_lens, max_q_len   # extend: rows of each sequence (int32 [B]), their most
+    self.shared_len = shared_len                            # decode: leading tokens whose blocks are the same in every table
+
+  def describe_prefill(self) -> None:
+    """Rows and contexts of a padded prefill batch in the packed form that ``paged_extend`` takes, once per step."""
+    if self.q_lens is None:
+      B, S = self.slots.shape
+      dev = self.slots.device
+      self.q_lens = (self.slots >= 0).sum(1, dtype=torch.int32)
+      self.q_starts = torch.arange(0, B * S, S, dtype=torch.int32, device=dev)
+      self.context_lens = self.q_lens + torch.tensor(self.prefix_lens, dtype=torch.int32).to(dev)
+      self.max_q_len = S
 
 
 class Attention(nn.Module):
@@ -110,44 +126,38 @@ class Attention(nn.Module):
     self.out_b = nn.Parameter(torch.zeros(cfg.hidden_size, dtype=dtype))
     self.sinks = nn.Parameter(torch.zeros(self.nq, dtype=dtype))
 
-  def _qkv(self, x, pos, rot):
+  def _qkv(self, x, pos, rot, cache: Optional[CacheView], need_kv: bool):
+    """Rotated q [N, Hq, D] and, with ``need_kv``, k and v [N, Hkv, D] of all rows of x; k and v are in the cache afterwards."""
     qkv = ops.linear(ops.rmsnorm(x, self.norm, self.cfg.rms_eps), self.qkv_w, self.qkv_b)
-    lead = x.shape[:-1]
+    qkv, pos = qkv.reshape(-1, qkv.size(-1)), pos.reshape(-1)
+    N = qkv.size(0)
+    if qkv.is_cuda:
+      kc, vc, slots = (None, None, None) if cache is None else (cache.k_cache[self.layer], cache.v_cache[self.layer], cache.slots.reshape(-1))
+      return sops.rope_append(qkv, pos, *rot, self.nq, self.nkv, kc, vc, slots, need_kv=need_kv)
     q, k, v = qkv.split([self.nq * self.d, self.nkv * self.d, self.nkv * self.d], dim=-1)
-    q = apply_rotary(q.reshape(*lead, self.nq, self.d), pos, *rot)
-    k = apply_rotary(k.reshape(*lead, self.nkv, self.d), pos, *rot)
-    return q, k, v.reshape(*lead, self.nkv, self.d)
+    q = apply_rotary(q.reshape(N, self.nq, self.d), pos, *rot)
+    k = apply_rotary(k.reshape(N, self.nkv, self.d), pos, *rot)
+    v = v.reshape(N, self.nkv, self.d)
+    if cache is not None:
+      sops.kv_store(k.contiguous(), v.contiguous(), cache.k_cache[self.layer], cache.v_cache[self.layer], cache.slots.reshape(-1))
+    return q, k, v
+
+  def _out(self, x, o):
+    return x + ops.linear(o.reshape(*x.shape[:-1], self.nq * self.d), self.out_w, self.out_b)
 
   def prefill(self, x, pos, rot, cache: Optional[CacheView]):
     """x [B,S,H]; positions [B,S] (absolute).  Sequences with a cached prefix attend to it through
-    keys/values gathered from the cache (their own rows are written first)."""
+    the pages of the cache (their own rows are written first)."""
     B, S, _ = x.shape
-    q, k, v = self._qkv(x, pos, rot)
-    if cache is not None:
-      sops.kv_store(k.reshape(B * S, self.nkv, self.d).contiguous(), v.reshape(B * S, self.nkv, self.d).contiguous(),
-                    cache.k_cache[self.layer], cache.v_cache[self.layer], cache.slots.reshape(-1))
     has_prefix = cache is not None and cache.prefix_lens is not None and any(p > 0 for p in cache.prefix_lens)
-    if not has_prefix:
-      o = self._dense_attention(q, k, v)
+    q, k, v = self._qkv(x, pos, rot, cache, need_kv=not has_prefix)
+    if has_prefix:
+      cache.describe_prefill()
+      o = sops.paged_extend(q, cache.k_cache[self.layer], cache.v_cache[self.layer], cache.block_tables, cache.context_lens,
+                            cache.q_starts, cache.q_lens, self.sinks, self.scale, self.window, max_q_len=cache.max_q_len)
     else:
-      o = torch.empty(B, S, self.nq, self.d, dtype=x.dtype, device=x.device)
-      for b in range(B):
-        p = int(cache.prefix_lens[b])
-        if p == 0:
-          o[b:b + 1] = self._dense_attention(q[b:b + 1], k[b:b + 1], v[b:b + 1])
-          continue
-        n = int((cache.slots[b] >= 0).sum())                  # new tokens of this sequence
-        tab = cache.block_tables[b].long()
-        idx = torch.arange(p, device=x.device)
-        slot = tab[idx // cache.block_size] * cache.block_size + idx % cache.block_size
-        kc = cache.k_cache[self.layer].view(-1, self.nkv, self.d)[slot]
-        vc = cache.v_cache[self.layer].view(-1, self.nkv, self.d)[slot]
-        qf = torch.cat((torch.zeros(p, self.nq, self.d, dtype=x.dtype, device=x.device), q[b, :n]), 0).unsqueeze(0)
-        kf = torch.cat((kc, k[b, :n]), 0).unsqueeze(0)
-        vf = torch.cat((vc, v[b, :n]), 0).unsqueeze(0)
-        o[b, :n] = self._dense_attention(qf, kf, vf)[0, p:]
-        o[b, n:] = 0
-    return x + ops.linear(o.reshape(B, S, self.nq * self.d), self.out_w, self.out_b)
+      o = self._dense_attention(q.view(B, S, self.nq, self.d), k.view(B, S, self.nkv, self.d), v.reshape(B, S, self.nkv, self.d))
+    return self._out(x, o)
 
   def _dense_attention(self, q, k, v):
     if q.is_cuda:
@@ -156,11 +166,21 @@ class Attention(nn.Module):
 
   def decode(self, x, pos, rot, cache: CacheView):
     """x [B,H]: one token per sequence."""
-    q, k, v = self._qkv(x, pos, rot)
-    sops.kv_store(k.contiguous(), v.contiguous(), cache.k_cache[self.layer], cache.v_cache[self.layer], cache.slots)
-    o = sops.paged_decode(q, cache.k_cache[self.layer], cache.v_cache[self.layer], cache.block_tables,
-                          cache.context_lens, self.sinks, self.scale, self.window)
-    return x + ops.linear(o.reshape(x.size(0), self.nq * self.d), self.out_w, self.out_b)
+    q, _, _ = self._qkv(x, pos, rot, cache, need_kv=False)
+    kc, vc = cache.k_cache[self.layer], cache.v_cache[self.layer]
+    if cache.shared_len > 0 and self.window == 0:             # a window rarely reaches back into the shared part
+      o = sops.shared_prefix_decode(q, kc, vc, cache.block_tables, cache.context_lens, cache.shared_len, self.sinks, self.scale)
+    else:
+      o = sops.paged_decode(q, kc, vc, cache.block_tables, cache.context_lens, self.sinks, self.scale, self.window)
+    return self._out(x, o)
+
+  def extend(self, x, pos, rot, cache: CacheView):
+    """x [N,H]: cache.q_lens[b] tokens of each sequence from row cache.q_starts[b] on; every row belongs to a sequence."""
+    q, _, _ = self._qkv(x, pos, rot, cache, need_kv=False)
+    o = sops.paged_extend(q, cache.k_cache[self.layer], cache.v_cache[self.layer], cache.block_tables, cache.context_lens,
+                          cache.q_starts, cache.q_lens, self.sinks, self.scale, self.window, max_q_len=cache.max_q_len,
+                          out=torch.empty_like(q))
+    return self._out(x, o)
 
 
 class MoEMLP(nn.Module):
@@ -279,7 +299,8 @@ class Transformer(nn.Module):
   def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, *, cache: Optional[CacheView] = None,
               is_prefill: bool = True, return_hidden_states: bool = False, up_to_layer: Optional[int] = None,
               from_layer: Optional[int] = None, hidden_in: Optional[torch.Tensor] = None, no_logits: bool = False):
-    """prefill: input_ids / positions [B,S]; decode: [B].  ``from_layer`` resumes from ``hidden_in``
+    """prefill: input_ids / positions [B,S]; decode: [B]; extend (a cache view with q_lens, not is_prefill): [N] packed rows,
+    logits for each.  ``from_layer`` resumes from ``hidden_in``
     (the state returned by an earlier call that stopped at ``up_to_layer``).  Returns logits (fp32),
     or (logits | None, {layer: hidden}) with ``return_hidden_states``; a call that stops before the
     last layer returns its final hidden state under key ``up_to_layer``."""
@@ -289,8 +310,9 @@ class Transformer(nn.Module):
     x = hidden_in if (start > 0 and hidden_in is not None) else ops.embedding(input_ids, self.embed, 1.0)
     rot = (self.inv_freq, self.conc)
     taps: Dict[int, torch.Tensor] = {}
+    mode = "prefill" if is_prefill else "decode" if cache.q_lens is None else "extend"
     for i in range(start, stop):
-      x = self.attn[i].prefill(x, positions, rot, cache) if is_prefill else self.attn[i].decode(x, positions, rot, cache)
+      x = getattr(self.attn[i], mode)(x, positions, rot, cache)
       x = self.mlp[i](x)
       if return_hidden_states and (i + 1) in (self.cfg.probe_layer, self.cfg.judge_layer):
         taps[i + 1] = x.detach()

@@ -1,0 +1,103 @@
+"""Engine on CPU: drafted tokens and shared prefixes change how many steps a generation takes, not what it says."""
+import pytest
+import torch
+
+from nmoe_b200.serve import BlockPool, Engine, Sequence, ServeConfig, Transformer
+from nmoe_b200.serve.engine import LookupDraft
+
+
+@pytest.fixture(scope="module")
+def model():
+  torch.manual_seed(0)
+  cfg = ServeConfig(num_hidden_layers=3, num_experts=4, experts_per_token=2, vocab_size=64, hidden_size=64, intermediate_size=64,
+                    head_dim=16, num_attention_heads=4, num_key_value_heads=2, sliding_window=8, initial_context_length=64,
+                    rope_scaling_factor=1.0, probe_layer=2, judge_layer=3)
+  m = Transformer(cfg, dtype=torch.float32)
+  m.init_weights(std=0.2)
+  return m
+
+
+PROMPTS = [[3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8] * 2 + t for t in ([7, 7], [10, 11, 12, 13, 14], [3, 1, 4, 1])] + [[20, 21, 22]]
+
+
+def test_lookup_proposes_what_followed():
+  d = LookupDraft()
+  t = [1, 2, 3, 4, 9, 1, 2, 3]
+  assert d.propose(t, 4) == [4, 9, 1, 2] and d.propose(t, 1) == [4]
+  assert d.propose(t + [8], 4) == []                           # nothing like (2, 3, 8) or (3, 8) before
+  assert d.propose(t + [8, 2, 3], 5) == [8, 2, 3]              # the pair (2, 3), its latest place: index 7, then 8
+  assert LookupDraft().propose([5], 3) == [] and LookupDraft().propose([5, 5, 5], 3) == [5]
+
+
+def test_reserve_takes_only_free_blocks():
+  pool = BlockPool(num_blocks=4, block_size=4)
+  a, b = Sequence([1, 2, 3, 4, 5]), Sequence([6])
+  pool.allocate(a)
+  pool.allocate(b)
+  assert pool.reserve(a, 2) == 2 and len(a.block_table) == 2   # fits its own block
+  assert pool.reserve(a, 20) == 7 and len(a.block_table) == 3 and pool.n_free == 0
+  assert pool.reserve(b, 9) == 3
+  pool.release(a)
+  pool.release(b)
+  assert pool.n_free == 4
+
+
+@pytest.mark.parametrize("k", [1, 3, 7])
+@pytest.mark.parametrize("num_blocks", [None, 22])
+def test_drafts_leave_greedy_output_as_it_is(model, k, num_blocks):
+  plain = Engine(model, max_seq_len=80, max_batch=3, block_size=4).generate(PROMPTS, max_new_tokens=30, stop_tokens=[60])
+  eng = Engine(model, max_seq_len=80, max_batch=3, block_size=4, num_blocks=num_blocks)
+  seen = []
+  out = eng.generate(PROMPTS, max_new_tokens=30, stop_tokens=[60], draft_tokens=k, on_token=lambda sid, t: seen.append(t))
+  assert out == plain
+  assert eng.steps["drafted"] > 0 and 0 < eng.steps["accepted"] <= eng.steps["drafted"]
+  assert eng.pool.n_free == eng.num_blocks and not eng.drafts
+  # a stop token ends a sequence where it stands: what was drafted behind it is not handed out
+  assert len(seen) == sum(len(o) for o in out) + sum(1 for o in out if len(o) < 30)
+
+
+def test_drafts_save_steps(model, monkeypatch):
+  """With the right continuation proposed every time, 61 tokens take one prefill and ceil(60 / 5) steps."""
+  plain = Engine(model, max_seq_len=200, max_batch=4, block_size=4).generate(PROMPTS, max_new_tokens=61)
+  full = [p + o for p, o in zip(PROMPTS, plain)]
+  monkeypatch.setattr(LookupDraft, "propose", lambda self, t, k: next(f for f in full if f[:len(t)] == t)[len(t):len(t) + k])
+  eng = Engine(model, max_seq_len=200, max_batch=4, block_size=4)
+  assert eng.generate(PROMPTS, max_new_tokens=61, draft_tokens=4) == plain
+  assert eng.steps["decode"] == 12 and eng.steps["accepted"] == eng.steps["drafted"] == 4 * 48
+
+
+def test_drafts_with_sampling(model):
+  """top_k = 1 leaves one token: sampling has to say what greedy says.  With more, the same seed repeats itself."""
+  greedy = Engine(model, max_seq_len=80, max_batch=4, block_size=4).generate(PROMPTS, max_new_tokens=20)
+  run = lambda top_k, seed: Engine(model, max_seq_len=80, max_batch=4, block_size=4).generate(
+    PROMPTS, max_new_tokens=20, temperature=0.7, top_k=top_k, generator=torch.Generator().manual_seed(seed), draft_tokens=3)
+  assert run(1, 0) == greedy
+  assert run(8, 1) == run(8, 1) and run(8, 1) != run(8, 2)
+  assert all(len(o) == 20 for o in run(8, 3))
+
+
+def test_a_shared_prefix_is_found_and_changes_nothing(model, monkeypatch):
+  from nmoe_b200.serve import engine as E
+  from nmoe_b200.serve import ops as S
+  calls = []
+  inner = S.shared_prefix_decode
+  monkeypatch.setattr(S, "shared_prefix_decode", lambda q, k, v, t, c, n, *a: calls.append((len(q), n)) or inner(q, k, v, t, c, n, *a))
+  run = lambda: Engine(model, max_seq_len=80, max_batch=3, block_size=4).generate(PROMPTS[:3], max_new_tokens=10)
+  # the three are admitted together: none finds the other's blocks, so nothing is shared ...
+  monkeypatch.setattr(E, "MIN_SHARED_TOKENS", 4)
+  plain = run()
+  assert not calls
+  # ... until one has gone before
+  eng = Engine(model, max_seq_len=80, max_batch=3, block_size=4)
+  eng.generate(PROMPTS[:1], max_new_tokens=1)
+  assert eng.generate(PROMPTS[:3], max_new_tokens=10) == plain
+  assert calls and set(calls) == {(3, 24)}
+  calls.clear()
+  monkeypatch.setattr(E, "MIN_SHARED_TOKENS", 25)
+  eng.generate(PROMPTS[:3], max_new_tokens=10)
+  assert not calls
+
+
+def test_draft_arguments():
+  with pytest.raises(ValueError):
+    Engine.generate(None, [], draft_tokens=-1)

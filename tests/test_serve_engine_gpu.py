@@ -1,0 +1,92 @@
+"""The serving engine on the GPU with its operators together: append, shared prefix, drafted tokens, verification."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def models():
+  from nmoe_b200.serve import ServeConfig, Transformer
+  cfg = ServeConfig(num_hidden_layers=3, num_experts=8, experts_per_token=2, vocab_size=512, hidden_size=256, intermediate_size=160,
+                    head_dim=64, num_attention_heads=8, num_key_value_heads=2, sliding_window=16, initial_context_length=128,
+                    rope_scaling_factor=1.0, probe_layer=2, judge_layer=3)
+  mg = Transformer(cfg, dtype=torch.bfloat16, device=torch.device("cuda"), max_tokens=1024)
+  mg.init_weights(std=0.05)
+  mc = Transformer(cfg, dtype=torch.float32)
+  mc.load_state_dict({k: v.float().cpu() for k, v in mg.state_dict().items()})
+  yield mg, mc
+  mg.rdep.close()
+
+
+def _cos(a, b):
+  return torch.nn.functional.cosine_similarity(a.float().cpu().flatten(), b.float().cpu().flatten(), dim=0).item()
+
+
+def test_decode_behind_a_shared_prefix_tracks_the_fp32_model(models):
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.serve import Engine
+  mg, mc = models
+  g = torch.Generator().manual_seed(0)
+  rubric = torch.randint(0, 512, (150,), generator=g).tolist()
+  docs = [rubric + torch.randint(0, 512, (n,), generator=g).tolist() for n in (3, 40, 17, 90, 1)]
+  eg, ec = Engine(mg, max_seq_len=320, max_batch=8), Engine(mc, max_seq_len=320, max_batch=8)
+  for e in (eg, ec):                     # the rubric goes before, so that all five find its blocks
+    e.generate([rubric], max_new_tokens=1)
+    for d in docs:
+      e.add(d, 6)
+  lg, ids_g = eg.step()
+  lc, ids_c = ec.step()
+  assert eg.steps["cached_tokens"] == ec.steps["cached_tokens"] == 5 * 144
+  assert _cos(lg, lc) > 0.97
+  for _ in range(4):
+    for sg, sc, t in zip(ids_g, ids_c, lc.argmax(-1).tolist()):
+      eg.update(sg, t)
+      ec.update(sc, t)
+    lg, ids_g = eg.step()
+    lc, ids_c = ec.step()
+    assert _cos(lg, lc) > 0.95           # bf16 + MXFP8 experts vs fp32, a few near-tied routing decisions flip
+  G.check_status()
+
+
+def test_drafted_step_scores_like_single_steps(models):
+  """Logits of a packed step over drafted tokens against the fp32 model's one-token steps over the same tokens."""
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.serve import Engine
+  mg, mc = models
+  g = torch.Generator().manual_seed(1)
+  prompts = [torch.randint(0, 512, (n,), generator=g).tolist() * 2 for n in (9, 20, 33)]
+  eg, ec = Engine(mg, max_seq_len=160, max_batch=4), Engine(mc, max_seq_len=160, max_batch=4)
+  for e in (eg, ec):
+    for p in prompts:
+      e.add(p, 40)
+    e.step()
+    for s, p in zip(list(e.running), prompts):
+      e.update(s.seq_id, p[0])           # the text starts over: the lookup finds what follows
+  logits, tokens, cache, lens = eg._decode_drafts(list(eg.running), 3)
+  assert lens == [4, 4, 4] and tokens.tolist() == sum((p[:4] for p in prompts), [])
+  for j in range(4):
+    lc, ids = ec.step()
+    assert _cos(logits[j::4], lc) > 0.95
+    for sid, p in zip(ids, prompts):
+      ec.update(sid, p[j + 1])
+  G.check_status()
+
+
+@pytest.mark.parametrize("temperature,top_k", [(0.0, 0), (0.8, 0), (0.8, 5)])
+def test_generate_with_drafts_and_a_shared_rubric(models, temperature, top_k, monkeypatch):
+  """Whatever is proposed (here mostly nonsense, in numbers that change from step to step), generation goes through."""
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.serve import Engine
+  from nmoe_b200.serve.engine import LookupDraft
+  monkeypatch.setattr(LookupDraft, "propose", lambda self, t, k: [(7 * t[-1] + i) % 512 for i in range(min(k, len(t) % 5))])
+  mg, _ = models
+  g = torch.Generator().manual_seed(2)
+  rubric = torch.randint(0, 512, (100,), generator=g).tolist()
+  prompts = [rubric + rubric[b:b + 20] for b in range(6)]
+  eng = Engine(mg, max_seq_len=256, max_batch=4, num_blocks=48)          # two admission waves, blocks run short
+  gen = torch.Generator(device="cuda").manual_seed(3)
+  out = eng.generate(prompts, max_new_tokens=30, temperature=temperature, top_k=top_k, generator=gen, draft_tokens=4)
+  assert all(len(o) == 30 and all(0 <= t < 512 for t in o) for o in out)
+  assert eng.steps["drafted"] > 0 and eng.pool.n_free == eng.num_blocks
+  G.check_status()

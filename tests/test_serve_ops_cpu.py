@@ -100,3 +100,19 @@ def test_refusals():
               dict(out=torch.zeros(4)), dict(out=i32([0, 0]))):
     with pytest.raises(ValueError):
       S.verify_draft(**{**ok, **bad})
+
+
+def test_status_record_made_in_inference_mode_can_be_reset():
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  dev = torch.device("cpu")
+  G._STATUS.pop(dev, None)
+  try:
+    with torch.inference_mode():
+      G.status_buffer(dev)
+    G.status_buffer(dev)[0] = 2
+    with pytest.raises(NativeLibraryError, match="code=2"):
+      G.check_status(dev)
+    G.check_status(dev)
+  finally:
+    G._STATUS.pop(dev, None)
