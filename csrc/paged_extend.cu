@@ -67,6 +67,17 @@ NMOE_DEVICE bool px_wait(uint64_t* bar, uint32_t parity, volatile int* abort_fla
   }
   return true;
 }
+NMOE_DEVICE bool px_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 NMOE_DEVICE void px_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -87,6 +98,28 @@ NMOE_DEVICE float px_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// three-input maximum and two fp32 operations per instruction (sm_100)
+NMOE_DEVICE float px_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+NMOE_DEVICE uint64_t px_pack(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+NMOE_DEVICE void px_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+NMOE_DEVICE uint64_t px_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+NMOE_DEVICE uint64_t px_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 NMOE_DEVICE void px_cp16(uint32_t dst, const void* src, uint32_t bytes) {      // bytes 0: the 16 bytes become zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -119,7 +152,7 @@ __global__ void __launch_bounds__(PxSmem<D, TILES>::kThreads, (D == 64 && TILES 
 k_paged_extend(const ExtendParams p) {
   using SM = PxSmem<D, TILES>;
   constexpr int kStages = SM::kStages;
-  constexpr int kLag = kStages - 2;          // see the loader
+  constexpr int kLag = 2;                    // see the loader
   constexpr int kRows = TILES * PX_BM;
   constexpr int kThreads = SM::kThreads;
   constexpr int kMmaWarp = 4 * TILES;
@@ -243,53 +276,62 @@ k_paged_extend(const ExtendParams p) {
   float m = -1e30f, l = 0.f;
   if (warp > kMmaWarp) {
     // ------------------------------------------------------------ loaders: K and V rows of a block from their pages
-    // A stage is announced kLag blocks after it was asked for.  kLag <= kStages - 2: block i + 1 must be announced
-    // before block i is released (S of i + 1 is issued before P V of i), so asking for block i + kStages must not
-    // come before announcing block i + 1.
-    constexpr int kChunks = D / 8, kRowsPass = SM::kLoaders / kChunks, kPasses = PX_BN / kRowsPass;
-    const int tid = threadIdx.x - (kMmaWarp + 1) * 32;
-    const int c = tid % kChunks, r0 = tid / kChunks;
+    // Blocks are announced in order once they have landed: normally kLag blocks after they were asked for, all at once
+    // when the ring is full, since the block that would make room may be waiting for one of them.
+    // Each warp owns kRowsWarp keys of a block; a lane looks one of them up (a block ahead, so that the page table's
+    // latency is covered) and the warp shares the addresses by shuffle: a lookup per copied piece took 2500 cycles a block.
+    constexpr int kChunks = D / 8, kRowsWarp = PX_BN / (SM::kLoaders / 32), kRowsPass = 32 / kChunks;
+    static_assert(kRowsWarp <= 32 && kRowsWarp % kRowsPass == 0, "one lookup per lane");
+    const int lw = warp - kMmaWarp - 1;
+    const int c = lane % kChunks, rp = lane / kChunks;
     const long long row_elems = static_cast<long long>(p.hkv) * D;
-    const long long col = static_cast<long long>(hk) * D + c * 8;
+    const long long head_off = static_cast<long long>(hk) * D;
+    auto look_up = [&](int i) -> long long {                     // element offset of this lane's key in block i, -1: zeros
+      const int key = key0 + i * PX_BN + lw * kRowsWarp + lane;
+      if (lane >= kRowsWarp || i >= n_blk || key >= k_end) return -1;
+      const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
+      const int page = __ldg(table + pi);
+      if (page < 0 || page >= p.num_blocks) return -2;
+      return (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + head_off;
+    };
+    long long next = look_up(0);
     bool bad = false;
+    int told = 0;                                                // blocks announced so far
+    auto announce = [&](int upto) {                              // this thread's copies of the blocks before upto have landed
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0)
+        for (int t = told; t < upto; ++t) mbar_arrive(&kv_full[t % kStages]);
+      told = upto;
+    };
     for (int i = 0; i < n_blk && ok; ++i) {
       const int st = i % kStages;
-      ok = px_wait(&kv_empty[st], ((i / kStages) & 1) ^ 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, 0); *abort_flag = 1; break; }
+      const uint32_t empty_ph = ((i / kStages) & 1) ^ 1;
+      if (!__all_sync(0xffffffffu, px_test(&kv_empty[st], empty_ph))) {
+        if (told < i) { px_cp_wait<0>(); announce(i); }
+        ok = px_wait(&kv_empty[st], empty_ph, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, 0); *abort_flag = 1; break; }
+      }
       const uint32_t kd = smem_u32(sKV + st * SM::kStage), vd = kd + SM::kKV;
+      const long long mine = next;
+      bad = bad || mine == -2;
+      next = look_up(i + 1);
 #pragma unroll
-      for (int s = 0; s < kPasses; ++s) {
-        const int r = r0 + s * kRowsPass, key = key0 + i * PX_BN + r;
-        long long at = 0;
-        uint32_t bytes = 0;
-        if (key < k_end) {
-          const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
-          const int page = __ldg(table + pi);
-          if (page >= 0 && page < p.num_blocks) {
-            at = (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + col;
-            bytes = 16;
-          } else {
-            bad = true;
-          }
-        }
+      for (int s = 0; s < kRowsWarp / kRowsPass; ++s) {
+        const int rw = s * kRowsPass + rp, r = lw * kRowsWarp + rw;
+        const long long at = __shfl_sync(0xffffffffu, mine, rw);
+        const uint32_t bytes = at >= 0 ? 16 : 0;
+        const long long from = at >= 0 ? at + c * 8 : 0;
         const uint32_t o = (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        px_cp16(kd + o, p.k_cache + at, bytes);
-        px_cp16(vd + o, p.v_cache + at, bytes);
+        px_cp16(kd + o, p.k_cache + from, bytes);
+        px_cp16(vd + o, p.v_cache + from, bytes);
       }
       px_cp_commit();
-      if (i >= kLag) {
-        px_cp_wait<kLag>();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[(i - kLag) % kStages]);
-      }
+      if (i - kLag >= told) { px_cp_wait<kLag>(); announce(i - kLag + 1); }
     }
     px_cp_wait<0>();
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (ok && lane == 0)
-      for (int i = max(0, n_blk - kLag); i < n_blk; ++i) mbar_arrive(&kv_full[i % kStages]);
+    if (ok && told < n_blk) announce(n_blk);
     if (bad) report_status(p.status, kStatusBadIndex, 1022, b, 0);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issue
@@ -300,16 +342,16 @@ k_paged_extend(const ExtendParams p) {
         const int st = i % kStages;
         if (!px_wait(&kv_full[st], (i / kStages) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1031, i, 0); *abort_flag = 1; return false; }
         tc_fence_after_sync();
-        const uint32_t ka = smem_u32(sKV + st * SM::kStage);
+        const uint64_t ka = make_smem_desc(smem_u32(sKV + st * SM::kStage), 0, 1024, kSwizzle128B);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
           if (t * PX_BM >= n_valid) continue;
-          const uint32_t qa = smem_u32(sQ + t * SM::kQTile);
+          const uint64_t qa = make_smem_desc(smem_u32(sQ + t * SM::kQTile), 0, 1024, kSwizzle128B);
           const uint32_t d = tmem_base + t * 128 + (i & 1) * PX_BN;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
-            mma_f16_ss(d, make_smem_desc(qa + (j >> 2) * (PX_BM * 128) + (j & 3) * 32, 0, 1024, kSwizzle128B),
-                       make_smem_desc(ka + (j >> 2) * (PX_BN * 128) + (j & 3) * 32, 0, 1024, kSwizzle128B), idesc_s, j != 0 ? 1u : 0u);
+            mma_f16_ss(d, qa + (((j >> 2) * (PX_BM * 128) + (j & 3) * 32) >> 4), ka + (((j >> 2) * (PX_BN * 128) + (j & 3) * 32) >> 4),
+                       idesc_s, j != 0 ? 1u : 0u);
           mma_commit(&s_full[t * 2 + (i & 1)]);
         }
         return true;
@@ -318,7 +360,7 @@ k_paged_extend(const ExtendParams p) {
       for (int i = 0; good && i < n_blk; ++i) {
         if (i + 1 < n_blk) { good = issue_s(i + 1); if (!good) break; }
         const int st = i % kStages;
-        const uint32_t va = smem_u32(sKV + st * SM::kStage + SM::kKV);
+        const uint64_t va = make_smem_desc(smem_u32(sKV + st * SM::kStage + SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
           if (t * PX_BM >= n_valid) continue;
@@ -327,8 +369,7 @@ k_paged_extend(const ExtendParams p) {
           const uint32_t a_t = tmem_base + t * 128 + (i & 1) * PX_BN;
 #pragma unroll
           for (int j = 0; j < PX_BN / 16; ++j)
-            px_mma_ts(tmem_base + kTmemO + t * D, a_t + j * 8, make_smem_desc(va + j * 2048, PX_BN * 128, 1024, kSwizzle128B),
-                      idesc_pv, (i | j) != 0 ? 1u : 0u);
+            px_mma_ts(tmem_base + kTmemO + t * D, a_t + j * 8, va + ((j * 2048) >> 4), idesc_pv, (i | j) != 0 ? 1u : 0u);
           mma_commit(i + 1 < n_blk ? &pv_done[t] : &o_full[t]);
         }
         mma_commit(&kv_empty[st]);
@@ -366,9 +407,11 @@ k_paged_extend(const ExtendParams p) {
         for (int t = 0; t < PX_BN; ++t)
           if (t < from || t >= to) r[t] = 0xff800000u;                       // -inf
       }
-      float mx = -INFINITY;
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains: one would be 64 latencies long
 #pragma unroll
-      for (int t = 0; t < PX_BN; ++t) mx = fmaxf(mx, __uint_as_float(r[t]));
+      for (int t = 0; t < PX_BN; t += 2)
+        mx4[(t >> 1) & 3] = px_max3(mx4[(t >> 1) & 3], __uint_as_float(r[t]), __uint_as_float(r[t + 1]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       const float m_cand = fmaxf(m, mx * p.scale_log2);
       bool grow = m_cand - m > kPxRescale;
       if (i == 0) { grow = false; m = m_cand; }
@@ -390,20 +433,24 @@ k_paged_extend(const ExtendParams p) {
         }
         tmem_st_wait();
       }
-      float rs = 0.f;
+      const uint64_t sc2 = px_pack(p.scale_log2, p.scale_log2), nm2 = px_pack(-m, -m);
+      uint64_t rs2[4] = {0, 0, 0, 0};                                        // pairs of partial sums, both halves 0.f
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         uint32_t pk[16];
 #pragma unroll
         for (int t = 0; t < 32; t += 2) {
-          const float p0 = px_exp2(fmaf(__uint_as_float(r[hf * 32 + t]), p.scale_log2, -m));
-          const float p1 = px_exp2(fmaf(__uint_as_float(r[hf * 32 + t + 1]), p.scale_log2, -m));
-          rs += p0 + p1;
+          float x0, x1;
+          px_unpack(px_fma2(px_pack(__uint_as_float(r[hf * 32 + t]), __uint_as_float(r[hf * 32 + t + 1])), sc2, nm2), x0, x1);
+          const float p0 = px_exp2(x0), p1 = px_exp2(x1);
+          rs2[(t >> 1) & 3] = px_add2(rs2[(t >> 1) & 3], px_pack(p0, p1));
           pk[t >> 1] = pack_bf16x2(p0, p1);
         }
         px_tmem_st_x16(s_addr + hf * 16, pk);
       }
-      l += rs;
+      float sa, sb;
+      px_unpack(px_add2(px_add2(rs2[0], rs2[1]), px_add2(rs2[2], rs2[3])), sa, sb);
+      l += sa + sb;
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
