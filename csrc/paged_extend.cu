@@ -42,11 +42,13 @@ struct ExtendParams {
   float *part_o, *part_ml;
   StatusRecord* status;
   long long q_stride, bt_stride;
-  int n_rows, n_seqs, hq, hkv, group, block_size, block_shift, num_blocks, max_blocks, max_q_len, window, sinks_fp32;
+  int n_rows, n_seqs, hq, hkv, group, block_size, block_shift, num_blocks, capacity, max_q_len, window, sinks_fp32;
   int key_begin, key_end;             // only keys in [key_begin, key_end) count here
   int flat;                           // 1: the tokens of all sequences are one list that reads the first sequence's pages
-  int splits;                         // CTAs of a cluster = splits of the keys
-  int part_mode;                      // 0 none, 1 write partial results, 2 join those of the launch before
+  int splits, groups;                 // the keys of a row list are divided over groups x splits CTAs, splits = a cluster
+  int part_mode;                      // 0 none, 1 write partial results (one set per group), 2 join those of the launch before
+  int n_sets;                         // sets of partial results to join
+  long long set_rows;                 // rows of a set
   float scale_log2;
 };
 
@@ -130,6 +132,120 @@ NMOE_DEVICE void px_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) 
 NMOE_DEVICE void px_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 NMOE_DEVICE void px_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Rows of one list: its first row, its number of tokens (0 where the lengths are out of range) and its context.
+NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start, int& n, int& ctx) {
+  start = 0;
+  n = p.n_seqs;
+  ctx = 0;
+  if (p.flat) return;
+  start = p.q_starts != nullptr ? p.q_starts[b] : b;
+  n = p.q_lens != nullptr ? p.q_lens[b] : 1;
+  ctx = p.context_lens[b];
+  if (start < 0 || n < 0 || start > p.n_rows || n > p.n_rows - start || n > p.max_q_len) {
+    if (speaker) report_status(p.status, kStatusBadIndex, 1020, b, start);
+    n = 0;
+  } else if (ctx > p.capacity) {
+    if (speaker) report_status(p.status, kStatusBadIndex, 1021, b, ctx);
+    ctx = p.capacity;
+  }
+}
+// Keys [lo, hi) that a token of the list sees.
+NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool speaker, int& lo, int& hi) {
+  int pos = ctx - n + tok;
+  if (p.flat) {
+    const int c = p.context_lens[tok];
+    if (c > p.capacity && speaker) report_status(p.status, kStatusBadIndex, 1021, tok, c);
+    pos = min(c, p.capacity) - 1;
+  }
+  lo = max(p.window > 0 ? max(0, pos - p.window + 1) : 0, p.key_begin);
+  hi = min(pos + 1, p.key_end);
+}
+NMOE_DEVICE float px_sink(const ExtendParams& p, int h) {         // log2 units
+  if (p.sinks == nullptr) return -INFINITY;
+  return 1.4426950408889634f * (p.sinks_fp32 ? static_cast<const float*>(p.sinks)[h]
+                                             : __bfloat162float(static_cast<const __nv_bfloat16*>(p.sinks)[h]));
+}
+
+// Sum of (m, l, O) pieces relative to a common maximum, 8 columns a thread.
+struct PxSum {
+  float top, sum, acc[8];
+  NMOE_DEVICE void start(float t) {
+    top = t;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  }
+  NMOE_DEVICE void add(float2 ml, float4 a, float4 d) {
+    const float w = px_exp2(ml.x - top);
+    sum += w * ml.y;
+    acc[0] += w * a.x; acc[1] += w * a.y; acc[2] += w * a.z; acc[3] += w * a.w;
+    acc[4] += w * d.x; acc[5] += w * d.y; acc[6] += w * d.z; acc[7] += w * d.w;
+  }
+  NMOE_DEVICE void store(__nv_bfloat16* dst, float sink) const {
+    const float f = sum > 0.f ? 1.f / (sum + px_exp2(sink - top)) : 0.f;
+    int4 v;
+    uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vv[e] = pack_bf16x2(acc[2 * e] * f, acc[2 * e + 1] * f);
+    *reinterpret_cast<int4*>(dst) = v;
+  }
+};
+
+// Joins what the CTAs of a cluster hold for the rows row0 .. row0 + n_valid (sx [rows][D] fp32 in 16-byte pieces swizzled
+// by row, s_ml [rows][2]) and, in part_mode 2, the sets of the launch before.  Every CTA takes a run of the rows.
+template <int D, int kThreads>
+NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int start, int row0, int n_valid, int hk, int unit) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int splits = p.splits, rank = unit % splits, group = unit / splits, g = p.group;
+  if (splits > 1) cl.sync();
+  else __syncthreads();
+  if (p.part_mode == 2) px_wait_prior_grid();
+  const int per = (n_valid + splits - 1) / splits;
+  const int ra = rank * per, rb = min(n_valid, ra + per);
+  for (int i = threadIdx.x; i < (rb - ra) * (D / 8); i += kThreads) {
+    const int r = ra + i / (D / 8), c = i % (D / 8);
+    const int rr = row0 + r, tok = rr / g, h = hk * g + rr - tok * g;
+    const long long row = static_cast<long long>(start + tok) * p.hq + h;
+    const float sink = p.part_mode == 1 ? -INFINITY : px_sink(p, h);
+    float mm = -1e30f;
+    for (int s = 0; s < splits; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(splits > 1 ? cl.map_shared_rank(s_ml + 2 * r, s) : s_ml + 2 * r);
+      if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+    }
+    if (p.part_mode == 2)
+      for (int s = 0; s < p.n_sets; ++s) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
+        if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+      }
+    PxSum t;
+    t.start(fmaxf(mm, sink));
+    for (int s = 0; s < splits; ++s) {
+      const float* xr = sx + r * D;
+      const float* mr = s_ml + 2 * r;
+      if (splits > 1) { xr = cl.map_shared_rank(xr, s); mr = cl.map_shared_rank(mr, s); }
+      const float2 ml = *reinterpret_cast<const float2*>(mr);
+      if (ml.y > 0.f)
+        t.add(ml, reinterpret_cast<const float4*>(xr)[(2 * c) ^ (r & 7)], reinterpret_cast<const float4*>(xr)[(2 * c + 1) ^ (r & 7)]);
+    }
+    if (p.part_mode == 2)
+      for (int s = 0; s < p.n_sets; ++s) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
+        const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
+        if (ml.y > 0.f) t.add(ml, __ldcg(o), __ldcg(o + 1));
+      }
+    if (p.part_mode == 1) {
+      const long long at = group * p.set_rows + row;
+      float4* o = reinterpret_cast<float4*>(p.part_o + at * D) + 2 * c;
+      o[0] = make_float4(t.acc[0], t.acc[1], t.acc[2], t.acc[3]);
+      o[1] = make_float4(t.acc[4], t.acc[5], t.acc[6], t.acc[7]);
+      if (c == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(t.top, t.sum);
+    } else {
+      t.store(p.out + row * D + c * 8, sink);
+    }
+  }
+  if (splits > 1) cl.sync();                                     // nobody leaves while its rows may still be read
+}
+
 // Layout of shared memory.  D = 64: 4 stages of 16 KB, with one row tile two CTAs fit an SM; D = 128: 32 KB stages,
 // one CTA an SM.  The exchange of partial results reuses the stages (O as fp32, 16-byte pieces swizzled by row).
 template <int D, int TILES>
@@ -174,34 +290,17 @@ k_paged_extend(const ExtendParams p) {
   int* s_range = reinterpret_cast<int*>(tmem_slot + 2);          // [2] first key, end of keys
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = p.splits, rank = static_cast<int>(blockIdx.x) % splits;
-  const int n_tiles_x = static_cast<int>(gridDim.x) / splits;
+  // the keys are divided over units = groups x splits CTAs, the splits of a group being a cluster
+  const int units = p.splits * p.groups, unit = static_cast<int>(blockIdx.x) % units;
+  const int n_tiles_x = static_cast<int>(gridDim.x) / units;
   // tiles with the longest contexts (the last ones of a prompt) first: better tail
-  const int tile_x = n_tiles_x - 1 - static_cast<int>(blockIdx.x) / splits;
+  const int tile_x = n_tiles_x - 1 - static_cast<int>(blockIdx.x) / units;
   const int hk = blockIdx.y, b = p.flat ? 0 : blockIdx.z, g = p.group;
 
-  // ---------------------------------------------------------------- what this CTA works on
-  int start, n, ctx = 0;
-  const int capacity = static_cast<int>(min(static_cast<long long>(p.max_blocks) * p.block_size, 0x7fffffffll));
-  const bool speaker = tile_x == 0 && rank == 0 && hk == 0 && threadIdx.x == 0;
-  bool live = true;
-  if (p.flat) {
-    start = 0;
-    n = p.n_seqs;
-  } else {
-    start = p.q_starts != nullptr ? p.q_starts[b] : b;
-    n = p.q_lens != nullptr ? p.q_lens[b] : 1;
-    ctx = p.context_lens[b];
-    if (start < 0 || n < 0 || start > p.n_rows || n > p.n_rows - start || n > p.max_q_len) {
-      if (speaker) report_status(p.status, kStatusBadIndex, 1020, b, start);
-      live = false;
-    } else if (ctx > capacity) {
-      if (speaker) report_status(p.status, kStatusBadIndex, 1021, b, ctx);
-      ctx = capacity;
-    }
-  }
+  int start, n, ctx;
+  px_list(p, b, tile_x == 0 && unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
   const int row0 = tile_x * kRows;                               // first row of this CTA's tiles
-  const int n_valid = live ? min(kRows, n * g - row0) : 0;       // rows that exist
+  const int n_valid = min(kRows, n * g - row0);                  // rows that exist
   if (n_valid <= 0) {                                            // uniform over the cluster
     if (p.part_mode == 1) px_launch_dependents();
     if (p.part_mode == 2) px_wait_prior_grid();
@@ -249,17 +348,7 @@ k_paged_extend(const ExtendParams p) {
   int lo = 0, hi = 0;
   const int my_row = threadIdx.x;                                // softmax threads: row inside the CTA's tiles
   if (warp < 4 * TILES && my_row < n_valid) {
-    const int tok = (row0 + my_row) / g;
-    int pos;
-    if (p.flat) {
-      const int c = p.context_lens[tok];
-      if (c > capacity && hk == 0 && rank == 0 && (row0 + my_row) % g == 0) report_status(p.status, kStatusBadIndex, 1021, tok, c);
-      pos = min(c, capacity) - 1;
-    } else {
-      pos = ctx - n + tok;
-    }
-    lo = max(p.window > 0 ? max(0, pos - p.window + 1) : 0, p.key_begin);
-    hi = min(pos + 1, p.key_end);
+    px_bounds(p, (row0 + my_row) / g, n, ctx, hk == 0 && unit == 0 && (row0 + my_row) % g == 0, lo, hi);
     if (lo < hi) {
       atomicMin(&s_range[0], lo);
       atomicMax(&s_range[1], hi);
@@ -268,8 +357,8 @@ k_paged_extend(const ExtendParams p) {
   __syncthreads();
   const int k_begin = s_range[0], k_end = s_range[1];
   const int n_blocks_all = k_end > k_begin ? (k_end - k_begin + PX_BN - 1) / PX_BN : 0;
-  const int blk0 = static_cast<int>(static_cast<long long>(n_blocks_all) * rank / splits);
-  const int n_blk = static_cast<int>(static_cast<long long>(n_blocks_all) * (rank + 1) / splits) - blk0;
+  const int blk0 = static_cast<int>(static_cast<long long>(n_blocks_all) * unit / units);
+  const int n_blk = static_cast<int>(static_cast<long long>(n_blocks_all) * (unit + 1) / units) - blk0;
   const int key0 = n_blk > 0 ? k_begin + blk0 * PX_BN : 0;       // first key of this CTA
 
   bool ok = true;
@@ -471,14 +560,9 @@ k_paged_extend(const ExtendParams p) {
 
   // ---------------------------------------------------------------- results
   const bool softmax_warp = warp < 4 * TILES && (warp >> 2) * PX_BM + (warp & 3) * 32 < n_valid;
-  const bool direct = splits == 1 && p.part_mode == 0;
+  const bool direct = p.splits == 1 && p.part_mode == 0;
   float* sx = reinterpret_cast<float*>(sKV);                     // [kRows][D], 16-byte pieces swizzled by row
   float* s_ml = sx + kRows * D;                                  // [kRows][2]
-  auto sink_of = [&](int h) -> float {                           // log2 units
-    if (p.sinks == nullptr) return -INFINITY;
-    return 1.4426950408889634f * (p.sinks_fp32 ? static_cast<const float*>(p.sinks)[h]
-                                               : __bfloat162float(static_cast<const __nv_bfloat16*>(p.sinks)[h]));
-  };
   if (!direct) __syncthreads();                                  // every MMA of the CTA is done: the stages are free
   if (softmax_warp) {
     const uint32_t tmem_o = tmem_base + kTmemO + (warp >> 2) * D + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -486,7 +570,7 @@ k_paged_extend(const ExtendParams p) {
     __nv_bfloat16* orow = nullptr;
     if (direct && my_row < n_valid) {
       const int rr = row0 + my_row, tok = rr / g, h = hk * g + rr - tok * g;
-      const float sk = sink_of(h), mm = fmaxf(m, sk);
+      const float sk = px_sink(p, h), mm = fmaxf(m, sk);
       f = l > 0.f ? px_exp2(m - mm) / (l * px_exp2(m - mm) + px_exp2(sk - mm)) : 0.f;
       orow = p.out + (static_cast<long long>(start + tok) * p.hq + h) * D;
     }
@@ -530,78 +614,370 @@ k_paged_extend(const ExtendParams p) {
   }
   if (direct) return;
 
-  // join the splits (and the launch before): this CTA takes every splits-th run of rows, 8 columns a thread
-  cg::cluster_group cl = cg::this_cluster();
-  if (splits > 1) cl.sync();
-  if (p.part_mode == 2) px_wait_prior_grid();
-  const int per = (n_valid + splits - 1) / splits;
-  const int ra = rank * per, rb = min(n_valid, ra + per);
-  for (int i = threadIdx.x; i < (rb - ra) * (D / 8); i += kThreads) {
-    const int r = ra + i / (D / 8), c = i % (D / 8);
-    const int rr = row0 + r, tok = rr / g, h = hk * g + rr - tok * g;
-    const long long grow = static_cast<long long>(start + tok) * p.hq + h;
-    float mm = -1e30f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(splits > 1 ? cl.map_shared_rank(s_ml + 2 * r, s) : s_ml + 2 * r);
-      if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
-    }
-    float2 pm = make_float2(0.f, 0.f);
-    if (p.part_mode == 2) {
-      pm = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + grow);
-      if (pm.y > 0.f) mm = fmaxf(mm, pm.x);
-    }
-    const float sk = p.part_mode == 1 ? -INFINITY : sink_of(h);
-    const float top = fmaxf(mm, sk);
-    float acc[8], sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    auto add = [&](float4 a, float4 d, float w) {
-      acc[0] += w * a.x; acc[1] += w * a.y; acc[2] += w * a.z; acc[3] += w * a.w;
-      acc[4] += w * d.x; acc[5] += w * d.y; acc[6] += w * d.z; acc[7] += w * d.w;
-    };
-    for (int s = 0; s < splits; ++s) {
-      const float* xr = sx + r * D;
-      const float* mr = s_ml + 2 * r;
-      if (splits > 1) { xr = cl.map_shared_rank(xr, s); mr = cl.map_shared_rank(mr, s); }
-      const float2 ml = *reinterpret_cast<const float2*>(mr);
-      if (!(ml.y > 0.f)) continue;
-      const float w = px_exp2(ml.x - top);
-      sum += w * ml.y;
-      add(reinterpret_cast<const float4*>(xr)[(2 * c) ^ (r & 7)], reinterpret_cast<const float4*>(xr)[(2 * c + 1) ^ (r & 7)], w);
-    }
-    if (pm.y > 0.f) {
-      const float w = px_exp2(pm.x - top);
-      sum += w * pm.y;
-      const float4* o = reinterpret_cast<const float4*>(p.part_o + grow * D) + 2 * c;
-      add(__ldcg(o), __ldcg(o + 1), w);
-    }
-    if (p.part_mode == 1) {
-      float4* o = reinterpret_cast<float4*>(p.part_o + grow * D) + 2 * c;
-      o[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      o[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      if (c == 0) reinterpret_cast<float2*>(p.part_ml)[grow] = make_float2(top, sum);
-    } else {
-      const float f = sum > 0.f ? 1.f / (sum + px_exp2(sk - top)) : 0.f;
-      int4 v;
-      uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) vv[e] = pack_bf16x2(acc[2 * e] * f, acc[2 * e + 1] * f);
-      *reinterpret_cast<int4*>(p.out + grow * D + c * 8) = v;
-    }
-  }
-  if (splits > 1) cl.sync();                                     // nobody leaves while its rows may still be read
+  px_join<D, kThreads>(p, sx, s_ml, start, row0, n_valid, hk, unit);
 }
 
-template <int D, int TILES>
-static cudaError_t px_launch(const ExtendParams& p, int tiles, int z, cudaStream_t st) {
-  auto kern = k_paged_extend<D, TILES>;
+// ------------------------------------------------------------------------------------------------------------------
+// Few rows (up to 40): the same attention where a tile of 128 would be mostly empty, as in decode steps.  It is bound by
+// the bytes of K and V, so the matrix work goes where its results are easy to use: with keys as the rows of the warp-wide
+// mma and 8 query rows as its columns, S^T = K Q^T and O^T += V^T P^T waste nothing at 8 rows, every lane exponentiates
+// its own share (a tcgen05 tile gives a whole row of 64 keys to one lane: 1350 cycles a block for one busy warp), and no
+// barrier is needed.  Each of four warps streams its own tiles of 32 (D = 64) or 16 keys through three stages of 8 KB,
+// with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
+// movmatrix; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
+template <int D, int NT>
+struct PxFew {
+  static constexpr int kWarps = 4, kThreads = 128, kStages = 3;
+  static constexpr int kTile = 2048 / D;                   // keys per tile: K and V together are 8 KB
+  static constexpr int kKV = kTile * D * 2;
+  static constexpr int kRing = kStages * 2 * kKV;          // of a warp
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kOStride = D + 4;                   // floats; a warp leaves its O in its ring
+  static_assert(kRows * kOStride * 4 + kRows * 8 <= kRing, "O of a warp fits its ring");
+  static constexpr int kBytes = kWarps * kRing + kRows * (D + 2) * 4 + 128;
+};
+
+NMOE_DEVICE void px_ldm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+NMOE_DEVICE void px_ldm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+NMOE_DEVICE uint32_t px_transpose(uint32_t v) {            // of an 8x8 matrix of 16-bit values over the warp
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+NMOE_DEVICE void px_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
+  using F = PxFew<D, NT>;
+  constexpr int kTile = F::kTile, kStages = F::kStages, MT = kTile / 16, KS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  float* sx = reinterpret_cast<float*>(smem + F::kWarps * F::kRing);       // [rows][D], joined over the warps
+  float* s_ml = sx + F::kRows * D;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = p.splits * p.groups, unit = blockIdx.x, hk = blockIdx.y, b = p.flat ? 0 : blockIdx.z, g = p.group;
+  int start, n, ctx;
+  px_list(p, b, unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
+  const int n_valid = min(F::kRows, n * g);                      // the host launches this kernel only where all rows fit
+  if (n_valid <= 0) {                                            // uniform over the cluster
+    if (p.part_mode == 1) px_launch_dependents();
+    if (p.part_mode == 2) px_wait_prior_grid();
+    return;
+  }
+  if (p.part_mode == 1) px_launch_dependents();
+  const int* table = p.block_tables + b * p.bt_stride;
+
+  // keys of the list, and the bounds inside which no row needs a mask (every warp works them out)
+  int k_begin = 0x7fffffff, k_end = 0, w_lo = 0, w_hi = 0x7fffffff;
+  for (int r = lane; r < n_valid; r += 32) {
+    int lo, hi;
+    px_bounds(p, r / g, n, ctx, hk == 0 && unit == 0 && warp == 0 && r % g == 0, lo, hi);
+    w_lo = max(w_lo, lo);
+    w_hi = min(w_hi, hi);
+    if (lo < hi) { k_begin = min(k_begin, lo); k_end = max(k_end, hi); }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    k_begin = min(k_begin, __shfl_xor_sync(0xffffffffu, k_begin, o));
+    k_end = max(k_end, __shfl_xor_sync(0xffffffffu, k_end, o));
+    w_lo = max(w_lo, __shfl_xor_sync(0xffffffffu, w_lo, o));
+    w_hi = min(w_hi, __shfl_xor_sync(0xffffffffu, w_hi, o));
+  }
+  const int tiles_all = k_end > k_begin ? (k_end - k_begin + kTile - 1) / kTile : 0;
+  const int tile0 = static_cast<int>(static_cast<long long>(tiles_all) * unit / units);
+  const int n_tiles = static_cast<int>(static_cast<long long>(tiles_all) * (unit + 1) / units) - tile0;
+  const int n_mine = n_tiles > warp ? (n_tiles - warp + F::kWarps - 1) / F::kWarps : 0;      // tiles warp, warp + 4, ...
+  const int key0 = (tiles_all > 0 ? k_begin : 0) + (tile0 + warp) * kTile;
+
+  // loads: a lane looks one key up, the warp shares the addresses; a tile ahead, so that the lookup's latency is covered
+  constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
+  const uint32_t ring = smem_u32(smem + warp * F::kRing);
+  const long long row_elems = static_cast<long long>(p.hkv) * D, head_off = static_cast<long long>(hk) * D;
+  bool bad = false;
+  auto look_up = [&](int i) -> long long {
+    const int key = key0 + i * F::kWarps * kTile + lane;
+    if (lane >= kTile || i >= n_mine || key >= k_end) return -1;
+    const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
+    const int page = __ldg(table + pi);
+    if (page < 0 || page >= p.num_blocks) return -2;
+    return (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + head_off;
+  };
+  long long next = look_up(0);
+  auto load = [&](int i) {                                       // asks for tile i (past the last one: an empty group)
+    if (i < n_mine) {
+      const long long mine = next;
+      bad = bad || mine == -2;
+      next = look_up(i + 1);
+      const int c = lane % kChunks;
+      const uint32_t kd = ring + (i % kStages) * (2 * F::kKV);
+#pragma unroll
+      for (int s = 0; s < kTile / kRowsPass; ++s) {
+        const int r = s * kRowsPass + lane / kChunks;
+        const long long at = __shfl_sync(0xffffffffu, mine, r);
+        const uint32_t bytes = at >= 0 ? 16 : 0;
+        const long long from = at >= 0 ? at + c * 8 : 0;
+        const uint32_t o = r * (D * 2) + ((c ^ (r & 7)) << 4);
+        px_cp16(kd + o, p.k_cache + from, bytes);
+        px_cp16(kd + F::kKV + o, p.v_cache + from, bytes);
+      }
+    }
+    px_cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load(i);
+
+  // Q^T as B operands: column = row of the list, k = dims
+  uint32_t qf[KS][NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + (lane >> 2);
+    const bool in = r < n_valid;
+    const int tok = in ? r / g : 0, h = hk * g + (in ? r - tok * g : 0);
+    const __nv_bfloat16* src = p.q + (start + tok) * p.q_stride + static_cast<long long>(h) * D + (lane & 3) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[ks][nt][e] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8)) : 0u;
+  }
+
+  float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[ks][nt][e] = 0.f;
+    m[nt][0] = m[nt][1] = -1e30f;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
+  // rows that ldmatrix reads for this lane: K as stored, V transposed
+  const int kr = lane & 15, kc = lane >> 4;                      // key, 16-byte piece of the 16 dims
+  const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
+
+  for (int i = 0; i < n_mine; ++i) {
+    load(i + kStages - 1);
+    px_cp_wait<kStages - 1>();
+    __syncwarp();                                                // every lane's copies of tile i are there
+    const uint32_t ks_addr = ring + (i % kStages) * (2 * F::kKV), vs_addr = ks_addr + F::kKV;
+    float s[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[4];
+        const int r = mt * 16 + kr;
+        px_ldm(ks_addr + r * (D * 2) + (((ks * 2 + kc) ^ (r & 7)) << 4), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) px_mma(s[mt][nt], a, qf[ks][nt][0], qf[ks][nt][1]);
+      }
+    }
+    const int k0 = key0 + i * F::kWarps * kTile;
+    if (k0 < w_lo || k0 + kTile > w_hi) {
+#pragma unroll 1
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll 1
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + (lane & 3) * 2 + e;
+          int lo = 0, hi = 0;
+          if (r < n_valid) px_bounds(p, r / g, n, ctx, false, lo, hi);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const int ka = k0 + mt * 16 + (lane >> 2);
+#pragma unroll
+            for (int q = 0; q < NT; ++q)                         // constant indices: s stays in registers
+#pragma unroll
+              for (int f = 0; f < 2; ++f)
+                if (q == nt && f == e) {
+                  if (ka < lo || ka >= hi) s[mt][q][f] = -INFINITY;
+                  if (ka + 8 < lo || ka + 8 >= hi) s[mt][q][2 + f] = -INFINITY;
+                }
+          }
+        }
+    }
+    float mx[NT][2];
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+        if (MT == 2) v = px_max3(v, s[MT - 1][nt][e], s[MT - 1][nt][2 + e]);
+        mx[nt][e] = v * p.scale_log2;
+        grow = grow || mx[nt][e] > m[nt][e] + kPxRescale;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = mx[nt][e];
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, w));
+          const float up = fmaxf(m[nt][e], v), alpha = px_exp2(m[nt][e] - up);
+          m[nt][e] = up;
+          l[nt][e] *= alpha;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) { o[ks][nt][e] *= alpha; o[ks][nt][2 + e] *= alpha; }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float e4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) e4[e] = px_exp2(fmaf(s[mt][nt][e], p.scale_log2, -m[nt][e & 1]));
+        l[nt][0] += e4[0] + e4[2];
+        l[nt][1] += e4[1] + e4[3];
+        pf[nt][0] = px_transpose(pack_bf16x2(e4[0], e4[1]));
+        pf[nt][1] = px_transpose(pack_bf16x2(e4[2], e4[3]));
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[4];
+        const int r = mt * 16 + vr;
+        px_ldm_t(vs_addr + r * (D * 2) + (((ks * 2 + vc) ^ (r & 7)) << 4), a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) px_mma(o[ks][nt], a, pf[nt][0], pf[nt][1]);
+      }
+    }
+    __syncwarp();                                                // the stage may be filled again
+  }
+  px_cp_wait<0>();
+  if (bad) report_status(p.status, kStatusBadIndex, 1022, b, 0);
+  __syncwarp();
+
+  // every warp leaves its rows in its ring, the CTA joins them
+  float* wo = reinterpret_cast<float*>(smem + warp * F::kRing);
+  float* wml = wo + F::kRows * F::kOStride;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + (lane & 3) * 2 + e;
+      float v = l[nt][e];
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+      if (lane < 4) { wml[2 * r] = m[nt][e]; wml[2 * r + 1] = v; }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        wo[r * F::kOStride + ks * 16 + (lane >> 2)] = o[ks][nt][e];
+        wo[r * F::kOStride + ks * 16 + 8 + (lane >> 2)] = o[ks][nt][2 + e];
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_valid * (D / 8); i += F::kThreads) {
+    const int r = i / (D / 8), c = i % (D / 8);
+    float mm = -1e30f;
+    float2 ml[F::kWarps];
+#pragma unroll
+    for (int w = 0; w < F::kWarps; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(smem + w * F::kRing + F::kRows * F::kOStride * 4 + r * 8);
+      if (ml[w].y > 0.f) mm = fmaxf(mm, ml[w].x);
+    }
+    PxSum t;
+    t.start(mm);
+#pragma unroll
+    for (int w = 0; w < F::kWarps; ++w) {
+      const float4* src = reinterpret_cast<const float4*>(smem + w * F::kRing + (r * F::kOStride + c * 8) * 4);
+      if (ml[w].y > 0.f) t.add(ml[w], src[0], src[1]);
+    }
+    reinterpret_cast<float4*>(sx + r * D)[(2 * c) ^ (r & 7)] = make_float4(t.acc[0], t.acc[1], t.acc[2], t.acc[3]);
+    reinterpret_cast<float4*>(sx + r * D)[(2 * c + 1) ^ (r & 7)] = make_float4(t.acc[4], t.acc[5], t.acc[6], t.acc[7]);
+    if (c == 0) reinterpret_cast<float2*>(s_ml)[r] = make_float2(mm, t.sum);
+  }
+  px_join<D, F::kThreads>(p, sx, s_ml, start, 0, n_valid, hk, unit);
+}
+
+// Joins the sets of a launch that split the keys over several clusters; 8 columns a thread.
+template <int D>
+__global__ void __launch_bounds__(256) k_paged_join(const ExtendParams p) {
+  px_wait_prior_grid();
+  const int b = blockIdx.y;
+  int start, n, ctx;
+  px_list(p, b, false, start, n, ctx);
+  const int i = blockIdx.x * 256 + threadIdx.x, c = i % (D / 8), h = i / (D / 8) % p.hq, tok = i / (D / 8) / p.hq;
+  if (tok >= n) return;
+  const long long row = static_cast<long long>(start + tok) * p.hq + h;
+  const float sink = px_sink(p, h);
+  float mm = -1e30f;
+  for (int s = 0; s < p.n_sets; ++s) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
+    if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+  }
+  PxSum t;
+  t.start(fmaxf(mm, sink));
+  for (int s = 0; s < p.n_sets; ++s) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
+    const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
+    if (ml.y > 0.f) t.add(ml, __ldcg(o), __ldcg(o + 1));
+  }
+  t.store(p.out + row * D + c * 8, sink);
+}
+
+// How a call is cut: which kernel, tiles a list, CTAs the keys of a tile are split over.
+struct PxPlan {
+  int nt;                 // > 0: the kernel for few rows, 8 * nt of them
+  int tiles_cta;          // row tiles of a CTA (kernel for many rows)
+  long long tiles;
+  int splits, groups;
+};
+
+// `lists` row lists of up to `rows` rows that see at most `keys` keys each; groups only where partial sets may be written.
+static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys, bool may_group) {
+  PxPlan q;
+  const int few_most = D == 64 ? 40 : 32;
+  q.nt = 0;
+  q.tiles = 1;
+  q.tiles_cta = 1;
+  long long slots, least;                  // CTAs the GPU holds at once; keys that make a split worth while
+  if (rows <= few_most) {
+    const int t = static_cast<int>((rows + 7) / 8);
+    q.nt = D == 64 ? (t == 4 ? 5 : t) : (t == 3 ? 4 : t);
+    slots = 296;
+    least = 2 * 4 * (2048 / D);
+  } else {
+    // two tiles a CTA halve the K/V traffic; one tile spreads few rows over more SMs
+    const long long pairs = (rows + 2 * PX_BM - 1) / (2 * PX_BM);
+    q.tiles_cta = rows > PX_BM && pairs * lists * hkv >= 148 ? 2 : 1;
+    q.tiles = q.tiles_cta == 2 ? pairs : (rows + PX_BM - 1) / PX_BM;
+    slots = D == 64 && q.tiles_cta == 1 ? 296 : 148;
+    least = 4 * PX_BN;
+  }
+  const long long base = q.tiles * lists * hkv;
+  long long units = slots / (base > slots ? slots : base);
+  const long long worth = keys / least;
+  if (units > worth) units = worth;
+  if (units < 1) units = 1;
+  q.splits = 1;
+  while (q.splits < 8 && q.splits * 2 <= units) q.splits *= 2;
+  q.groups = may_group && units >= 2 * q.splits ? static_cast<int>(units / q.splits) : 1;
+  return q;
+}
+
+template <typename K>
+static cudaError_t px_launch(K kern, const ExtendParams& p, dim3 grid, int threads, int smem, bool dependent, cudaStream_t st) {
   // per device, so set at every launch (it only stores a number): a process may use several
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PxSmem<D, TILES>::kBytes);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.splits, p.hkv, z);
-  cfg.blockDim = dim3(PxSmem<D, TILES>::kThreads);
-  cfg.dynamicSmemBytes = PxSmem<D, TILES>::kBytes;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   int n = 0;
@@ -610,7 +986,7 @@ static cudaError_t px_launch(const ExtendParams& p, int tiles, int z, cudaStream
     at[n].val.clusterDim.x = p.splits; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (p.part_mode == 2) {
+  if (dependent) {
     at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -620,43 +996,90 @@ static cudaError_t px_launch(const ExtendParams& p, int tiles, int z, cudaStream
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-// Tiles, splits and launch for `lists` row lists of up to `rows` rows each that see at most `keys` keys.
-static int px_run(ExtendParams& p, int D, long long rows, int lists, long long keys, cudaStream_t st) {
-  // two tiles a CTA halve the K/V traffic; one tile spreads few rows over more SMs
-  const long long pairs = (rows + 2 * PX_BM - 1) / (2 * PX_BM);
-  const bool two = rows > PX_BM && pairs * lists * p.hkv >= 148;
-  const long long tiles = two ? pairs : (rows + PX_BM - 1) / PX_BM;
-  if (tiles > (1 << 20)) return -5;
-  // split the keys while SMs are free and every split keeps four blocks
-  const long long room = (D == 64 && !two) ? 296 : 148;
-  int splits = 1;
-  while (splits < 8 && tiles * lists * p.hkv * splits * 2 <= room && keys >= static_cast<long long>(splits) * 2 * 4 * PX_BN) splits *= 2;
-  p.splits = splits;
+template <int D, int NT>
+static cudaError_t px_few(const ExtendParams& p, dim3 grid, cudaStream_t st) {
+  return px_launch(k_paged_few<D, NT>, p, grid, PxFew<D, NT>::kThreads, PxFew<D, NT>::kBytes, p.part_mode == 2, st);
+}
+template <int D, int TILES>
+static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
+  return px_launch(k_paged_extend<D, TILES>, p, grid, PxSmem<D, TILES>::kThreads, PxSmem<D, TILES>::kBytes, p.part_mode == 2, st);
+}
+
+static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream_t st) {
+  if (q.tiles * q.splits * q.groups > 0x3fffffff) return -5;
+  p.splits = q.splits;
+  p.groups = q.groups;
+  const dim3 grid(static_cast<unsigned>(q.tiles) * q.splits * q.groups, p.hkv, lists);
   cudaError_t e;
-  if (D == 64) e = two ? px_launch<64, 2>(p, static_cast<int>(tiles), lists, st) : px_launch<64, 1>(p, static_cast<int>(tiles), lists, st);
-  else e = two ? px_launch<128, 2>(p, static_cast<int>(tiles), lists, st) : px_launch<128, 1>(p, static_cast<int>(tiles), lists, st);
+  if (D == 64) {
+    switch (q.nt) {
+      case 0: e = q.tiles_cta == 2 ? px_many<64, 2>(p, grid, st) : px_many<64, 1>(p, grid, st); break;
+      case 1: e = px_few<64, 1>(p, grid, st); break;
+      case 2: e = px_few<64, 2>(p, grid, st); break;
+      case 3: e = px_few<64, 3>(p, grid, st); break;
+      default: e = px_few<64, 5>(p, grid, st); break;
+    }
+  } else {
+    switch (q.nt) {
+      case 0: e = q.tiles_cta == 2 ? px_many<128, 2>(p, grid, st) : px_many<128, 1>(p, grid, st); break;
+      case 1: e = px_few<128, 1>(p, grid, st); break;
+      case 2: e = px_few<128, 2>(p, grid, st); break;
+      default: e = px_few<128, 4>(p, grid, st); break;
+    }
+  }
   return e == cudaSuccess ? 0 : static_cast<int>(e);
+}
+
+struct PxCall {
+  PxPlan first, second;      // second: each sequence's own keys behind a shared prefix
+};
+
+static PxCall px_call(int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int max_q_len, int window, int prefix_len) {
+  const long long capacity = static_cast<long long>(max_blocks) * block_size;
+  const int g = Hq / Hkv;
+  PxCall c;
+  if (prefix_len <= 0) {
+    const long long keys = window > 0 && window + static_cast<long long>(max_q_len) < capacity ? window + max_q_len : capacity;
+    c.first = c.second = px_plan(D, Hkv, static_cast<long long>(max_q_len) * g, B, keys, true);
+  } else {
+    const long long own = capacity - prefix_len;
+    c.first = px_plan(D, Hkv, static_cast<long long>(B) * g, 1, prefix_len, true);
+    c.second = px_plan(D, Hkv, g, B, window > 0 && window < own ? window : own, false);
+  }
+  return c;
 }
 
 }  // namespace nmoe
 
 using namespace nmoe;
 
+// Floats of workspace that nmoe_paged_extend needs for a call of these sizes (0: none).
+extern "C" long long nmoe_paged_extend_workspace(int n_rows, int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
+                                                 int max_q_len, int window, int prefix_len) {
+  if (Hkv < 1 || Hq < Hkv) return 0;
+  const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
+  if (prefix_len <= 0 && c.first.groups == 1) return 0;
+  return static_cast<long long>(c.first.groups) * n_rows * Hq * (D + 2);
+}
+
 // q [n_rows, Hq, D] (rows q_stride apart), out [n_rows, Hq, D]; caches [num_blocks, block_size, Hkv, D]; block_tables [B] rows
-// of max_blocks entries, bt_stride apart; context_lens, q_starts, q_lens [B].  prefix_len < 0: extend.  Otherwise one token
-// per sequence (q_starts, q_lens null) behind prefix_len common keys, with a workspace of n_rows * Hq * (D + 2) floats.
+// of max_blocks entries, bt_stride apart; context_lens, q_starts, q_lens [B].  prefix_len > 0: one token per sequence
+// (q_starts, q_lens null) behind that many common keys.  workspace: see above.
 extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* k_cache, const void* v_cache,
                                  const int* block_tables, long long bt_stride, const int* context_lens,
                                  const int* q_starts, const int* q_lens, const void* sinks, int sinks_fp32, void* out,
                                  int n_rows, int B, int Hq, int Hkv, int D, int block_size, int num_blocks, int max_blocks,
-                                 int max_q_len, int window, float scale, int prefix_len, float* workspace, void* status,
-                                 cudaStream_t st) {
+                                 int max_q_len, int window, float scale, int prefix_len, float* workspace,
+                                 long long workspace_floats, void* status, cudaStream_t st) {
   if (B == 0 || n_rows == 0 || max_q_len == 0) return 0;
   if (Hkv < 1 || Hkv > 65535 || Hq % Hkv != 0 || block_size < 1 || B < 0 || B > 65535 || !(scale > 0.f)) return -1;
   if (D != 64 && D != 128) return -2;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0 || (n_rows > 1 && q_stride % 8 != 0)) return -3;
-  if (static_cast<long long>(n_rows) * (Hq / Hkv) > 0x7fffffffll - 256) return -4;
+  if (static_cast<long long>(n_rows) * Hq > 0x7fffffffll / (D / 8) - 256) return -4;
+  if (prefix_len > 0 && (q_starts != nullptr || q_lens != nullptr)) return -5;
+  if (workspace_floats < nmoe_paged_extend_workspace(n_rows, B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len)) return -6;
+  const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
   ExtendParams p;
   p.q = static_cast<const __nv_bfloat16*>(q); p.k_cache = static_cast<const __nv_bfloat16*>(k_cache);
   p.v_cache = static_cast<const __nv_bfloat16*>(v_cache); p.out = static_cast<__nv_bfloat16*>(out);
@@ -666,19 +1089,31 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
   p.block_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (block_size == 1 << s) p.block_shift = s;
-  p.max_blocks = max_blocks; p.max_q_len = max_q_len; p.window = window; p.sinks_fp32 = sinks_fp32;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.part_o = workspace; p.part_ml = workspace ? workspace + static_cast<long long>(n_rows) * Hq * D : nullptr;
-  p.key_begin = 0; p.key_end = 0x7fffffff; p.flat = 0; p.part_mode = 0;
   const long long capacity = static_cast<long long>(max_blocks) * block_size;
-  long long keys = window > 0 && window + max_q_len < capacity ? window + max_q_len : capacity;
-  if (prefix_len <= 0) return px_run(p, D, static_cast<long long>(max_q_len) * p.group, B, keys, st);
-  if (workspace == nullptr || q_starts != nullptr || q_lens != nullptr) return -5;
+  p.capacity = static_cast<int>(capacity < 0x7fffff00ll ? capacity : 0x7fffff00ll);
+  p.max_q_len = max_q_len; p.window = window; p.sinks_fp32 = sinks_fp32;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.set_rows = static_cast<long long>(n_rows) * Hq;
+  p.n_sets = c.first.groups;
+  p.part_o = workspace;
+  p.part_ml = workspace != nullptr ? workspace + p.n_sets * p.set_rows * D : nullptr;
+  p.key_begin = 0; p.key_end = 0x7fffffff; p.flat = 0; p.part_mode = 0;
+  if (prefix_len <= 0) {
+    if (c.first.groups == 1) return px_run(p, c.first, D, B, st);
+    p.part_mode = 1;
+    const int rc = px_run(p, c.first, D, B, st);
+    if (rc != 0) return rc;
+    p.part_mode = 2;
+    p.splits = 1;
+    const long long pieces = static_cast<long long>(max_q_len) * Hq * (D / 8);
+    const dim3 grid(static_cast<unsigned>((pieces + 255) / 256), B);
+    const cudaError_t e = D == 64 ? px_launch(k_paged_join<64>, p, grid, 256, 0, true, st) : px_launch(k_paged_join<128>, p, grid, 256, 0, true, st);
+    return e == cudaSuccess ? 0 : static_cast<int>(e);
+  }
   ExtendParams f = p;
   f.flat = 1; f.part_mode = 1; f.key_end = prefix_len;
-  const int rc = px_run(f, D, static_cast<long long>(B) * p.group, 1, prefix_len, st);
+  const int rc = px_run(f, c.first, D, 1, st);
   if (rc != 0) return rc;
   p.part_mode = 2; p.key_begin = prefix_len;
-  keys = window > 0 && window < capacity - prefix_len ? window : capacity - prefix_len;
-  return px_run(p, D, p.group, B, keys, st);
+  return px_run(p, c.second, D, B, st);
 }

@@ -90,13 +90,13 @@ def _on(device: torch.device):
 _FN = {}
 
 
-def _fn(name: str, sig: str):
+def _fn(name: str, sig: str, result=ctypes.c_int):
   """C entry with its argument types set once (p pointer, i int, l long long, f float): plain numbers can be passed."""
   f = _FN.get(name)
   if f is None:
     f = getattr(L.lib(), name)
     f.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}[c] for c in sig]
-    f.restype = ctypes.c_int
+    f.restype = result
     _FN[name] = f
   return f
 
@@ -245,6 +245,21 @@ def _attention_args(q, k_cache, v_cache, block_tables, sinks):
   return q, sinks
 
 
+def _attend(what, q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, out, scale, window, max_q_len, prefix_len):
+  """The launch behind ``paged_extend`` and ``shared_prefix_decode`` (on q's device)."""
+  N, Hq, D = q.shape
+  sizes = N, context_lens.numel(), Hq, k_cache.size(2), D
+  need = _fn("nmoe_paged_extend_workspace", "iiiiiiiiii", ctypes.c_longlong)(
+    *sizes, k_cache.size(1), block_tables.size(1), max_q_len, window, prefix_len)
+  # partial results (O, m, l) where the keys of a row are split over more CTAs than exchange them directly
+  work = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+  L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifiplpp")(
+    _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), _p(q_starts),
+    _p(q_lens), _p(sinks), int(sinks is not None and sinks.dtype == torch.float32), _p(out), *sizes, k_cache.size(1), k_cache.size(0),
+    block_tables.size(1), max_q_len, window, scale, prefix_len, _p(work), need, _p(status_buffer(q.device)), _stream()),
+    what, 2 if need else 1)
+
+
 def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                  context_lens: torch.Tensor, q_starts: torch.Tensor, q_lens: torch.Tensor, sinks: Optional[torch.Tensor],
                  scale: float, window: int = 0, *, max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -272,11 +287,8 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   with _on(q.device):
     out = torch.zeros(N, Hq, D, dtype=q.dtype, device=q.device) if out is None else out
     _need(_aligned(out), "out must start on a 16-byte boundary")
-    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifippp")(
-      _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), _p(q_starts),
-      _p(q_lens), _p(sinks), int(sinks is not None and sinks.dtype == torch.float32), _p(out), N, B, Hq, k_cache.size(2), D,
-      k_cache.size(1), k_cache.size(0), block_tables.size(1), min(max_q_len, N), window, scale, 0, 0,
-      _p(status_buffer(q.device)), _stream()), "paged_extend")
+    _attend("paged_extend", q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, out, scale, window,
+            min(max_q_len, N), 0)
   return out
 
 
@@ -302,13 +314,8 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
   context_lens = context_lens.contiguous()
   with _on(q.device):
     out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    # (O, m, l) of every row over the prefix
-    work = torch.empty(B * Hq * (D + 2), dtype=torch.float32, device=q.device) if prefix_len > 0 else None
-    L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifippp")(
-      _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), 0, 0, _p(sinks),
-      int(sinks is not None and sinks.dtype == torch.float32), _p(out), B, B, Hq, k_cache.size(2), D, k_cache.size(1),
-      k_cache.size(0), block_tables.size(1), 1, window, scale, prefix_len, _p(work),
-      _p(status_buffer(q.device)), _stream()), "shared_prefix_decode", 2 if prefix_len > 0 else 1)
+    _attend("shared_prefix_decode", q, k_cache, v_cache, block_tables, context_lens, None, None, sinks, out, scale, window, 1,
+            prefix_len)
   return out
 
 
