@@ -22,6 +22,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common/ptx.cuh"
 
 namespace cg = cooperative_groups;
@@ -969,11 +971,17 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
   return q;
 }
 
-template <typename K>
-static cudaError_t px_launch(K kern, const ExtendParams& p, dim3 grid, int threads, int smem, bool dependent, cudaStream_t st) {
-  // per device, so set at every launch (it only stores a number): a process may use several
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <void (*kern)(ExtendParams)>
+static cudaError_t px_launch(const ExtendParams& p, dim3 grid, int threads, int smem, bool dependent, cudaStream_t st) {
+  static std::atomic<unsigned long long> ready{0};               // of this kernel: devices where its shared memory has been raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (smem > 0 && (dev > 63 || !((ready.load() >> dev) & 1))) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev <= 63) ready.fetch_or(1ull << dev);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -998,11 +1006,11 @@ static cudaError_t px_launch(K kern, const ExtendParams& p, dim3 grid, int threa
 
 template <int D, int NT>
 static cudaError_t px_few(const ExtendParams& p, dim3 grid, cudaStream_t st) {
-  return px_launch(k_paged_few<D, NT>, p, grid, PxFew<D, NT>::kThreads, PxFew<D, NT>::kBytes, p.part_mode == 2, st);
+  return px_launch<k_paged_few<D, NT>>(p, grid, PxFew<D, NT>::kThreads, PxFew<D, NT>::kBytes, p.part_mode == 2, st);
 }
 template <int D, int TILES>
 static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
-  return px_launch(k_paged_extend<D, TILES>, p, grid, PxSmem<D, TILES>::kThreads, PxSmem<D, TILES>::kBytes, p.part_mode == 2, st);
+  return px_launch<k_paged_extend<D, TILES>>(p, grid, PxSmem<D, TILES>::kThreads, PxSmem<D, TILES>::kBytes, p.part_mode == 2, st);
 }
 
 static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream_t st) {
@@ -1107,7 +1115,7 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
     p.splits = 1;
     const long long pieces = static_cast<long long>(max_q_len) * Hq * (D / 8);
     const dim3 grid(static_cast<unsigned>((pieces + 255) / 256), B);
-    const cudaError_t e = D == 64 ? px_launch(k_paged_join<64>, p, grid, 256, 0, true, st) : px_launch(k_paged_join<128>, p, grid, 256, 0, true, st);
+    const cudaError_t e = D == 64 ? px_launch<k_paged_join<64>>(p, grid, 256, 0, true, st) : px_launch<k_paged_join<128>>(p, grid, 256, 0, true, st);
     return e == cudaSuccess ? 0 : static_cast<int>(e);
   }
   ExtendParams f = p;

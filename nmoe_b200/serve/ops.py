@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -77,14 +78,14 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
 
 # ------------------------------------------------------------------ shared pieces of the operators below
-def _need(ok: bool, what: str) -> None:
-  if not ok:
-    raise ValueError(what)
+# A decode step calls these once a layer with a few microseconds of device work each, so the checks are written to cost
+# little where they pass: attributes are read once, messages are built only on the way out.
+_HERE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
   """Launches go to the current stream of the tensors' own device, whichever device is current."""
-  return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+  return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 _FN = {}
@@ -105,26 +106,35 @@ def _p(t: Optional[torch.Tensor]) -> int:
   return 0 if t is None else t.data_ptr()
 
 
-def _stream() -> int:
-  return torch.cuda.current_stream().cuda_stream
+def _stream(device: torch.device) -> int:
+  return torch._C._cuda_getCurrentRawStream(device.index)       # torch.cuda.current_stream builds a Stream object every time
 
 
-def _aligned(t: torch.Tensor) -> bool:
-  return t.data_ptr() % 16 == 0
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(*sizes: int) -> int:
+  """Floats of partial results of a call of these sizes; a function of the sizes alone."""
+  return _fn("nmoe_paged_extend_workspace", "iiiiiiiiii", ctypes.c_longlong)(*sizes)
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, Hkv: int, D: int) -> None:
-  _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be [num_blocks, block_size, Hkv, D]")
-  _need(k_cache.size(2) == Hkv and k_cache.size(3) == D, f"the cache holds {tuple(k_cache.shape[2:])} heads x dims, expected ({Hkv}, {D})")
-  _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "k_cache and v_cache must be contiguous")
-  _need(k_cache.dtype == like.dtype and v_cache.dtype == like.dtype, "the cache and the activations must have one dtype")
-  _need(k_cache.device == like.device and v_cache.device == like.device, "the cache must be on the activations' device")
+  shape, dt, dev = k_cache.shape, like.dtype, like.device
+  if len(shape) != 4 or shape != v_cache.shape:
+    raise ValueError("k_cache and v_cache must be [num_blocks, block_size, Hkv, D]")
+  if shape[2] != Hkv or shape[3] != D:
+    raise ValueError(f"the cache holds {tuple(shape[2:])} heads x dims, expected ({Hkv}, {D})")
+  if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    raise ValueError("k_cache and v_cache must be contiguous")
+  if k_cache.dtype != dt or v_cache.dtype != dt:
+    raise ValueError("the cache and the activations must have one dtype")
+  if k_cache.device != dev or v_cache.device != dev:
+    raise ValueError("the cache must be on the activations' device")
+  if like.is_cuda and (k_cache.data_ptr() | v_cache.data_ptr()) % 16 != 0:
+    raise ValueError("the cache must start on a 16-byte boundary")
 
 
-def _check_ints(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-  for name, t in tensors.items():
-    if t is not None:
-      _need(t.dtype == torch.int32 and t.device == device, f"{name} must be int32 on {device}")
+def _check_int32(t: torch.Tensor, device: torch.device, what: str) -> None:
+  if t.dtype != torch.int32 or t.device != device:
+    raise ValueError(f"{what} must be int32 on {device}")
 
 
 # ------------------------------------------------------------------ rotate and append
@@ -156,38 +166,44 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tens
   nothing; the others are distinct.  Returns q [N, n_heads, D] and, with ``need_kv``, rotated k and v [N, n_kv_heads, D]
   (else None).  A slot past the cache is skipped and shows up in ``check_status``."""
   heads = n_heads + 2 * n_kv_heads
-  _need(n_heads > 0 and n_kv_heads > 0 and qkv.dim() == 2 and qkv.size(1) % heads == 0, "qkv must be [N, (n_heads + 2 n_kv_heads) * D]")
-  N, D = qkv.size(0), qkv.size(1) // heads
-  dev = qkv.device
-  _need(positions.shape == (N,) and positions.dtype in (torch.int64, torch.int32) and positions.device == dev,
-        "positions must be [N] int64 or int32 on qkv's device")
-  _need(inv_freq.shape == (D // 2,) and inv_freq.dtype == torch.float32 and D % 2 == 0 and inv_freq.device == dev,
-        "inv_freq must be [D/2] fp32 on qkv's device")
-  _need((slots is None) == (k_cache is None) == (v_cache is None), "slots, k_cache and v_cache go together")
-  if slots is not None:
+  if n_heads <= 0 or n_kv_heads <= 0 or qkv.dim() != 2 or qkv.size(1) % heads != 0:
+    raise ValueError("qkv must be [N, (n_heads + 2 n_kv_heads) * D]")
+  N, width = qkv.shape
+  D, dev = width // heads, qkv.device
+  if positions.shape != (N,) or positions.dtype not in (torch.int64, torch.int32) or positions.device != dev:
+    raise ValueError("positions must be [N] int64 or int32 on qkv's device")
+  if inv_freq.shape != (D // 2,) or inv_freq.dtype != torch.float32 or D % 2 != 0 or inv_freq.device != dev:
+    raise ValueError("inv_freq must be [D/2] fp32 on qkv's device")
+  n_slots = 0
+  if slots is None or k_cache is None or v_cache is None:
+    if not (slots is None and k_cache is None and v_cache is None):
+      raise ValueError("slots, k_cache and v_cache go together")
+  else:
     _check_cache(k_cache, v_cache, qkv, n_kv_heads, D)
-    _check_ints(dev, slots=slots)
-    _need(slots.shape == (N,), "slots must be [N]")
+    _check_int32(slots, dev, "slots")
+    if slots.shape != (N,):
+      raise ValueError("slots must be [N]")
+    slots = slots.contiguous()
+    n_slots = k_cache.size(0) * k_cache.size(1)
   if not qkv.is_cuda:
     q, k, v = rope_append_reference(qkv, positions, inv_freq, conc, n_heads, n_kv_heads, k_cache, v_cache, slots)
     return (q, k, v) if need_kv else (q, None, None)
-  _need(qkv.dtype == torch.bfloat16, "the CUDA kernel takes bf16")
-  _need(D % 16 == 0 and D <= 512, f"head dim {D}: the kernel takes multiples of 16 up to 512")
-  if qkv.stride(1) != 1 or (N > 1 and qkv.stride(0) % 8 != 0) or not _aligned(qkv):
-    qkv = qkv.clone(memory_format=torch.contiguous_format)      # odd strides or start: one copy brings the rows to 16-byte boundaries
+  if qkv.dtype != torch.bfloat16:
+    raise ValueError("the CUDA kernel takes bf16")
+  if D % 16 != 0 or D > 512:
+    raise ValueError(f"head dim {D}: the kernel takes multiples of 16 up to 512")
+  row = qkv.stride(0) if N > 1 else width
+  if row % 8 != 0 or qkv.data_ptr() % 16 != 0 or qkv.stride(1) != 1:
+    qkv, row = qkv.clone(memory_format=torch.contiguous_format), width    # one copy brings the rows to 16-byte boundaries
   positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-  n_slots = 0
-  if slots is not None:
-    slots = slots.contiguous()
-    n_slots = k_cache.size(0) * k_cache.size(1)
-    _need(_aligned(k_cache) and _aligned(v_cache), "the cache must start on a 16-byte boundary")
   with _on(dev):
-    q = torch.empty(N, n_heads, D, dtype=qkv.dtype, device=dev)
-    k = torch.empty(N, n_kv_heads, D, dtype=qkv.dtype, device=dev) if need_kv else None
+    q = torch.empty((N, n_heads, D), dtype=torch.bfloat16, device=dev)
+    k = torch.empty((N, n_kv_heads, D), dtype=torch.bfloat16, device=dev) if need_kv else None
     v = torch.empty_like(k) if need_kv else None
     L.check(_fn("nmoe_rope_append", "plpipfppplpppiiiipp")(
-      _p(qkv), qkv.stride(0) if N > 1 else qkv.size(1), _p(positions), int(positions.dtype == torch.int64), _p(inv_freq), conc, _p(slots), _p(k_cache),
-      _p(v_cache), n_slots, _p(q), _p(k), _p(v), N, n_heads, n_kv_heads, D, _p(status_buffer(dev)), _stream()), "rope_append")
+      qkv.data_ptr(), row, positions.data_ptr(), positions.dtype == torch.int64, inv_freq.data_ptr(), conc, _p(slots), _p(k_cache),
+      _p(v_cache), n_slots, q.data_ptr(), _p(k), _p(v), N, n_heads, n_kv_heads, D, status_buffer(dev).data_ptr(), _stream(dev)),
+      "rope_append")
   return q, k, v
 
 
@@ -219,45 +235,56 @@ def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_st
 
 
 def _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window):
-  _need(q.dim() == 3, "q must be [N, Hq, D]")
-  _need(k_cache.dim() == 4, "k_cache and v_cache must be [num_blocks, block_size, Hkv, D]")
-  Hq, D, Hkv, B = q.size(1), q.size(2), k_cache.size(2), context_lens.numel()
-  _need(Hkv > 0 and Hq % Hkv == 0, f"{Hq} query heads cannot be grouped over {Hkv} key/value heads")
+  """Checks what both attention operators ask for; q and sinks come back as the kernel takes them."""
+  if q.dim() != 3:
+    raise ValueError("q must be [N, Hq, D]")
+  if k_cache.dim() != 4:
+    raise ValueError("k_cache and v_cache must be [num_blocks, block_size, Hkv, D]")
+  N, Hq, D = q.shape
+  Hkv, dev = k_cache.size(2), q.device
+  if Hkv == 0 or Hq % Hkv != 0:
+    raise ValueError(f"{Hq} query heads cannot be grouped over {Hkv} key/value heads")
   _check_cache(k_cache, v_cache, q, Hkv, D)
-  _check_ints(q.device, block_tables=block_tables, context_lens=context_lens)
-  _need(block_tables.dim() == 2 and block_tables.size(0) == B and context_lens.dim() == 1, "block_tables must be [B, n], context_lens [B]")
-  _need(sinks is None or (sinks.shape == (Hq,) and sinks.device == q.device), "sinks must be [Hq] on q's device")
-  _need(window >= 0, "window must not be negative")
-  _need(scale > 0, "scale must be positive")
-
-
-def _attention_args(q, k_cache, v_cache, block_tables, sinks):
-  """What the kernel asks of its operands beyond the checks above; q and sinks may come back as copies."""
-  _need(q.dtype == torch.bfloat16, "the CUDA kernel takes bf16")
-  _need(q.size(2) in (64, 128), f"head dim {q.size(2)}: the kernel takes 64 and 128")
-  _need(_aligned(k_cache) and _aligned(v_cache), "the cache must start on a 16-byte boundary")
-  _need(block_tables.stride(1) == 1 or block_tables.size(1) <= 1, "the rows of block_tables must be dense")
-  if q.stride(2) != 1 or q.stride(1) != q.size(2) or (q.size(0) > 1 and q.stride(0) % 8 != 0) or not _aligned(q):
+  _check_int32(block_tables, dev, "block_tables")
+  _check_int32(context_lens, dev, "context_lens")
+  if context_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.size(0) != context_lens.size(0):
+    raise ValueError("block_tables must be [B, n], context_lens [B]")
+  if sinks is not None and (sinks.shape != (Hq,) or sinks.device != dev):
+    raise ValueError("sinks must be [Hq] on q's device")
+  if window < 0:
+    raise ValueError("window must not be negative")
+  if not scale > 0:
+    raise ValueError("scale must be positive")
+  if not q.is_cuda:
+    return q, sinks
+  if q.dtype != torch.bfloat16:
+    raise ValueError("the CUDA kernel takes bf16")
+  if D != 64 and D != 128:
+    raise ValueError(f"head dim {D}: the kernel takes 64 and 128")
+  if block_tables.size(1) > 1 and block_tables.stride(1) != 1:
+    raise ValueError("the rows of block_tables must be dense")
+  if not q.is_contiguous() and (q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 != 0) or q.data_ptr() % 16 != 0:
     q = q.clone(memory_format=torch.contiguous_format)
   if sinks is not None:
-    sinks = sinks.detach()
-    sinks = sinks.contiguous() if sinks.dtype in (torch.bfloat16, torch.float32) else sinks.float().contiguous()
+    sinks = sinks.detach().contiguous()
+    if sinks.dtype != torch.bfloat16 and sinks.dtype != torch.float32:
+      sinks = sinks.float()
   return q, sinks
 
 
 def _attend(what, q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, out, scale, window, max_q_len, prefix_len):
   """The launch behind ``paged_extend`` and ``shared_prefix_decode`` (on q's device)."""
   N, Hq, D = q.shape
-  sizes = N, context_lens.numel(), Hq, k_cache.size(2), D
-  need = _fn("nmoe_paged_extend_workspace", "iiiiiiiiii", ctypes.c_longlong)(
-    *sizes, k_cache.size(1), block_tables.size(1), max_q_len, window, prefix_len)
+  num_blocks, block_size, Hkv, _ = k_cache.shape
+  B, width, dev = context_lens.size(0), block_tables.size(1), q.device
+  need = _attend_workspace(N, B, Hq, Hkv, D, block_size, width, max_q_len, window, prefix_len)
   # partial results (O, m, l) where the keys of a row are split over more CTAs than exchange them directly
-  work = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+  work = torch.empty((need,), dtype=torch.float32, device=dev) if need else None
   L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifiplpp")(
-    _p(q), q.stride(0), _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(context_lens), _p(q_starts),
-    _p(q_lens), _p(sinks), int(sinks is not None and sinks.dtype == torch.float32), _p(out), *sizes, k_cache.size(1), k_cache.size(0),
-    block_tables.size(1), max_q_len, window, scale, prefix_len, _p(work), need, _p(status_buffer(q.device)), _stream()),
-    what, 2 if need else 1)
+    q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+    context_lens.data_ptr(), _p(q_starts), _p(q_lens), _p(sinks), sinks is not None and sinks.dtype == torch.float32, out.data_ptr(),
+    N, B, Hq, Hkv, D, block_size, num_blocks, width, max_q_len, window, scale, prefix_len, _p(work), need,
+    status_buffer(dev).data_ptr(), _stream(dev)), what, 2 if need else 1)
 
 
 def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -271,24 +298,27 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   key gives zeros.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.
   Lengths or pages outside their tensors are skipped and show up in ``check_status``."""
-  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
-  N, Hq, D = q.shape
-  B = context_lens.numel()
-  _check_ints(q.device, q_starts=q_starts, q_lens=q_lens)
-  _need(q_starts.shape == (B,) and q_lens.shape == (B,), "q_starts and q_lens must be [B]")
+  given = q
+  q, sinks = _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
+  dev, N = q.device, q.size(0)
+  _check_int32(q_starts, dev, "q_starts")
+  _check_int32(q_lens, dev, "q_lens")
+  if q_starts.shape != context_lens.shape or q_lens.shape != context_lens.shape:
+    raise ValueError("q_starts and q_lens must be [B]")
   max_q_len = N if max_q_len is None else int(max_q_len)
-  _need(max_q_len >= 0, "max_q_len must not be negative")
-  if out is not None:
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.is_contiguous(), "out must be contiguous and like q")
+  if max_q_len < 0:
+    raise ValueError("max_q_len must not be negative")
+  if out is not None and (out.shape != given.shape or out.dtype != given.dtype or out.device != dev or not out.is_contiguous()):
+    raise ValueError("out must be contiguous and like q")
   if not q.is_cuda:
     return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window, out)
-  q, sinks = _attention_args(q, k_cache, v_cache, block_tables, sinks)
-  context_lens, q_starts, q_lens = context_lens.contiguous(), q_starts.contiguous(), q_lens.contiguous()
-  with _on(q.device):
-    out = torch.zeros(N, Hq, D, dtype=q.dtype, device=q.device) if out is None else out
-    _need(_aligned(out), "out must start on a 16-byte boundary")
-    _attend("paged_extend", q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, out, scale, window,
-            min(max_q_len, N), 0)
+  if out is not None and out.data_ptr() % 16 != 0:
+    raise ValueError("out must start on a 16-byte boundary")
+  with _on(dev):
+    if out is None:
+      out = torch.zeros(q.shape, dtype=q.dtype, device=dev)
+    _attend("paged_extend", q, k_cache, v_cache, block_tables, context_lens.contiguous(), q_starts.contiguous(), q_lens.contiguous(),
+            sinks, out, scale, window, min(max_q_len, N), 0)
   return out
 
 
@@ -302,20 +332,19 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
   q [B, Hq, D] -> [B, Hq, D]; block_tables [B, n] hold every sequence's whole table (prefix pages included; where the prefix
   ends inside a page, each table may have its own copy of that page).  ``context_lens`` counts the current token; a sequence
   with a context of 0 (a padding row) gives zeros, one shorter than the prefix sees its part of it."""
-  _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
-  B, Hq, D = q.shape
-  _need(context_lens.numel() == B, "q must hold one token per sequence")
-  _need(0 <= prefix_len <= block_tables.size(1) * k_cache.size(1), "prefix_len must lie within the block tables")
+  q, sinks = _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
+  if context_lens.size(0) != q.size(0):
+    raise ValueError("q must hold one token per sequence")
+  if not 0 <= prefix_len <= block_tables.size(1) * k_cache.size(1):
+    raise ValueError("prefix_len must lie within the block tables")
   if not q.is_cuda:
     one = torch.ones_like(context_lens)
     return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, torch.cumsum(one, 0) - 1,
                                   torch.minimum(one, context_lens), sinks, scale, window)
-  q, sinks = _attention_args(q, k_cache, v_cache, block_tables, sinks)
-  context_lens = context_lens.contiguous()
   with _on(q.device):
-    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    _attend("shared_prefix_decode", q, k_cache, v_cache, block_tables, context_lens, None, None, sinks, out, scale, window, 1,
-            prefix_len)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _attend("shared_prefix_decode", q, k_cache, v_cache, block_tables, context_lens.contiguous(), None, None, sinks, out, scale, window,
+            1, prefix_len)
   return out
 
 
@@ -372,17 +401,26 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
   Returns (out [N] int32: the emitted tokens from row q_starts[b] on, -1 behind them; n_out [B] int32: how many, at least 1
   for a sequence with rows).  Rows of no sequence are -1, or left as they were in a given ``out``.  A drafted token outside
   the vocabulary fails and shows up in ``check_status``."""
-  _need(target_probs.dim() == 2 and target_probs.size(1) > 0, "target_probs must be [N, V]")
+  if target_probs.dim() != 2 or target_probs.size(1) == 0:
+    raise ValueError("target_probs must be [N, V]")
   N, V = target_probs.shape
-  B, dev = q_lens.numel(), target_probs.device
-  _need(target_probs.dtype == torch.float32, "target_probs must be fp32")
-  _need(draft_probs is None or (draft_probs.shape == (N, V) and draft_probs.dtype == torch.float32 and draft_probs.device == dev),
-        "draft_probs must be like target_probs")
-  _need(tokens.shape == (N,) and tokens.dtype in (torch.int64, torch.int32) and tokens.device == dev, "tokens must be [N] int64 or int32")
-  _need(uniforms.shape == (N,) and uniforms.dtype == torch.float32 and uniforms.device == dev, "uniforms must be [N] fp32")
-  _check_ints(dev, q_starts=q_starts, q_lens=q_lens, out=out)
-  _need(q_starts.shape == (B,) and q_lens.shape == (B,), "q_starts and q_lens must be [B]")
-  _need(out is None or (out.shape == (N,) and out.is_contiguous()), "out must be a contiguous [N]")
+  dev = target_probs.device
+  if target_probs.dtype != torch.float32:
+    raise ValueError("target_probs must be fp32")
+  if draft_probs is not None and (draft_probs.shape != (N, V) or draft_probs.dtype != torch.float32 or draft_probs.device != dev):
+    raise ValueError("draft_probs must be like target_probs")
+  if tokens.shape != (N,) or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != dev:
+    raise ValueError("tokens must be [N] int64 or int32 on target_probs' device")
+  if uniforms.shape != (N,) or uniforms.dtype != torch.float32 or uniforms.device != dev:
+    raise ValueError("uniforms must be [N] fp32 on target_probs' device")
+  _check_int32(q_starts, dev, "q_starts")
+  _check_int32(q_lens, dev, "q_lens")
+  if q_starts.dim() != 1 or q_starts.shape != q_lens.shape:
+    raise ValueError("q_starts and q_lens must be [B]")
+  if out is not None:
+    _check_int32(out, dev, "out")
+    if out.shape != (N,) or not out.is_contiguous():
+      raise ValueError("out must be a contiguous [N]")
   if not target_probs.is_cuda:
     return verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, draft_probs, out)
   if target_probs.stride(1) != 1 and V > 1:
@@ -392,9 +430,9 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
   tokens, uniforms, q_starts, q_lens = tokens.contiguous(), uniforms.contiguous(), q_starts.contiguous(), q_lens.contiguous()
   with _on(dev):
     out = torch.full((N,), -1, dtype=torch.int32, device=dev) if out is None else out
-    n_out = torch.empty(B, dtype=torch.int32, device=dev)
+    n_out = torch.empty(q_lens.shape, dtype=torch.int32, device=dev)
     L.check(_fn("nmoe_verify_draft", "plplpippppp" + "iiipp")(
-      _p(target_probs), target_probs.stride(0), _p(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), _p(tokens),
-      int(tokens.dtype == torch.int64), _p(uniforms), _p(q_starts), _p(q_lens), _p(out), _p(n_out), N, B, V,
-      _p(status_buffer(dev)), _stream()), "verify_draft")
+      target_probs.data_ptr(), target_probs.stride(0), _p(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
+      tokens.data_ptr(), tokens.dtype == torch.int64, uniforms.data_ptr(), q_starts.data_ptr(), q_lens.data_ptr(), out.data_ptr(),
+      n_out.data_ptr(), N, q_lens.size(0), V, status_buffer(dev).data_ptr(), _stream(dev)), "verify_draft")
   return out, n_out
