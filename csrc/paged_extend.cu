@@ -6,10 +6,12 @@
 // head of the group, 128 rows to a tile, so every K/V block is read once for all of them.  Each row carries its own
 // bounds [lo, hi) of visible keys (causal end, window, shared part); a block that lies inside all of them needs no mask.
 //
-// Pipeline of a CTA, 64 keys at a time: four loader warps gather the block's K and V rows from their pages with
+// Pipeline of a CTA (one tile), 64 keys at a time: two loader warps gather the block's K and V rows from their pages with
 // cp.async (16 bytes a lane, any page size, zero fill outside the CTA's keys, so that what lies there cannot reach the
-// products), one thread issues the MMAs (S of block i+1 before P V of block i), four warps per tile own 32 rows each:
-// running maximum and sum in fp32, P as bf16 back to tensor memory as the A operand of P V.  The running maximum is
+// products), one thread issues the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back to
+// tensor memory as the A operand of P V.  A block is a chain of latencies (S, softmax, P V) of some 1900 cycles in which a
+// warp keeps no unit busy, so the SM is filled with chains: three CTAs for D = 64 (S single-buffered to fit tensor
+// memory), two for D = 128.  The running maximum is
 // raised only when it grows by more than 2^8; the stale one is exact after the final division.  P is rounded to bf16
 // because the tensor core multiplies it with bf16 values; the sum l takes the unrounded p.
 //
@@ -248,46 +250,44 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
   if (splits > 1) cl.sync();                                     // nobody leaves while its rows may still be read
 }
 
-// Layout of shared memory.  D = 64: 4 stages of 16 KB, with one row tile two CTAs fit an SM; D = 128: 32 KB stages,
-// one CTA an SM.  The exchange of partial results reuses the stages (O as fp32, 16-byte pieces swizzled by row).
-template <int D, int TILES>
+// Layout of shared memory.  The exchange of partial results reuses the stages (O as fp32, 16-byte pieces swizzled by row).
+template <int D>
 struct PxSmem {
-  // loader threads: two warps keep the two CTAs of an SM at 8 warps and 128 registers each
-  static constexpr int kLoaders = D == 64 && TILES == 1 ? 64 : 128;
-  static constexpr int kThreads = 4 * TILES * 32 + 32 + kLoaders;
-  static constexpr int kStages = 4;
-  static constexpr int kQTile = PX_BM * D * 2;
+  static constexpr int kCtas = D == 64 ? 3 : 2;            // of an SM: 66 KB and 100 KB of shared memory, 128 and 256 columns of tensor memory
+  static constexpr int kBufs = D == 64 ? 1 : 2;            // S buffers of 64 columns
+  static constexpr int kLoaders = 64;                      // threads
+  static constexpr int kThreads = 4 * 32 + 32 + kLoaders;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kQ = PX_BM * D * 2;
   static constexpr int kKV = PX_BN * D * 2;                // one of K, V
   static constexpr int kStage = 2 * kKV;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kExchange = TILES * PX_BM * (D + 2) * 4;
+  static constexpr int kExchange = PX_BM * (D + 2) * 4;
   static constexpr int kBody = kRing > kExchange ? kRing : kExchange;
-  static constexpr int kBytes = TILES * kQTile + kBody + 256 + 1024;
+  static constexpr int kBytes = kQ + kBody + 256 + 1024;
+  static constexpr uint32_t kTmemCols = kBufs * PX_BN + D;
 };
 
-template <int D, int TILES>
-__global__ void __launch_bounds__(PxSmem<D, TILES>::kThreads, (D == 64 && TILES == 1) ? 2 : 1)
-k_paged_extend(const ExtendParams p) {
-  using SM = PxSmem<D, TILES>;
-  constexpr int kStages = SM::kStages;
-  constexpr int kLag = 2;                    // see the loader
-  constexpr int kRows = TILES * PX_BM;
+template <int D>
+__global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged_extend(const ExtendParams p) {
+  using SM = PxSmem<D>;
+  constexpr int kStages = SM::kStages, kBufs = SM::kBufs;
+  constexpr int kLag = kStages - 1;          // see the loader
   constexpr int kThreads = SM::kThreads;
-  constexpr int kMmaWarp = 4 * TILES;
-  constexpr uint32_t kTmemCols = TILES == 1 ? 256 : 512;
-  constexpr uint32_t kTmemO = TILES * 128;
+  constexpr int kMmaWarp = 4;
+  constexpr uint32_t kTmemO = kBufs * PX_BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + TILES * SM::kQTile;
+  uint8_t* sKV = sQ + SM::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SM::kBody);
   uint64_t* kv_full = bars;                  // [kStages]
   uint64_t* kv_empty = kv_full + kStages;    // [kStages]
-  uint64_t* s_full = kv_empty + kStages;     // [tile][buf]
-  uint64_t* p_full = s_full + 2 * TILES;     // [tile][buf]
-  uint64_t* pv_done = p_full + 2 * TILES;    // [tile]
-  uint64_t* o_full = pv_done + TILES;        // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
+  uint64_t* s_full = kv_empty + kStages;     // [kBufs]
+  uint64_t* p_full = s_full + kBufs;         // [kBufs]
+  uint64_t* pv_done = p_full + kBufs;
+  uint64_t* o_full = pv_done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_range = reinterpret_cast<int*>(tmem_slot + 2);          // [2] first key, end of keys
 
@@ -301,8 +301,8 @@ k_paged_extend(const ExtendParams p) {
 
   int start, n, ctx;
   px_list(p, b, tile_x == 0 && unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
-  const int row0 = tile_x * kRows;                               // first row of this CTA's tiles
-  const int n_valid = min(kRows, n * g - row0);                  // rows that exist
+  const int row0 = tile_x * PX_BM;                               // first row of this CTA's tile
+  const int n_valid = min(PX_BM, n * g - row0);                  // rows that exist
   if (n_valid <= 0) {                                            // uniform over the cluster
     if (p.part_mode == 1) px_launch_dependents();
     if (p.part_mode == 2) px_wait_prior_grid();
@@ -312,44 +312,44 @@ k_paged_extend(const ExtendParams p) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) { mbar_init(&kv_full[i], SM::kLoaders / 32); mbar_init(&kv_empty[i], 1); }
-    for (int t = 0; t < TILES; ++t) {
-      const int rows = min(PX_BM, n_valid - t * PX_BM);
-      const int warps = rows > 0 ? (rows + 31) / 32 : 1;
-      for (int i = 0; i < 2; ++i) { mbar_init(&s_full[2 * t + i], 1); mbar_init(&p_full[2 * t + i], warps); }
-      mbar_init(&pv_done[t], 1);
-      mbar_init(&o_full[t], 1);
-    }
+    for (int i = 0; i < kBufs; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], (n_valid + 31) / 32); }
+    mbar_init(pv_done, 1);
+    mbar_init(o_full, 1);
     s_range[0] = 0x7fffffff;
     s_range[1] = 0;
     *abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == kMmaWarp) {
-    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_alloc(tmem_slot, SM::kTmemCols);
     tmem_relinquish();
   }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  // Row r of the tile lies in lane r + 32 * turn of tensor memory (modulo 128), the turn differing between the CTAs of an
+  // SM: the busy warps of tiles with few rows then sit on different schedulers.
+  const int turn = static_cast<int>((tmem_base & 511u) / SM::kTmemCols) * (4 / SM::kBufs / 2 + 1) & 3;
   // rows of Q, 128-byte swizzle, K-major; rows that do not exist are zero
-  for (int i = threadIdx.x; i < kRows * (D / 8); i += kThreads) {
-    const int r = i / (D / 8), c = i % (D / 8), rr = row0 + r;
+  for (int i = threadIdx.x; i < PX_BM * (D / 8); i += kThreads) {
+    const int r = i / (D / 8), c = i % (D / 8), rr = row0 + r, at = (r + 32 * turn) & 127;
     int4 v = make_int4(0, 0, 0, 0);
     if (r < n_valid) {
       const int tok = rr / g, h = hk * g + rr - tok * g;
       v = ld_nc_v4(p.q + (start + tok) * p.q_stride + static_cast<long long>(h) * D + c * 8);
     }
-    *reinterpret_cast<int4*>(sQ + (r >> 7) * SM::kQTile + (c >> 3) * (PX_BM * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+    *reinterpret_cast<int4*>(sQ + (c >> 3) * (PX_BM * 128) + at * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
   }
   fence_proxy_async_smem();
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
   // every CTA holds its tensor memory before a dependent launch may ask for some
   if (p.part_mode == 1) px_launch_dependents();
 
   // bounds of this thread's row
   int lo = 0, hi = 0;
-  const int my_row = threadIdx.x;                                // softmax threads: row inside the CTA's tiles
-  if (warp < 4 * TILES && my_row < n_valid) {
+  const int quad_row = (((warp & 3) - turn) & 3) * 32, my_row = quad_row + lane;         // softmax threads: row of the tile
+  const bool softmax_warp = warp < kMmaWarp && quad_row < n_valid;
+  if (softmax_warp && my_row < n_valid) {
     px_bounds(p, (row0 + my_row) / g, n, ctx, hk == 0 && unit == 0 && (row0 + my_row) % g == 0, lo, hi);
     if (lo < hi) {
       atomicMin(&s_range[0], lo);
@@ -429,49 +429,43 @@ k_paged_extend(const ExtendParams p) {
     if (elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_bf16(PX_BM, PX_BN, 0, 0);
       constexpr uint32_t idesc_pv = make_idesc_bf16(PX_BM, D, 0, 1);
+      const uint64_t qa = make_smem_desc(smem_u32(sQ), 0, 1024, kSwizzle128B);
       auto issue_s = [&](int i) -> bool {
         const int st = i % kStages;
         if (!px_wait(&kv_full[st], (i / kStages) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1031, i, 0); *abort_flag = 1; return false; }
         tc_fence_after_sync();
         const uint64_t ka = make_smem_desc(smem_u32(sKV + st * SM::kStage), 0, 1024, kSwizzle128B);
+        const uint32_t d = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          if (t * PX_BM >= n_valid) continue;
-          const uint64_t qa = make_smem_desc(smem_u32(sQ + t * SM::kQTile), 0, 1024, kSwizzle128B);
-          const uint32_t d = tmem_base + t * 128 + (i & 1) * PX_BN;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-            mma_f16_ss(d, qa + (((j >> 2) * (PX_BM * 128) + (j & 3) * 32) >> 4), ka + (((j >> 2) * (PX_BN * 128) + (j & 3) * 32) >> 4),
-                       idesc_s, j != 0 ? 1u : 0u);
-          mma_commit(&s_full[t * 2 + (i & 1)]);
-        }
+        for (int j = 0; j < D / 16; ++j)
+          mma_f16_ss(d, qa + (((j >> 2) * (PX_BM * 128) + (j & 3) * 32) >> 4), ka + (((j >> 2) * (PX_BN * 128) + (j & 3) * 32) >> 4),
+                     idesc_s, j != 0 ? 1u : 0u);
+        mma_commit(&s_full[i % kBufs]);
         return true;
       };
       bool good = n_blk > 0 && issue_s(0);
       for (int i = 0; good && i < n_blk; ++i) {
-        if (i + 1 < n_blk) { good = issue_s(i + 1); if (!good) break; }
+        if (kBufs == 2 && i + 1 < n_blk) { good = issue_s(i + 1); if (!good) break; }
         const int st = i % kStages;
         const uint64_t va = make_smem_desc(smem_u32(sKV + st * SM::kStage + SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
+        if (!px_wait(&p_full[i % kBufs], (i / kBufs) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1032, i, 0); *abort_flag = 1; break; }
+        tc_fence_after_sync();
+        const uint32_t a_t = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          if (t * PX_BM >= n_valid) continue;
-          if (!px_wait(&p_full[t * 2 + (i & 1)], (i >> 1) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1032, i, t); *abort_flag = 1; good = false; break; }
-          tc_fence_after_sync();
-          const uint32_t a_t = tmem_base + t * 128 + (i & 1) * PX_BN;
-#pragma unroll
-          for (int j = 0; j < PX_BN / 16; ++j)
-            px_mma_ts(tmem_base + kTmemO + t * D, a_t + j * 8, va + ((j * 2048) >> 4), idesc_pv, (i | j) != 0 ? 1u : 0u);
-          mma_commit(i + 1 < n_blk ? &pv_done[t] : &o_full[t]);
-        }
+        for (int j = 0; j < PX_BN / 16; ++j)
+          px_mma_ts(tmem_base + kTmemO, a_t + j * 8, va + ((j * 2048) >> 4), idesc_pv, (i | j) != 0 ? 1u : 0u);
         mma_commit(&kv_empty[st]);
+        if (i + 1 == n_blk) mma_commit(o_full);
+        else if (kBufs == 2) mma_commit(pv_done);
+        // one buffer: S goes over P once P V has read it (the tensor core takes the products in order)
+        if (kBufs == 1 && i + 1 < n_blk) good = issue_s(i + 1);
       }
     }
     __syncwarp();
-  } else if ((warp >> 2) * PX_BM + (warp & 3) * 32 < n_valid) {
-    // ------------------------------------------------------------ softmax: warp -> (tile, 32 rows)
-    const int tile = warp >> 2;
+  } else if (softmax_warp) {
+    // ------------------------------------------------------------ softmax, 32 rows a warp
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tmem_o = tmem_base + kTmemO + tile * D + lane_addr;
+    const uint32_t tmem_o = tmem_base + kTmemO + lane_addr;
     const bool mine = my_row < n_valid;
     // bounds inside which no row of this warp needs a mask
     int w_lo = mine ? lo : 0, w_hi = mine ? hi : 0x7fffffff;
@@ -481,36 +475,45 @@ k_paged_extend(const ExtendParams p) {
       w_hi = min(w_hi, __shfl_xor_sync(0xffffffffu, w_hi, o));
     }
     for (int i = 0; i < n_blk; ++i) {
-      const int bf = i & 1;
-      const uint32_t s_addr = tmem_base + lane_addr + tile * 128 + bf * PX_BN;
-      ok = px_wait(&s_full[tile * 2 + bf], (i >> 1) & 1, abort_flag);
+      const int bf = i % kBufs;
+      const uint32_t s_addr = tmem_base + lane_addr + bf * PX_BN;
+      ok = px_wait(&s_full[bf], (i / kBufs) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1033, i, tile); *abort_flag = 1; break; }
+      if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1033, i, 0); *abort_flag = 1; break; }
       tc_fence_after_sync();
-      uint32_t r[PX_BN];
-      tmem_ld_32x32b_x32(s_addr, r);
-      tmem_ld_32x32b_x32(s_addr + 32, r + 32);
-      tmem_ld_wait();
+      // S in halves of 32 keys, the first read twice: 80 registers a thread hold no more
       const int k0 = key0 + i * PX_BN;
-      if (k0 < w_lo || k0 + PX_BN > w_hi) {
-        const int from = lo - k0, to = hi - k0;
+      const bool edge = k0 < w_lo || k0 + PX_BN > w_hi;
+      uint32_t r[32];
+      auto half = [&](int hf) {
+        tmem_ld_32x32b_x32(s_addr + hf * 32, r);
+        tmem_ld_wait();
+        if (edge) {
+          const int from = lo - k0 - hf * 32, to = hi - k0 - hf * 32;
 #pragma unroll
-        for (int t = 0; t < PX_BN; ++t)
-          if (t < from || t >= to) r[t] = 0xff800000u;                       // -inf
+          for (int t = 0; t < 32; ++t)
+            if (t < from || t >= to) r[t] = 0xff800000u;                     // -inf
+        }
+      };
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains: one would be 32 latencies long
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        half(hf);
+#pragma unroll
+        for (int t = 0; t < 32; t += 2)
+          mx4[(t >> 1) & 3] = px_max3(mx4[(t >> 1) & 3], __uint_as_float(r[t]), __uint_as_float(r[t + 1]));
       }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains: one would be 64 latencies long
-#pragma unroll
-      for (int t = 0; t < PX_BN; t += 2)
-        mx4[(t >> 1) & 3] = px_max3(mx4[(t >> 1) & 3], __uint_as_float(r[t]), __uint_as_float(r[t + 1]));
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       const float m_cand = fmaxf(m, mx * p.scale_log2);
       bool grow = m_cand - m > kPxRescale;
       if (i == 0) { grow = false; m = m_cand; }
       if (__any_sync(0xffffffffu, grow)) {
-        ok = px_wait(&pv_done[tile], (i - 1) & 1, abort_flag);               // O is final for the blocks before
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1034, i, tile); *abort_flag = 1; break; }
-        tc_fence_after_sync();
+        if (kBufs == 2) {                                                    // O is final for the blocks before (one buffer: S says so)
+          ok = px_wait(pv_done, (i - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1034, i, 0); *abort_flag = 1; break; }
+          tc_fence_after_sync();
+        }
         float alpha = 1.f;
         if (grow) { alpha = px_exp2(m - m_cand); m = m_cand; l *= alpha; }
 #pragma unroll 1
@@ -526,33 +529,36 @@ k_paged_extend(const ExtendParams p) {
       }
       const uint64_t sc2 = px_pack(p.scale_log2, p.scale_log2), nm2 = px_pack(-m, -m);
       uint64_t rs2[4] = {0, 0, 0, 0};                                        // pairs of partial sums, both halves 0.f
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t pk[16];
+      auto exps = [&](uint32_t (&pk)[16]) {
 #pragma unroll
         for (int t = 0; t < 32; t += 2) {
           float x0, x1;
-          px_unpack(px_fma2(px_pack(__uint_as_float(r[hf * 32 + t]), __uint_as_float(r[hf * 32 + t + 1])), sc2, nm2), x0, x1);
+          px_unpack(px_fma2(px_pack(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nm2), x0, x1);
           const float p0 = px_exp2(x0), p1 = px_exp2(x1);
           rs2[(t >> 1) & 3] = px_add2(rs2[(t >> 1) & 3], px_pack(p0, p1));
           pk[t >> 1] = pack_bf16x2(p0, p1);
         }
-        px_tmem_st_x16(s_addr + hf * 16, pk);
-      }
+      };
+      uint32_t pa[16], pb[16];
+      exps(pb);
+      half(0);                                                               // before P goes over it
+      exps(pa);
+      px_tmem_st_x16(s_addr, pa);
+      px_tmem_st_x16(s_addr + 16, pb);
       float sa, sb;
       px_unpack(px_add2(px_add2(rs2[0], rs2[1]), px_add2(rs2[2], rs2[3])), sa, sb);
       l += sa + sb;
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[tile * 2 + bf]);
+      if (lane == 0) mbar_arrive(&p_full[bf]);
     }
     // The end of the last P V has a barrier of its own: pv_done alternates its parity with every block, and when a
     // warp gets here it may still be two phases behind (P V of the block before runs after S of the last one) or done.
     if (ok && n_blk > 0) {
-      ok = px_wait(&o_full[tile], 0, abort_flag);
+      ok = px_wait(o_full, 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1035, 0, tile); *abort_flag = 1; }
+      if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1035, 0, 0); *abort_flag = 1; }
     }
     tc_fence_after_sync();
   }
@@ -561,13 +567,12 @@ k_paged_extend(const ExtendParams p) {
   }
 
   // ---------------------------------------------------------------- results
-  const bool softmax_warp = warp < 4 * TILES && (warp >> 2) * PX_BM + (warp & 3) * 32 < n_valid;
   const bool direct = p.splits == 1 && p.part_mode == 0;
-  float* sx = reinterpret_cast<float*>(sKV);                     // [kRows][D], 16-byte pieces swizzled by row
-  float* s_ml = sx + kRows * D;                                  // [kRows][2]
+  float* sx = reinterpret_cast<float*>(sKV);                     // [PX_BM][D], 16-byte pieces swizzled by row
+  float* s_ml = sx + PX_BM * D;                                  // [PX_BM][2]
   if (!direct) __syncthreads();                                  // every MMA of the CTA is done: the stages are free
   if (softmax_warp) {
-    const uint32_t tmem_o = tmem_base + kTmemO + (warp >> 2) * D + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t tmem_o = tmem_base + kTmemO + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float f = 1.f;
     __nv_bfloat16* orow = nullptr;
     if (direct && my_row < n_valid) {
@@ -612,7 +617,7 @@ k_paged_extend(const ExtendParams p) {
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, kTmemCols);
+    tmem_dealloc(tmem_base, SM::kTmemCols);
   }
   if (direct) return;
 
@@ -934,7 +939,6 @@ __global__ void __launch_bounds__(256) k_paged_join(const ExtendParams p) {
 // How a call is cut: which kernel, tiles a list, CTAs the keys of a tile are split over.
 struct PxPlan {
   int nt;                 // > 0: the kernel for few rows, 8 * nt of them
-  int tiles_cta;          // row tiles of a CTA (kernel for many rows)
   long long tiles;
   int splits, groups;
 };
@@ -945,7 +949,6 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
   const int few_most = D == 64 ? 40 : 32;
   q.nt = 0;
   q.tiles = 1;
-  q.tiles_cta = 1;
   long long slots, least;                  // CTAs the GPU holds at once; keys that make a split worth while
   if (rows <= few_most) {
     const int t = static_cast<int>((rows + 7) / 8);
@@ -953,11 +956,8 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
     slots = 296;
     least = 2 * 4 * (2048 / D);
   } else {
-    // two tiles a CTA halve the K/V traffic; one tile spreads few rows over more SMs
-    const long long pairs = (rows + 2 * PX_BM - 1) / (2 * PX_BM);
-    q.tiles_cta = rows > PX_BM && pairs * lists * hkv >= 148 ? 2 : 1;
-    q.tiles = q.tiles_cta == 2 ? pairs : (rows + PX_BM - 1) / PX_BM;
-    slots = D == 64 && q.tiles_cta == 1 ? 296 : 148;
+    q.tiles = (rows + PX_BM - 1) / PX_BM;
+    slots = D == 64 ? 3 * 148 : 2 * 148;
     least = 4 * PX_BN;
   }
   const long long base = q.tiles * lists * hkv;
@@ -1008,9 +1008,9 @@ template <int D, int NT>
 static cudaError_t px_few(const ExtendParams& p, dim3 grid, cudaStream_t st) {
   return px_launch<k_paged_few<D, NT>>(p, grid, PxFew<D, NT>::kThreads, PxFew<D, NT>::kBytes, p.part_mode == 2, st);
 }
-template <int D, int TILES>
+template <int D>
 static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
-  return px_launch<k_paged_extend<D, TILES>>(p, grid, PxSmem<D, TILES>::kThreads, PxSmem<D, TILES>::kBytes, p.part_mode == 2, st);
+  return px_launch<k_paged_extend<D>>(p, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st);
 }
 
 static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream_t st) {
@@ -1021,7 +1021,7 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
   cudaError_t e;
   if (D == 64) {
     switch (q.nt) {
-      case 0: e = q.tiles_cta == 2 ? px_many<64, 2>(p, grid, st) : px_many<64, 1>(p, grid, st); break;
+      case 0: e = px_many<64>(p, grid, st); break;
       case 1: e = px_few<64, 1>(p, grid, st); break;
       case 2: e = px_few<64, 2>(p, grid, st); break;
       case 3: e = px_few<64, 3>(p, grid, st); break;
@@ -1029,7 +1029,7 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
     }
   } else {
     switch (q.nt) {
-      case 0: e = q.tiles_cta == 2 ? px_many<128, 2>(p, grid, st) : px_many<128, 1>(p, grid, st); break;
+      case 0: e = px_many<128>(p, grid, st); break;
       case 1: e = px_few<128, 1>(p, grid, st); break;
       case 2: e = px_few<128, 2>(p, grid, st); break;
       default: e = px_few<128, 4>(p, grid, st); break;
