@@ -50,6 +50,7 @@ struct ExtendParams {
   int key_begin, key_end;             // only keys in [key_begin, key_end) count here
   int flat;                           // 1: the tokens of all sequences are one list that reads the first sequence's pages
   int splits, groups;                 // the keys of a row list are divided over groups x splits CTAs, splits = a cluster
+  int sorted;                         // 1: lists by falling context
   int part_mode;                      // 0 none, 1 write partial results (one set per group), 2 join those of the launch before
   int n_sets;                         // sets of partial results to join
   long long set_rows;                 // rows of a set
@@ -152,6 +153,26 @@ NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start,
     if (speaker) report_status(p.status, kStatusBadIndex, 1021, b, ctx);
     ctx = p.capacity;
   }
+}
+// The list of blocks with index z: the z-th longest context where one wave of CTAs does not hold them all, so that the long
+// ones start first and the short ones fill the end.  Every CTA ranks the contexts for itself.
+constexpr int PX_SORT_MOST = 256;
+template <int kThreads>
+NMOE_DEVICE int px_nth_longest(const ExtendParams& p, int z, int* s_len) {         // s_len: PX_SORT_MOST + 1 words of scratch
+  int& s_which = s_len[PX_SORT_MOST];
+  for (int t = threadIdx.x; t < p.n_seqs; t += kThreads)
+    s_len[t] = p.q_lens != nullptr && p.q_lens[t] <= 0 ? -1 : p.context_lens[t];
+  __syncthreads();
+  for (int t = threadIdx.x; t < p.n_seqs; t += kThreads) {
+    const int mine = s_len[t];
+    int rank = 0;
+    for (int u = 0; u < p.n_seqs; ++u) rank += s_len[u] > mine || (s_len[u] == mine && u < t) ? 1 : 0;
+    if (rank == z) s_which = t;
+  }
+  __syncthreads();
+  const int which = s_which;
+  __syncthreads();                                               // the scratch may be used for something else
+  return which;
 }
 // Keys [lo, hi) that a token of the list sees.
 NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool speaker, int& lo, int& hi) {
@@ -297,7 +318,7 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   const int n_tiles_x = static_cast<int>(gridDim.x) / units;
   // tiles with the longest contexts (the last ones of a prompt) first: better tail
   const int tile_x = n_tiles_x - 1 - static_cast<int>(blockIdx.x) / units;
-  const int hk = blockIdx.y, b = p.flat ? 0 : blockIdx.z, g = p.group;
+  const int hk = blockIdx.y, b = p.flat ? 0 : p.sorted ? px_nth_longest<kThreads>(p, blockIdx.z, reinterpret_cast<int*>(sKV)) : blockIdx.z, g = p.group;
 
   int start, n, ctx;
   px_list(p, b, tile_x == 0 && unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
@@ -629,19 +650,24 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
 // the bytes of K and V, so the matrix work goes where its results are easy to use: with keys as the rows of the warp-wide
 // mma and 8 query rows as its columns, S^T = K Q^T and O^T += V^T P^T waste nothing at 8 rows, every lane exponentiates
 // its own share (a tcgen05 tile gives a whole row of 64 keys to one lane: 1350 cycles a block for one busy warp), and no
-// barrier is needed.  Each of four warps streams its own tiles of 32 (D = 64) or 16 keys through three stages of 8 KB,
+// barrier is needed.  Each of four warps streams its own tiles of 16 or 32 keys through a ring of its own,
 // with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
 // movmatrix; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
 template <int D, int NT>
 struct PxFew {
-  static constexpr int kWarps = 4, kThreads = 128, kStages = 3;
-  static constexpr int kTile = 2048 / D;                   // keys per tile: K and V together are 8 KB
+  static constexpr int kWarps = 4, kThreads = 128;
+  // CTAs of an SM, as registers allow; the rings share what shared memory there is
+  static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT == 1 ? 3 : 2);
+  static constexpr int kTile = kCtas > 2 || D == 128 ? 16 : 32;          // keys per tile
   static constexpr int kKV = kTile * D * 2;
-  static constexpr int kRing = kStages * 2 * kKV;          // of a warp
   static constexpr int kRows = 8 * NT;
   static constexpr int kOStride = D + 4;                   // floats; a warp leaves its O in its ring
-  static_assert(kRows * kOStride * 4 + kRows * 8 <= kRing, "O of a warp fits its ring");
-  static constexpr int kBytes = kWarps * kRing + kRows * (D + 2) * 4 + 128;
+  static constexpr int kJoined = kRows * (D + 2) * 4;
+  static constexpr int kRingMost = ((232448 / kCtas - 1024 - 128 - kJoined) / kWarps) & ~127;
+  static constexpr int kStages = kRingMost / (2 * kKV) < 6 ? kRingMost / (2 * kKV) : 6;
+  static constexpr int kRing = kStages * 2 * kKV;          // of a warp
+  static_assert(kStages >= 2 && kRows * kOStride * 4 + kRows * 8 <= kRing, "O of a warp fits its ring");
+  static constexpr int kBytes = kWarps * kRing + kJoined + 128;
 };
 
 NMOE_DEVICE void px_ldm(uint32_t addr, uint32_t (&r)[4]) {
@@ -663,15 +689,17 @@ NMOE_DEVICE void px_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
+__global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const ExtendParams p) {
   using F = PxFew<D, NT>;
   constexpr int kTile = F::kTile, kStages = F::kStages, MT = kTile / 16, KS = D / 16;
+  const float inv_g = 1.f / static_cast<float>(p.group);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   float* sx = reinterpret_cast<float*>(smem + F::kWarps * F::kRing);       // [rows][D], joined over the warps
   float* s_ml = sx + F::kRows * D;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = p.splits * p.groups, unit = blockIdx.x, hk = blockIdx.y, b = p.flat ? 0 : blockIdx.z, g = p.group;
+  const int units = p.splits * p.groups, unit = blockIdx.x, hk = blockIdx.y, g = p.group;
+  const int b = p.flat ? 0 : p.sorted ? px_nth_longest<F::kThreads>(p, blockIdx.z, reinterpret_cast<int*>(smem)) : blockIdx.z;
   int start, n, ctx;
   px_list(p, b, unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
   const int n_valid = min(F::kRows, n * g);                      // the host launches this kernel only where all rows fit
@@ -683,21 +711,28 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
   if (p.part_mode == 1) px_launch_dependents();
   const int* table = p.block_tables + b * p.bt_stride;
 
-  // keys of the list, and the bounds inside which no row needs a mask (every warp works them out)
-  int k_begin = 0x7fffffff, k_end = 0, w_lo = 0, w_hi = 0x7fffffff;
-  for (int r = lane; r < n_valid; r += 32) {
-    int lo, hi;
-    px_bounds(p, r / g, n, ctx, hk == 0 && unit == 0 && warp == 0 && r % g == 0, lo, hi);
-    w_lo = max(w_lo, lo);
-    w_hi = min(w_hi, hi);
-    if (lo < hi) { k_begin = min(k_begin, lo); k_end = max(k_end, hi); }
-  }
+  // keys of the list, and the bounds inside which no row needs a mask
+  int k_begin, k_end, w_lo, w_hi;
+  if (!p.flat) {                                                 // both bounds grow from token to token
+    px_bounds(p, 0, n, ctx, false, k_begin, w_hi);
+    px_bounds(p, n - 1, n, ctx, false, w_lo, k_end);
+  } else {
+    k_begin = w_hi = 0x7fffffff;
+    k_end = w_lo = 0;
+    for (int t = lane; t < n; t += 32) {
+      int lo, hi;
+      px_bounds(p, t, n, ctx, hk == 0 && unit == 0 && warp == 0, lo, hi);
+      w_lo = max(w_lo, lo);
+      w_hi = min(w_hi, hi);
+      if (lo < hi) { k_begin = min(k_begin, lo); k_end = max(k_end, hi); }
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    k_begin = min(k_begin, __shfl_xor_sync(0xffffffffu, k_begin, o));
-    k_end = max(k_end, __shfl_xor_sync(0xffffffffu, k_end, o));
-    w_lo = max(w_lo, __shfl_xor_sync(0xffffffffu, w_lo, o));
-    w_hi = min(w_hi, __shfl_xor_sync(0xffffffffu, w_hi, o));
+    for (int o = 16; o > 0; o >>= 1) {
+      k_begin = min(k_begin, __shfl_xor_sync(0xffffffffu, k_begin, o));
+      k_end = max(k_end, __shfl_xor_sync(0xffffffffu, k_end, o));
+      w_lo = max(w_lo, __shfl_xor_sync(0xffffffffu, w_lo, o));
+      w_hi = min(w_hi, __shfl_xor_sync(0xffffffffu, w_hi, o));
+    }
   }
   const int tiles_all = k_end > k_begin ? (k_end - k_begin + kTile - 1) / kTile : 0;
   const int tile0 = static_cast<int>(static_cast<long long>(tiles_all) * unit / units);
@@ -718,30 +753,9 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
     if (page < 0 || page >= p.num_blocks) return -2;
     return (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + head_off;
   };
-  long long next = look_up(0);
-  auto load = [&](int i) {                                       // asks for tile i (past the last one: an empty group)
-    if (i < n_mine) {
-      const long long mine = next;
-      bad = bad || mine == -2;
-      next = look_up(i + 1);
-      const int c = lane % kChunks;
-      const uint32_t kd = ring + (i % kStages) * (2 * F::kKV);
+  long long ahead[kStages];
 #pragma unroll
-      for (int s = 0; s < kTile / kRowsPass; ++s) {
-        const int r = s * kRowsPass + lane / kChunks;
-        const long long at = __shfl_sync(0xffffffffu, mine, r);
-        const uint32_t bytes = at >= 0 ? 16 : 0;
-        const long long from = at >= 0 ? at + c * 8 : 0;
-        const uint32_t o = r * (D * 2) + ((c ^ (r & 7)) << 4);
-        px_cp16(kd + o, p.k_cache + from, bytes);
-        px_cp16(kd + F::kKV + o, p.v_cache + from, bytes);
-      }
-    }
-    px_cp_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) load(i);
-
+  for (int i = 0; i < kStages; ++i) ahead[i] = look_up(i);       // all the first tiles at once
   // Q^T as B operands: column = row of the list, k = dims
   uint32_t qf[KS][NT][2];
 #pragma unroll
@@ -755,6 +769,28 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) qf[ks][nt][e] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8)) : 0u;
   }
+
+  auto load = [&](int i, long long key_at) {                     // asks for tile i (past the last one: an empty group)
+    if (i < n_mine) {
+      bad = bad || key_at == -2;
+      const int c = lane % kChunks;
+      const uint32_t kd = ring + (i % kStages) * (2 * F::kKV);
+#pragma unroll
+      for (int s = 0; s < kTile / kRowsPass; ++s) {
+        const int r = s * kRowsPass + lane / kChunks;
+        const long long at = __shfl_sync(0xffffffffu, key_at, r);
+        const uint32_t bytes = at >= 0 ? 16 : 0;
+        const long long from = at >= 0 ? at + c * 8 : 0;
+        const uint32_t o = r * (D * 2) + ((c ^ (r & 7)) << 4);
+        px_cp16(kd + o, p.k_cache + from, bytes);
+        px_cp16(kd + F::kKV + o, p.v_cache + from, bytes);
+      }
+    }
+    px_cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load(i, ahead[i]);
+  long long next = ahead[kStages - 1];
 
   float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -771,7 +807,8 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
   const int vr = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
 
   for (int i = 0; i < n_mine; ++i) {
-    load(i + kStages - 1);
+    load(i + kStages - 1, next);
+    next = look_up(i + kStages);
     px_cp_wait<kStages - 1>();
     __syncwarp();                                                // every lane's copies of tile i are there
     const uint32_t ks_addr = ring + (i % kStages) * (2 * F::kKV), vs_addr = ks_addr + F::kKV;
@@ -793,24 +830,20 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
     }
     const int k0 = key0 + i * F::kWarps * kTile;
     if (k0 < w_lo || k0 + kTile > w_hi) {
-#pragma unroll 1
+#pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-#pragma unroll 1
+#pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + (lane & 3) * 2 + e;
+          // r / g; exact, since r < 64 and (r + 1/2) / g is at least 1 / (2 g) from a whole number
+          const int tok = static_cast<int>((static_cast<float>(r) + 0.5f) * inv_g);
           int lo = 0, hi = 0;
-          if (r < n_valid) px_bounds(p, r / g, n, ctx, false, lo, hi);
+          if (r < n_valid) px_bounds(p, tok, n, ctx, false, lo, hi);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             const int ka = k0 + mt * 16 + (lane >> 2);
-#pragma unroll
-            for (int q = 0; q < NT; ++q)                         // constant indices: s stays in registers
-#pragma unroll
-              for (int f = 0; f < 2; ++f)
-                if (q == nt && f == e) {
-                  if (ka < lo || ka >= hi) s[mt][q][f] = -INFINITY;
-                  if (ka + 8 < lo || ka + 8 >= hi) s[mt][q][2 + f] = -INFINITY;
-                }
+            if (ka < lo || ka >= hi) s[mt][nt][e] = -INFINITY;
+            if (ka + 8 < lo || ka + 8 >= hi) s[mt][nt][2 + e] = -INFINITY;
           }
         }
     }
@@ -887,8 +920,10 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
       }
     }
   __syncthreads();
+  const bool direct = p.splits == 1 && p.part_mode == 0;         // nothing to join but the warps
   for (int i = threadIdx.x; i < n_valid * (D / 8); i += F::kThreads) {
-    const int r = i / (D / 8), c = i % (D / 8);
+    const int r = i / (D / 8), c = i % (D / 8), tok = static_cast<int>((static_cast<float>(r) + 0.5f) * inv_g), h = hk * g + r - tok * g;
+    const float sink = direct ? px_sink(p, h) : -INFINITY;
     float mm = -1e30f;
     float2 ml[F::kWarps];
 #pragma unroll
@@ -897,16 +932,21 @@ __global__ void __launch_bounds__(128, 2) k_paged_few(const ExtendParams p) {
       if (ml[w].y > 0.f) mm = fmaxf(mm, ml[w].x);
     }
     PxSum t;
-    t.start(mm);
+    t.start(fmaxf(mm, sink));
 #pragma unroll
     for (int w = 0; w < F::kWarps; ++w) {
       const float4* src = reinterpret_cast<const float4*>(smem + w * F::kRing + (r * F::kOStride + c * 8) * 4);
       if (ml[w].y > 0.f) t.add(ml[w], src[0], src[1]);
     }
+    if (direct) {
+      t.store(p.out + (static_cast<long long>(start + tok) * p.hq + h) * D + c * 8, sink);
+      continue;
+    }
     reinterpret_cast<float4*>(sx + r * D)[(2 * c) ^ (r & 7)] = make_float4(t.acc[0], t.acc[1], t.acc[2], t.acc[3]);
     reinterpret_cast<float4*>(sx + r * D)[(2 * c + 1) ^ (r & 7)] = make_float4(t.acc[4], t.acc[5], t.acc[6], t.acc[7]);
     if (c == 0) reinterpret_cast<float2*>(s_ml)[r] = make_float2(mm, t.sum);
   }
+  if (direct) return;
   px_join<D, F::kThreads>(p, sx, s_ml, start, 0, n_valid, hk, unit);
 }
 
@@ -939,7 +979,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const ExtendParams p) {
 // How a call is cut: which kernel, tiles a list, CTAs the keys of a tile are split over.
 struct PxPlan {
   int nt;                 // > 0: the kernel for few rows, 8 * nt of them
-  long long tiles;
+  long long tiles, slots;
   int splits, groups;
 };
 
@@ -953,20 +993,23 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
   if (rows <= few_most) {
     const int t = static_cast<int>((rows + 7) / 8);
     q.nt = D == 64 ? (t == 4 ? 5 : t) : (t == 3 ? 4 : t);
-    slots = 296;
-    least = 2 * 4 * (2048 / D);
+    slots = 148 * (D == 64 ? (q.nt == 1 ? 4 : q.nt == 2 ? 3 : 2) : (q.nt == 1 ? 3 : 2));
+    least = 128;
   } else {
     q.tiles = (rows + PX_BM - 1) / PX_BM;
     slots = D == 64 ? 3 * 148 : 2 * 148;
     least = 4 * PX_BN;
   }
+  q.slots = slots;
   const long long base = q.tiles * lists * hkv;
   long long units = slots / (base > slots ? slots : base);
   const long long worth = keys / least;
   if (units > worth) units = worth;
   if (units < 1) units = 1;
   q.splits = 1;
-  while (q.splits < 8 && q.splits * 2 <= units) q.splits *= 2;
+  // large clusters leave SMs free that do not fill one; the kernel for few rows fits two CTAs best (99k keys: 84 us with 2,
+  // 113 with 8)
+  while (q.splits < (q.nt > 0 ? 2 : 8) && q.splits * 2 <= units) q.splits *= 2;
   q.groups = may_group && units >= 2 * q.splits ? static_cast<int>(units / q.splits) : 1;
   return q;
 }
@@ -1017,6 +1060,7 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
   if (q.tiles * q.splits * q.groups > 0x3fffffff) return -5;
   p.splits = q.splits;
   p.groups = q.groups;
+  p.sorted = !p.flat && lists > 1 && lists <= PX_SORT_MOST && q.tiles * q.splits * q.groups * p.hkv * lists > q.slots;
   const dim3 grid(static_cast<unsigned>(q.tiles) * q.splits * q.groups, p.hkv, lists);
   cudaError_t e;
   if (D == 64) {
