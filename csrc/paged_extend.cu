@@ -238,6 +238,7 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
       if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
     }
     if (p.part_mode == 2)
+#pragma unroll 8
       for (int s = 0; s < p.n_sets; ++s) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
         if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
@@ -252,12 +253,15 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
       if (ml.y > 0.f)
         t.add(ml, reinterpret_cast<const float4*>(xr)[(2 * c) ^ (r & 7)], reinterpret_cast<const float4*>(xr)[(2 * c + 1) ^ (r & 7)]);
     }
-    if (p.part_mode == 2)
-      for (int s = 0; s < p.n_sets; ++s) {
+    if (p.part_mode == 2) {
+#pragma unroll 4
+      for (int s = 0; s < p.n_sets; ++s) {                       // rows without keys hold zeros: nothing here waits for a comparison
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
         const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
-        if (ml.y > 0.f) t.add(ml, __ldcg(o), __ldcg(o + 1));
+        const float4 x = __ldcg(o), y = __ldcg(o + 1);
+        if (ml.y > 0.f) t.add(ml, x, y);
       }
+    }
     if (p.part_mode == 1) {
       const long long at = group * p.set_rows + row;
       float4* o = reinterpret_cast<float4*>(p.part_o + at * D) + 2 * c;
@@ -950,28 +954,47 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   px_join<D, F::kThreads>(p, sx, s_ml, start, 0, n_valid, hk, unit);
 }
 
-// Joins the sets of a launch that split the keys over several clusters; 8 columns a thread.
+// Joins the sets of a launch that split the keys over several clusters: a CTA for each row, D / 8 threads for its columns,
+// the others for other sets (dozens of them for a single long context: one after the other they took 32 us).
 template <int D>
-__global__ void __launch_bounds__(256) k_paged_join(const ExtendParams p) {
-  px_wait_prior_grid();
-  const int b = blockIdx.y;
+__global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
+  constexpr int kCols = D / 8, kParts = 128 / kCols;
+  __shared__ float s_max[4], s_acc[kParts][kCols][9];
+  const int b = blockIdx.y, c = threadIdx.x % kCols, part = threadIdx.x / kCols;
+  const int h = static_cast<int>(blockIdx.x) % p.hq, tok = static_cast<int>(blockIdx.x) / p.hq;
   int start, n, ctx;
   px_list(p, b, false, start, n, ctx);
-  const int i = blockIdx.x * 256 + threadIdx.x, c = i % (D / 8), h = i / (D / 8) % p.hq, tok = i / (D / 8) / p.hq;
-  if (tok >= n) return;
+  px_wait_prior_grid();
+  if (tok >= n) return;                                          // the whole CTA
   const long long row = static_cast<long long>(start + tok) * p.hq + h;
   const float sink = px_sink(p, h);
   float mm = -1e30f;
-  for (int s = 0; s < p.n_sets; ++s) {
+  for (int s = threadIdx.x; s < p.n_sets; s += 128) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
     if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
   }
+  mm = warp_max(mm);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mm;
+  __syncthreads();
   PxSum t;
-  t.start(fmaxf(mm, sink));
-  for (int s = 0; s < p.n_sets; ++s) {
+  t.start(fmaxf(px_max3(s_max[0], s_max[1], s_max[2]), fmaxf(s_max[3], sink)));
+#pragma unroll 4
+  for (int s = part; s < p.n_sets; s += kParts) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
     const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
-    if (ml.y > 0.f) t.add(ml, __ldcg(o), __ldcg(o + 1));
+    const float4 x = __ldcg(o), y = __ldcg(o + 1);
+    if (ml.y > 0.f) t.add(ml, x, y);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s_acc[part][c][e] = t.acc[e];
+  s_acc[part][c][8] = t.sum;
+  __syncthreads();
+  if (part > 0) return;
+#pragma unroll
+  for (int q = 1; q < kParts; ++q) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t.acc[e] += s_acc[q][c][e];
+    t.sum += s_acc[q][c][8];
   }
   t.store(p.out + row * D + c * 8, sink);
 }
@@ -1157,9 +1180,8 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
     if (rc != 0) return rc;
     p.part_mode = 2;
     p.splits = 1;
-    const long long pieces = static_cast<long long>(max_q_len) * Hq * (D / 8);
-    const dim3 grid(static_cast<unsigned>((pieces + 255) / 256), B);
-    const cudaError_t e = D == 64 ? px_launch<k_paged_join<64>>(p, grid, 256, 0, true, st) : px_launch<k_paged_join<128>>(p, grid, 256, 0, true, st);
+    const dim3 grid(static_cast<unsigned>(max_q_len) * Hq, B);
+    const cudaError_t e = D == 64 ? px_launch<k_paged_join<64>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128>>(p, grid, 128, 0, true, st);
     return e == cudaSuccess ? 0 : static_cast<int>(e);
   }
   ExtendParams f = p;

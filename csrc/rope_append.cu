@@ -18,6 +18,9 @@
 namespace nmoe {
 
 constexpr int kRopeThreads = 256;
+#ifndef ROPE_TPB
+#define ROPE_TPB 4
+#endif
 
 struct RopeAppendParams {
   const __nv_bfloat16* qkv;          // [N, (Hq + 2 Hkv) * D], rows qkv_stride apart
@@ -111,8 +114,9 @@ extern "C" int nmoe_rope_append(const void* qkv, long long qkv_stride, const voi
   p.q_out = static_cast<__nv_bfloat16*>(q_out); p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.v_out = static_cast<__nv_bfloat16*>(v_out); p.status = static_cast<StatusRecord*>(status);
   p.qkv_stride = qkv_stride; p.n_slots = n_slots; p.n_tokens = n_tokens; p.hq = hq; p.hkv = hkv; p.d = d;
-  p.pos64 = pos64; p.conc = conc; p.tokens_per_block = 1;
-  k_rope_append<<<n_tokens, kRopeThreads, p.tokens_per_block * (d / 2) * sizeof(float2), st>>>(p);
+  p.pos64 = pos64; p.conc = conc;
+  p.tokens_per_block = n_tokens >= 148 * 8 * 4 ? ROPE_TPB : 1;
+  k_rope_append<<<(n_tokens + p.tokens_per_block - 1) / p.tokens_per_block, kRopeThreads, p.tokens_per_block * (d / 2) * sizeof(float2), st>>>(p);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }

@@ -9,8 +9,10 @@
 // on how a row is split except where u * total falls within 1e-15 of a border.
 //
 // One row of V probabilities per sequence (two with a draft distribution) is all that has to be read: bandwidth for
-// many sequences, latency for one.  A cluster of CTAs shares a row, each warp owns a contiguous stretch; the sums meet
-// through distributed shared memory, and the warp whose stretch holds the crossing walks it once more from the L2.
+// many sequences, latency for one.  A cluster of CTAs shares a row, each warp owns a contiguous stretch that it reads in
+// batches of 512 entries (loads of a batch issued together: entry by entry the loop waited for memory 25 times a
+// stretch) and keeps the sum of every step of them; the CTAs' sums meet through distributed shared memory, and the warp
+// whose stretch holds the crossing walks one step of it once more from the L2.
 // No workspace, no atomics on global memory, the same result for every run.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -24,7 +26,9 @@ namespace nmoe {
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyMaxCluster = 8;
+constexpr int kVerifyMaxCluster = 16;
+constexpr int kVerifyBatch = 4;         // groups of 128 entries that a warp reads at once
+constexpr int kVerifySteps = 32;        // sums that a warp keeps of its stretch
 
 struct VerifyParams {
   const float* target;        // [N, V], rows target_stride apart
@@ -53,13 +57,13 @@ NMOE_DEVICE double verify_weight(float pv, float qv) {
   return d > 0.0 ? d : 0.0;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) k_verify_draft(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) k_verify_draft(const VerifyParams p) {
   cg::cluster_group cl = cg::this_cluster();
   const int n_cta = cl.num_blocks(), rank = cl.block_rank();
   const int b = blockIdx.x / n_cta;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int s_first;
-  __shared__ double s_warp[kVerifyWarps];
+  __shared__ double s_warp[kVerifyWarps], s_step[kVerifyWarps][kVerifySteps];
   __shared__ double s_all[2][kVerifyMaxCluster];        // every CTA's sum, written by the CTAs themselves; one row per attempt
   const int start = p.q_starts[b], n = p.q_lens[b];
   const bool fits = start >= 0 && n >= 0 && start <= p.n_rows && n <= p.n_rows - start;
@@ -99,31 +103,50 @@ __global__ void __launch_bounds__(kVerifyThreads) k_verify_draft(const VerifyPar
   const int groups = (p.vocab + 3) >> 2, n_warps = n_cta * kVerifyWarps;
   const int per = (groups + n_warps - 1) / n_warps, w = rank * kVerifyWarps + warp;
   const int v0 = min(p.vocab, w * per * 4), v1 = min(p.vocab, (w + 1) * per * 4);
-  auto load4 = [&](int v, double* o) {                  // weights of v .. v+3, 0 past the end
-    float pv[4] = {0.f, 0.f, 0.f, 0.f}, qv[4] = {0.f, 0.f, 0.f, 0.f};
+  auto read4 = [&](const float* src, int v, float (&o)[4]) {            // entries v .. v+3, 0 past the end of the stretch
     if (p.vec && v + 4 <= v1) {
-      *reinterpret_cast<float4*>(pv) = *reinterpret_cast<const float4*>(tp + v);
-      if (dp != nullptr) *reinterpret_cast<float4*>(qv) = *reinterpret_cast<const float4*>(dp + v);
+      const float4 f = *reinterpret_cast<const float4*>(src + v);
+      o[0] = f.x; o[1] = f.y; o[2] = f.z; o[3] = f.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (v + i < v1) { pv[i] = tp[v + i]; if (dp != nullptr) qv[i] = dp[v + i]; }
+      for (int i = 0; i < 4; ++i) o[i] = v + i < v1 ? src[v + i] : 0.f;
     }
+  };
+  auto weights = [&](int v, const float (&pv)[4], const float (&qv)[4], double (&o)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = v + i == hole ? 0.0 : verify_weight(pv[i], qv[i]);
   };
+  constexpr int kBatch = kVerifyBatch * 128;
+  const int batches = (per * 4 + kBatch - 1) / kBatch, per_step = (batches + kVerifySteps - 1) / kVerifySteps * kBatch;   // entries
   double total = 0.0;
   int attempt = 0;
   cl.barrier_wait();
   for (;; ++attempt) {
     double sum = 0.0;
-#pragma unroll 4
-    for (int v = v0 + lane * 4; v < v1; v += 128) {
-      double o[4];
-      load4(v, o);
-      sum += (o[0] + o[1]) + (o[2] + o[3]);
+    for (int v = v0, step = 0; v < v1; v += per_step, ++step) {
+      double mine = 0.0;
+      for (int w = v; w < min(v1, v + per_step); w += kBatch) {
+        float pv[kVerifyBatch][4], qv[kVerifyBatch][4];
+#pragma unroll
+        for (int u = 0; u < kVerifyBatch; ++u) read4(tp, w + u * 128 + lane * 4, pv[u]);
+        if (dp != nullptr) {
+#pragma unroll
+          for (int u = 0; u < kVerifyBatch; ++u) read4(dp, w + u * 128 + lane * 4, qv[u]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kVerifyBatch; ++u) qv[u][0] = qv[u][1] = qv[u][2] = qv[u][3] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kVerifyBatch; ++u) {
+          double o[4];
+          weights(w + u * 128 + lane * 4, pv[u], qv[u], o);
+          mine += (o[0] + o[1]) + (o[2] + o[3]);
+        }
+      }
+      mine = verify_warp_sum(mine);
+      if (lane == 0) s_step[warp][step] = mine;
+      sum += mine;
     }
-    sum = verify_warp_sum(sum);
     if (lane == 0) s_warp[warp] = sum;
     __syncthreads();
     if (threadIdx.x < n_cta) {
@@ -156,11 +179,23 @@ __global__ void __launch_bounds__(kVerifyThreads) k_verify_draft(const VerifyPar
       run += s;
     }
     if (pw == warp) {
+      __syncwarp();                                     // the step sums of lane 0
+      int at_step = 0;
+      double run2 = wbase;
+      for (int i = 0; v0 + i * per_step < v1; ++i) {
+        const double s = s_step[warp][i];
+        if (s > 0.0) { at_step = i; wbase = run2; if (run2 + s > goal) break; }
+        run2 += s;
+      }
       int found = -1, last = -1;
-      for (int v = v0; v < v1 && found < 0; v += 128) {
-        double o[4] = {0.0, 0.0, 0.0, 0.0};
+      const int e0 = v0 + at_step * per_step, e1 = min(v1, e0 + per_step);
+      for (int v = e0; v < e1 && found < 0; v += 128) {
+        double o[4];
         const int at = v + lane * 4;
-        if (at < v1) load4(at, o);
+        float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
+        read4(tp, at, pv);
+        if (dp != nullptr) read4(dp, at, qv);
+        weights(at, pv, qv, o);
         const double mine = (o[0] + o[1]) + (o[2] + o[3]);
         double inc = mine;
 #pragma unroll
@@ -212,7 +247,7 @@ extern "C" int nmoe_verify_draft(const float* target, long long target_stride, c
   p.vec = (reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) % 16 == 0 &&
           (target_stride | draft_stride) % 4 == 0;
   int cluster = 1;
-  while (cluster < kVerifyMaxCluster && n_seqs * cluster * 2 <= 296 && vocab >= cluster * 2 * kVerifyThreads * 4) cluster *= 2;
+  while (cluster < kVerifyMaxCluster && n_seqs * cluster * 2 <= 296 && vocab >= cluster * 2 * 4096) cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(n_seqs) * cluster);
   cfg.blockDim = dim3(kVerifyThreads);
@@ -221,7 +256,9 @@ extern "C" int nmoe_verify_draft(const float* target, long long target_stride, c
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, k_verify_draft, p);
+  cudaError_t e = cudaSuccess;
+  if (cluster > 8) e = cudaFuncSetAttribute(k_verify_draft, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, k_verify_draft, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
