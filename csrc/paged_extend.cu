@@ -137,6 +137,9 @@ NMOE_DEVICE void px_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) 
 NMOE_DEVICE void px_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 NMOE_DEVICE void px_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// x / g for x below g + 128 and 2^22, from 1 / g: (x + 1/2) / g is at least 1 / (2 g) from a whole number
+NMOE_DEVICE int px_div(int x, float inv_g) { return static_cast<int>((static_cast<float>(x) + 0.5f) * inv_g); }
+
 // Rows of one list: its first row, its number of tokens (0 where the lengths are out of range) and its context.
 NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start, int& n, int& ctx) {
   start = 0;
@@ -233,10 +236,15 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
     const long long row = static_cast<long long>(start + tok) * p.hq + h;
     const float sink = p.part_mode == 1 ? -INFINITY : px_sink(p, h);
     float mm = -1e30f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(splits > 1 ? cl.map_shared_rank(s_ml + 2 * r, s) : s_ml + 2 * r);
-      if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+    float2 ml[8];                                                // all loads before the first use: a remote read takes some 200 cycles
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      ml[s] = make_float2(0.f, 0.f);
+      if (s < splits) ml[s] = *reinterpret_cast<const float2*>(splits > 1 ? cl.map_shared_rank(s_ml + 2 * r, s) : s_ml + 2 * r);
     }
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (ml[s].y > 0.f) mm = fmaxf(mm, ml[s].x);
     if (p.part_mode == 2)
 #pragma unroll 8
       for (int s = 0; s < p.n_sets; ++s) {
@@ -245,13 +253,20 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
       }
     PxSum t;
     t.start(fmaxf(mm, sink));
-    for (int s = 0; s < splits; ++s) {
-      const float* xr = sx + r * D;
-      const float* mr = s_ml + 2 * r;
-      if (splits > 1) { xr = cl.map_shared_rank(xr, s); mr = cl.map_shared_rank(mr, s); }
-      const float2 ml = *reinterpret_cast<const float2*>(mr);
-      if (ml.y > 0.f)
-        t.add(ml, reinterpret_cast<const float4*>(xr)[(2 * c) ^ (r & 7)], reinterpret_cast<const float4*>(xr)[(2 * c + 1) ^ (r & 7)]);
+#pragma unroll
+    for (int s0 = 0; s0 < 8; s0 += 4) {
+      if (s0 >= splits) break;
+      float4 x[4], y[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s0 + s < splits) {
+          const float4* xr = reinterpret_cast<const float4*>(splits > 1 ? cl.map_shared_rank(sx + r * D, s0 + s) : sx + r * D);
+          x[s] = xr[(2 * c) ^ (r & 7)];
+          y[s] = xr[(2 * c + 1) ^ (r & 7)];
+        }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s0 + s < splits && ml[s0 + s].y > 0.f) t.add(ml[s0 + s], x[s], y[s]);
     }
     if (p.part_mode == 2) {
 #pragma unroll 4
@@ -282,11 +297,10 @@ struct PxSmem {
   static constexpr int kBufs = D == 64 ? 1 : 2;            // S buffers of 64 columns
   static constexpr int kLoaders = 64;                      // threads
   static constexpr int kThreads = 4 * 32 + 32 + kLoaders;
-  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kSlots = D == 64 ? 6 : 4;           // of the ring; K and V of a block take one each, so that K's is free after S
   static constexpr int kQ = PX_BM * D * 2;
-  static constexpr int kKV = PX_BN * D * 2;                // one of K, V
-  static constexpr int kStage = 2 * kKV;
-  static constexpr int kRing = kStages * kStage;
+  static constexpr int kKV = PX_BN * D * 2;                // a slot
+  static constexpr int kRing = kSlots * kKV;
   static constexpr int kExchange = PX_BM * (D + 2) * 4;
   static constexpr int kBody = kRing > kExchange ? kRing : kExchange;
   static constexpr int kBytes = kQ + kBody + 256 + 1024;
@@ -296,8 +310,8 @@ struct PxSmem {
 template <int D>
 __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged_extend(const ExtendParams p) {
   using SM = PxSmem<D>;
-  constexpr int kStages = SM::kStages, kBufs = SM::kBufs;
-  constexpr int kLag = kStages - 1;          // see the loader
+  constexpr int kSlots = SM::kSlots, kBufs = SM::kBufs;
+  constexpr int kLag = kSlots - 2;           // see the loader
   constexpr int kThreads = SM::kThreads;
   constexpr int kMmaWarp = 4;
   constexpr uint32_t kTmemO = kBufs * PX_BN;
@@ -306,9 +320,9 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + SM::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SM::kBody);
-  uint64_t* kv_full = bars;                  // [kStages]
-  uint64_t* kv_empty = kv_full + kStages;    // [kStages]
-  uint64_t* s_full = kv_empty + kStages;     // [kBufs]
+  uint64_t* kv_full = bars;                  // [kSlots]
+  uint64_t* kv_empty = kv_full + kSlots;     // [kSlots]
+  uint64_t* s_full = kv_empty + kSlots;      // [kBufs]
   uint64_t* p_full = s_full + kBufs;         // [kBufs]
   uint64_t* pv_done = p_full + kBufs;
   uint64_t* o_full = pv_done + 1;
@@ -327,6 +341,7 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   int start, n, ctx;
   px_list(p, b, tile_x == 0 && unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
   const int row0 = tile_x * PX_BM;                               // first row of this CTA's tile
+  const float inv_g = 1.f / static_cast<float>(g);
   const int n_valid = min(PX_BM, n * g - row0);                  // rows that exist
   if (n_valid <= 0) {                                            // uniform over the cluster
     if (p.part_mode == 1) px_launch_dependents();
@@ -336,7 +351,7 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   const int* table = p.block_tables + b * p.bt_stride;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) { mbar_init(&kv_full[i], SM::kLoaders / 32); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < kSlots; ++i) { mbar_init(&kv_full[i], SM::kLoaders / 32); mbar_init(&kv_empty[i], 1); }
     for (int i = 0; i < kBufs; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], (n_valid + 31) / 32); }
     mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
@@ -357,14 +372,25 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   // SM: the busy warps of tiles with few rows then sit on different schedulers.
   const int turn = static_cast<int>((tmem_base & 511u) / SM::kTmemCols) * (4 / SM::kBufs / 2 + 1) & 3;
   // rows of Q, 128-byte swizzle, K-major; rows that do not exist are zero
-  for (int i = threadIdx.x; i < PX_BM * (D / 8); i += kThreads) {
-    const int r = i / (D / 8), c = i % (D / 8), rr = row0 + r, at = (r + 32 * turn) & 127;
-    int4 v = make_int4(0, 0, 0, 0);
-    if (r < n_valid) {
-      const int tok = rr / g, h = hk * g + rr - tok * g;
-      v = ld_nc_v4(p.q + (start + tok) * p.q_stride + static_cast<long long>(h) * D + c * 8);
+  {
+    constexpr int kPieces = PX_BM * (D / 8), kEach = (kPieces + kThreads - 1) / kThreads;
+    const int tok0 = row0 / g, rem0 = row0 - tok0 * g;
+    int4 v[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {                            // all loads of a thread before the first store
+      const int i = threadIdx.x + k * kThreads, r = i / (D / 8), c = i % (D / 8);
+      v[k] = make_int4(0, 0, 0, 0);
+      if (i < kPieces && r < n_valid) {
+        const int dt = px_div(rem0 + r, inv_g), h = hk * g + rem0 + r - dt * g;
+        v[k] = ld_nc_v4(p.q + (start + tok0 + dt) * p.q_stride + static_cast<long long>(h) * D + c * 8);
+      }
     }
-    *reinterpret_cast<int4*>(sQ + (c >> 3) * (PX_BM * 128) + at * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = threadIdx.x + k * kThreads, r = i / (D / 8), c = i % (D / 8), at = (r + 32 * turn) & 127;
+      if (i < kPieces)
+        *reinterpret_cast<int4*>(sQ + (c >> 3) * (PX_BM * 128) + at * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+    }
   }
   fence_proxy_async_smem();
   // every CTA holds its tensor memory before a dependent launch may ask for some
@@ -391,63 +417,60 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   bool ok = true;
   float m = -1e30f, l = 0.f;
   if (warp > kMmaWarp) {
-    // ------------------------------------------------------------ loaders: K and V rows of a block from their pages
-    // Blocks are announced in order once they have landed: normally kLag blocks after they were asked for, all at once
-    // when the ring is full, since the block that would make room may be waiting for one of them.
+    // ------------------------------------------------------------ loaders: K, then V rows of a block from their pages
+    // Slots are announced in order once they have landed: normally kLag later than they were asked for, all at once when
+    // the ring is full, since what would make room may be waiting for one of them.
     // Each warp owns kRowsWarp keys of a block; a lane looks one of them up (a block ahead, so that the page table's
-    // latency is covered) and the warp shares the addresses by shuffle: a lookup per copied piece took 2500 cycles a block.
+    // latency is covered) and the warp shares the rows by shuffle: a lookup per copied piece took 2500 cycles a block.
     constexpr int kChunks = D / 8, kRowsWarp = PX_BN / (SM::kLoaders / 32), kRowsPass = 32 / kChunks;
     static_assert(kRowsWarp <= 32 && kRowsWarp % kRowsPass == 0, "one lookup per lane");
     const int lw = warp - kMmaWarp - 1;
     const int c = lane % kChunks, rp = lane / kChunks;
-    const long long row_elems = static_cast<long long>(p.hkv) * D;
-    const long long head_off = static_cast<long long>(hk) * D;
-    auto look_up = [&](int i) -> long long {                     // element offset of this lane's key in block i, -1: zeros
+    const long long row_bytes = static_cast<long long>(p.hkv) * D * 2, piece = (static_cast<long long>(hk) * D + c * 8) * 2;
+    auto look_up = [&](int i) -> int {                           // cache row of this lane's key in block i, -1: zeros, -2: no such page
       const int key = key0 + i * PX_BN + lw * kRowsWarp + lane;
       if (lane >= kRowsWarp || i >= n_blk || key >= k_end) return -1;
       const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
       const int page = __ldg(table + pi);
-      if (page < 0 || page >= p.num_blocks) return -2;
-      return (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + head_off;
+      return page < 0 || page >= p.num_blocks ? -2 : page * p.block_size + (key - pi * p.block_size);
     };
-    long long next = look_up(0);
+    int next = look_up(0), mine = -1;
     bool bad = false;
-    int told = 0;                                                // blocks announced so far
-    auto announce = [&](int upto) {                              // this thread's copies of the blocks before upto have landed
+    int told = 0;                                                // slots announced so far
+    auto announce = [&](int upto) {                              // this thread's copies for the slots before upto have landed
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
-        for (int t = told; t < upto; ++t) mbar_arrive(&kv_full[t % kStages]);
+        for (int t = told; t < upto; ++t) mbar_arrive(&kv_full[t % kSlots]);
       told = upto;
     };
-    for (int i = 0; i < n_blk && ok; ++i) {
-      const int st = i % kStages;
-      const uint32_t empty_ph = ((i / kStages) & 1) ^ 1;
+    for (int h = 0; h < 2 * n_blk && ok; ++h) {                  // K of block h / 2, then its V
+      const int st = h % kSlots;
+      const uint32_t empty_ph = ((h / kSlots) & 1) ^ 1;
       if (!__all_sync(0xffffffffu, px_test(&kv_empty[st], empty_ph))) {
-        if (told < i) { px_cp_wait<0>(); announce(i); }
+        if (told < h) { px_cp_wait<0>(); announce(h); }
         ok = px_wait(&kv_empty[st], empty_ph, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, 0); *abort_flag = 1; break; }
+        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, h, 0); *abort_flag = 1; break; }
       }
-      const uint32_t kd = smem_u32(sKV + st * SM::kStage), vd = kd + SM::kKV;
-      const long long mine = next;
-      bad = bad || mine == -2;
-      next = look_up(i + 1);
+      if ((h & 1) == 0) {
+        mine = next;
+        bad = bad || mine == -2;
+        next = look_up((h >> 1) + 1);
+      }
+      const uint32_t dst = smem_u32(sKV + st * SM::kKV);
+      const uint8_t* src = reinterpret_cast<const uint8_t*>((h & 1) != 0 ? p.v_cache : p.k_cache) + piece;
 #pragma unroll
       for (int s = 0; s < kRowsWarp / kRowsPass; ++s) {
         const int rw = s * kRowsPass + rp, r = lw * kRowsWarp + rw;
-        const long long at = __shfl_sync(0xffffffffu, mine, rw);
-        const uint32_t bytes = at >= 0 ? 16 : 0;
-        const long long from = at >= 0 ? at + c * 8 : 0;
-        const uint32_t o = (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        px_cp16(kd + o, p.k_cache + from, bytes);
-        px_cp16(vd + o, p.v_cache + from, bytes);
+        const int row = __shfl_sync(0xffffffffu, mine, rw);
+        px_cp16(dst + (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + max(row, 0) * row_bytes, row >= 0 ? 16u : 0u);
       }
       px_cp_commit();
-      if (i - kLag >= told) { px_cp_wait<kLag>(); announce(i - kLag + 1); }
+      if (h - kLag >= told) { px_cp_wait<kLag>(); announce(h - kLag + 1); }
     }
     px_cp_wait<0>();
-    if (ok && told < n_blk) announce(n_blk);
+    if (ok && told < 2 * n_blk) announce(2 * n_blk);
     if (bad) report_status(p.status, kStatusBadIndex, 1022, b, 0);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issue
@@ -456,23 +479,25 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
       constexpr uint32_t idesc_pv = make_idesc_bf16(PX_BM, D, 0, 1);
       const uint64_t qa = make_smem_desc(smem_u32(sQ), 0, 1024, kSwizzle128B);
       auto issue_s = [&](int i) -> bool {
-        const int st = i % kStages;
-        if (!px_wait(&kv_full[st], (i / kStages) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1031, i, 0); *abort_flag = 1; return false; }
+        const int st = 2 * i % kSlots;
+        if (!px_wait(&kv_full[st], (2 * i / kSlots) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1031, i, 0); *abort_flag = 1; return false; }
         tc_fence_after_sync();
-        const uint64_t ka = make_smem_desc(smem_u32(sKV + st * SM::kStage), 0, 1024, kSwizzle128B);
+        const uint64_t ka = make_smem_desc(smem_u32(sKV + st * SM::kKV), 0, 1024, kSwizzle128B);
         const uint32_t d = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
           mma_f16_ss(d, qa + (((j >> 2) * (PX_BM * 128) + (j & 3) * 32) >> 4), ka + (((j >> 2) * (PX_BN * 128) + (j & 3) * 32) >> 4),
                      idesc_s, j != 0 ? 1u : 0u);
         mma_commit(&s_full[i % kBufs]);
+        mma_commit(&kv_empty[st]);
         return true;
       };
       bool good = n_blk > 0 && issue_s(0);
       for (int i = 0; good && i < n_blk; ++i) {
         if (kBufs == 2 && i + 1 < n_blk) { good = issue_s(i + 1); if (!good) break; }
-        const int st = i % kStages;
-        const uint64_t va = make_smem_desc(smem_u32(sKV + st * SM::kStage + SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
+        const int st = (2 * i + 1) % kSlots;
+        const uint64_t va = make_smem_desc(smem_u32(sKV + st * SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
+        if (!px_wait(&kv_full[st], ((2 * i + 1) / kSlots) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1038, i, 0); *abort_flag = 1; break; }
         if (!px_wait(&p_full[i % kBufs], (i / kBufs) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1032, i, 0); *abort_flag = 1; break; }
         tc_fence_after_sync();
         const uint32_t a_t = tmem_base + (i % kBufs) * PX_BN;
@@ -747,17 +772,16 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   // loads: a lane looks one key up, the warp shares the addresses; a tile ahead, so that the lookup's latency is covered
   constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
   const uint32_t ring = smem_u32(smem + warp * F::kRing);
-  const long long row_elems = static_cast<long long>(p.hkv) * D, head_off = static_cast<long long>(hk) * D;
+  const long long row_bytes = static_cast<long long>(p.hkv) * D * 2, piece = (static_cast<long long>(hk) * D + lane % kChunks * 8) * 2;
   bool bad = false;
-  auto look_up = [&](int i) -> long long {
+  auto look_up = [&](int i) -> int {                             // cache row of this lane's key in tile i, -1: zeros, -2: no such page
     const int key = key0 + i * F::kWarps * kTile + lane;
     if (lane >= kTile || i >= n_mine || key >= k_end) return -1;
     const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
     const int page = __ldg(table + pi);
-    if (page < 0 || page >= p.num_blocks) return -2;
-    return (static_cast<long long>(page) * p.block_size + (key - pi * p.block_size)) * row_elems + head_off;
+    return page < 0 || page >= p.num_blocks ? -2 : page * p.block_size + (key - pi * p.block_size);
   };
-  long long ahead[kStages];
+  int ahead[kStages];
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ahead[i] = look_up(i);       // all the first tiles at once
   // Q^T as B operands: column = row of the list, k = dims
@@ -774,27 +798,27 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
       for (int e = 0; e < 2; ++e) qf[ks][nt][e] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8)) : 0u;
   }
 
-  auto load = [&](int i, long long key_at) {                     // asks for tile i (past the last one: an empty group)
+  auto load = [&](int i, int row_of) {                           // asks for tile i (past the last one: an empty group)
     if (i < n_mine) {
-      bad = bad || key_at == -2;
+      bad = bad || row_of == -2;
       const int c = lane % kChunks;
       const uint32_t kd = ring + (i % kStages) * (2 * F::kKV);
+      const uint8_t *ksrc = reinterpret_cast<const uint8_t*>(p.k_cache) + piece, *vsrc = reinterpret_cast<const uint8_t*>(p.v_cache) + piece;
 #pragma unroll
       for (int s = 0; s < kTile / kRowsPass; ++s) {
         const int r = s * kRowsPass + lane / kChunks;
-        const long long at = __shfl_sync(0xffffffffu, key_at, r);
-        const uint32_t bytes = at >= 0 ? 16 : 0;
-        const long long from = at >= 0 ? at + c * 8 : 0;
-        const uint32_t o = r * (D * 2) + ((c ^ (r & 7)) << 4);
-        px_cp16(kd + o, p.k_cache + from, bytes);
-        px_cp16(kd + F::kKV + o, p.v_cache + from, bytes);
+        const int row = __shfl_sync(0xffffffffu, row_of, r);
+        const long long from = max(row, 0) * row_bytes;
+        const uint32_t bytes = row >= 0 ? 16u : 0u, o = r * (D * 2) + ((c ^ (r & 7)) << 4);
+        px_cp16(kd + o, ksrc + from, bytes);
+        px_cp16(kd + F::kKV + o, vsrc + from, bytes);
       }
     }
     px_cp_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load(i, ahead[i]);
-  long long next = ahead[kStages - 1];
+  int next = ahead[kStages - 1];
 
   float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -839,8 +863,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + (lane & 3) * 2 + e;
-          // r / g; exact, since r < 64 and (r + 1/2) / g is at least 1 / (2 g) from a whole number
-          const int tok = static_cast<int>((static_cast<float>(r) + 0.5f) * inv_g);
+          const int tok = px_div(r, inv_g);
           int lo = 0, hi = 0;
           if (r < n_valid) px_bounds(p, tok, n, ctx, false, lo, hi);
 #pragma unroll
@@ -926,7 +949,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   __syncthreads();
   const bool direct = p.splits == 1 && p.part_mode == 0;         // nothing to join but the warps
   for (int i = threadIdx.x; i < n_valid * (D / 8); i += F::kThreads) {
-    const int r = i / (D / 8), c = i % (D / 8), tok = static_cast<int>((static_cast<float>(r) + 0.5f) * inv_g), h = hk * g + r - tok * g;
+    const int r = i / (D / 8), c = i % (D / 8), tok = px_div(r, inv_g), h = hk * g + r - tok * g;
     const float sink = direct ? px_sink(p, h) : -INFINITY;
     float mm = -1e30f;
     float2 ml[F::kWarps];
@@ -1151,7 +1174,7 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
   if (D != 64 && D != 128) return -2;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0 || (n_rows > 1 && q_stride % 8 != 0)) return -3;
-  if (static_cast<long long>(n_rows) * Hq > 0x7fffffffll / (D / 8) - 256) return -4;
+  if (static_cast<long long>(n_rows) * Hq > 0x7fffffffll / (D / 8) - 256 || static_cast<long long>(num_blocks) * block_size > 0x7fffffffll) return -4;
   if (prefix_len > 0 && (q_starts != nullptr || q_lens != nullptr)) return -5;
   if (workspace_floats < nmoe_paged_extend_workspace(n_rows, B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len)) return -6;
   const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
