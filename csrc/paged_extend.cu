@@ -20,6 +20,7 @@
 // sequences, partial (m, l, O) to a workspace), a dependent launch for each sequence's own keys that starts while the
 // first one drains and joins its rows at the end.
 #include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -27,6 +28,7 @@
 #include <atomic>
 
 #include "common/ptx.cuh"
+#include "common/tensormap.h"
 
 namespace cg = cooperative_groups;
 
@@ -53,6 +55,7 @@ struct ExtendParams {
   int sorted;                         // 1: lists by falling context
   int part_mode;                      // 0 none, 1 write partial results (one set per group), 2 join those of the launch before
   int n_sets;                         // sets of partial results to join
+  int tma_rows;                       // keys of a TMA box, 0: the page size does not allow it
   long long set_rows;                 // rows of a set
   float scale_log2;
 };
@@ -297,10 +300,10 @@ struct PxSmem {
   static constexpr int kBufs = D == 64 ? 1 : 2;            // S buffers of 64 columns
   static constexpr int kLoaders = 64;                      // threads
   static constexpr int kThreads = 4 * 32 + 32 + kLoaders;
-  static constexpr int kSlots = D == 64 ? 6 : 4;           // of the ring; K and V of a block take one each, so that K's is free after S
+  static constexpr int kStages = D == 64 ? 3 : 2;          // of K and of V
   static constexpr int kQ = PX_BM * D * 2;
-  static constexpr int kKV = PX_BN * D * 2;                // a slot
-  static constexpr int kRing = kSlots * kKV;
+  static constexpr int kKV = PX_BN * D * 2;                // a stage of one of them
+  static constexpr int kRing = 2 * kStages * kKV;
   static constexpr int kExchange = PX_BM * (D + 2) * 4;
   static constexpr int kBody = kRing > kExchange ? kRing : kExchange;
   static constexpr int kBytes = kQ + kBody + 256 + 1024;
@@ -308,10 +311,11 @@ struct PxSmem {
 };
 
 template <int D>
-__global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged_extend(const ExtendParams p) {
+__global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas)
+k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using SM = PxSmem<D>;
-  constexpr int kSlots = SM::kSlots, kBufs = SM::kBufs;
-  constexpr int kLag = kSlots - 2;           // see the loader
+  constexpr int kStages = SM::kStages, kBufs = SM::kBufs;
+  constexpr int kLag = kStages - 1;          // see the loaders
   constexpr int kThreads = SM::kThreads;
   constexpr int kMmaWarp = 4;
   constexpr uint32_t kTmemO = kBufs * PX_BN;
@@ -320,9 +324,9 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + SM::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SM::kBody);
-  uint64_t* kv_full = bars;                  // [kSlots]
-  uint64_t* kv_empty = kv_full + kSlots;     // [kSlots]
-  uint64_t* s_full = kv_empty + kSlots;      // [kBufs]
+  uint64_t* kv_full = bars;                  // [K, V][kStages]
+  uint64_t* kv_empty = kv_full + 2 * kStages;
+  uint64_t* s_full = kv_empty + 2 * kStages; // [kBufs]
   uint64_t* p_full = s_full + kBufs;         // [kBufs]
   uint64_t* pv_done = p_full + kBufs;
   uint64_t* o_full = pv_done + 1;
@@ -351,7 +355,7 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   const int* table = p.block_tables + b * p.bt_stride;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(&kv_full[i], SM::kLoaders / 32); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < 2 * kStages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
     for (int i = 0; i < kBufs; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], (n_valid + 31) / 32); }
     mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
@@ -409,68 +413,117 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
   }
   __syncthreads();
   const int k_begin = s_range[0], k_end = s_range[1];
-  const int n_blocks_all = k_end > k_begin ? (k_end - k_begin + PX_BN - 1) / PX_BN : 0;
+  // blocks start on a box of keys, so that all but the first and the last are whole boxes
+  const int k_from = p.tma_rows > 0 && k_end > k_begin ? k_begin - k_begin % p.tma_rows : k_begin;
+  const int n_blocks_all = k_end > k_begin ? (k_end - k_from + PX_BN - 1) / PX_BN : 0;
   const int blk0 = static_cast<int>(static_cast<long long>(n_blocks_all) * unit / units);
   const int n_blk = static_cast<int>(static_cast<long long>(n_blocks_all) * (unit + 1) / units) - blk0;
-  const int key0 = n_blk > 0 ? k_begin + blk0 * PX_BN : 0;       // first key of this CTA
+  const int key0 = n_blk > 0 ? k_from + blk0 * PX_BN : 0;        // first key of this CTA
 
   bool ok = true;
   float m = -1e30f, l = 0.f;
   if (warp > kMmaWarp) {
-    // ------------------------------------------------------------ loaders: K, then V rows of a block from their pages
-    // Slots are announced in order once they have landed: normally kLag later than they were asked for, all at once when
-    // the ring is full, since what would make room may be waiting for one of them.
-    // Each warp owns kRowsWarp keys of a block; a lane looks one of them up (a block ahead, so that the page table's
-    // latency is covered) and the warp shares the rows by shuffle: a lookup per copied piece took 2500 cycles a block.
-    constexpr int kChunks = D / 8, kRowsWarp = PX_BN / (SM::kLoaders / 32), kRowsPass = 32 / kChunks;
-    static_assert(kRowsWarp <= 32 && kRowsWarp % kRowsPass == 0, "one lookup per lane");
-    const int lw = warp - kMmaWarp - 1;
+    // ------------------------------------------------------------ loaders: one warp for K, one for V
+    // Where pages hold whole boxes of 8 to 64 keys, a block without keys outside [k_begin, k_end) comes by TMA, one box after
+    // the other from one lane.  Other blocks are copied by hand: every lane looks up two of the 64 keys (a block ahead, so
+    // that the page table's latency is covered) and the warp shares the rows by shuffle; such copies are announced in order
+    // once they have landed, normally kLag blocks after they were asked for, all at once when the ring is full, since what
+    // would make room may be waiting for one of them.
+    constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
+    const bool is_v = warp == kMmaWarp + 2;
     const int c = lane % kChunks, rp = lane / kChunks;
-    const long long row_bytes = static_cast<long long>(p.hkv) * D * 2, piece = (static_cast<long long>(hk) * D + c * 8) * 2;
-    auto look_up = [&](int i) -> int {                           // cache row of this lane's key in block i, -1: zeros, -2: no such page
-      const int key = key0 + i * PX_BN + lw * kRowsWarp + lane;
-      if (lane >= kRowsWarp || i >= n_blk || key >= k_end) return -1;
-      const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
-      const int page = __ldg(table + pi);
-      return page < 0 || page >= p.num_blocks ? -2 : page * p.block_size + (key - pi * p.block_size);
+    const long long row_bytes = static_cast<long long>(p.hkv) * D * 2;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + (static_cast<long long>(hk) * D + c * 8) * 2;
+    const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+    uint64_t *full = kv_full + (is_v ? kStages : 0), *empty = kv_empty + (is_v ? kStages : 0);
+    uint8_t* ring = sKV + (is_v ? kStages * SM::kKV : 0);
+    const int rows = p.tma_rows, n_box = rows > 0 ? PX_BN / rows : 0;
+    auto whole = [&](int i) -> bool {
+      const int k0 = key0 + i * PX_BN;
+      return rows > 0 && k0 >= k_begin && k0 + PX_BN <= k_end;
     };
-    int next = look_up(0), mine = -1;
+    // A lookup is a page and a place in it; they become a row only when the block's turn comes, so that nothing waits for
+    // the page table meanwhile.  -1: zeros, -2: no such page.
+    struct Spot { int page, in_page; };
+    auto spot_of = [&](int key) -> Spot {
+      if (key < k_begin || key >= k_end) return {-1, -1};
+      const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
+      return {__ldg(table + pi), key - pi * p.block_size};
+    };
+    auto row_of = [&](Spot s) -> int {
+      return s.in_page < 0 ? -1 : s.page < 0 || s.page >= p.num_blocks ? -2 : s.page * p.block_size + s.in_page;
+    };
+    Spot next[2];
+    auto look_up = [&](int i) {                                  // this lane's box, or its two keys, of block i
+      next[0] = next[1] = {-1, -1};
+      if (i >= n_blk) return;
+      const int k0 = key0 + i * PX_BN;
+      if (whole(i)) {
+        if (lane < n_box) next[0] = spot_of(k0 + lane * rows);
+      } else {
+        next[0] = spot_of(k0 + lane);
+        next[1] = spot_of(k0 + 32 + lane);
+      }
+    };
+    look_up(0);
     bool bad = false;
-    int told = 0;                                                // slots announced so far
-    auto announce = [&](int upto) {                              // this thread's copies for the slots before upto have landed
+    int told = 0, st = 0;                                        // blocks announced so far; stage
+    uint32_t ph = 1;
+    auto announce = [&](int upto) {                              // this thread's copies of the blocks before upto have landed
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
-        for (int t = told; t < upto; ++t) mbar_arrive(&kv_full[t % kSlots]);
+        for (int t = told; t < upto; ++t) mbar_arrive(&full[t % kStages]);
       told = upto;
     };
-    for (int h = 0; h < 2 * n_blk && ok; ++h) {                  // K of block h / 2, then its V
-      const int st = h % kSlots;
-      const uint32_t empty_ph = ((h / kSlots) & 1) ^ 1;
-      if (!__all_sync(0xffffffffu, px_test(&kv_empty[st], empty_ph))) {
-        if (told < h) { px_cp_wait<0>(); announce(h); }
-        ok = px_wait(&kv_empty[st], empty_ph, abort_flag);
+    for (int i = 0; i < n_blk && ok; ++i) {
+      if (!__all_sync(0xffffffffu, px_test(&empty[st], ph))) {
+        if (told < i) { px_cp_wait<0>(); announce(i); }
+        ok = px_wait(&empty[st], ph, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, h, 0); *abort_flag = 1; break; }
+        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, is_v); *abort_flag = 1; break; }
       }
-      if ((h & 1) == 0) {
-        mine = next;
-        bad = bad || mine == -2;
-        next = look_up((h >> 1) + 1);
+      int mine[2] = {row_of(next[0]), row_of(next[1])};
+      bool boxes = whole(i);
+      if (boxes && __any_sync(0xffffffffu, mine[0] == -2)) {     // a bad page among boxes: its keys become zeros
+        boxes = false;
+        mine[0] = row_of(spot_of(key0 + i * PX_BN + lane));
+        mine[1] = row_of(spot_of(key0 + i * PX_BN + 32 + lane));
       }
-      const uint32_t dst = smem_u32(sKV + st * SM::kKV);
-      const uint8_t* src = reinterpret_cast<const uint8_t*>((h & 1) != 0 ? p.v_cache : p.k_cache) + piece;
+      bad = bad || mine[0] == -2 || mine[1] == -2;
+      look_up(i + 1);
+      uint8_t* slot = ring + st * SM::kKV;
+      if (boxes) {
+        if (told < i) { px_cp_wait<0>(); announce(i); }
+        int row[8];
 #pragma unroll
-      for (int s = 0; s < kRowsWarp / kRowsPass; ++s) {
-        const int rw = s * kRowsPass + rp, r = lw * kRowsWarp + rw;
-        const int row = __shfl_sync(0xffffffffu, mine, rw);
-        px_cp16(dst + (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + max(row, 0) * row_bytes, row >= 0 ? 16u : 0u);
+        for (int x = 0; x < 8; ++x) row[x] = __shfl_sync(0xffffffffu, mine[0], x);
+        if (elect_one()) {
+          mbar_expect_tx(&full[st], SM::kKV);
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if (x < n_box) {
+#pragma unroll
+              for (int d = 0; d < D / 64; ++d) tma_load_2d(slot + d * (PX_BN * 128) + x * rows * 128, map, &full[st], hk * D + d * 64, row[x]);
+            }
+        }
+        __syncwarp();
+        told = i + 1;
+      } else {
+        const uint32_t dst = smem_u32(slot);
+#pragma unroll
+        for (int s = 0; s < PX_BN / kRowsPass; ++s) {
+          const int r = s * kRowsPass + rp;
+          const int row = __shfl_sync(0xffffffffu, mine[s >= PX_BN / kRowsPass / 2], r & 31);
+          px_cp16(dst + (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + max(row, 0) * row_bytes, row >= 0 ? 16u : 0u);
+        }
+        px_cp_commit();
+        if (i - kLag >= told) { px_cp_wait<kLag>(); announce(i - kLag + 1); }
       }
-      px_cp_commit();
-      if (h - kLag >= told) { px_cp_wait<kLag>(); announce(h - kLag + 1); }
+      if (++st == kStages) { st = 0; ph ^= 1; }
     }
     px_cp_wait<0>();
-    if (ok && told < 2 * n_blk) announce(2 * n_blk);
+    if (ok && told < n_blk) announce(n_blk);
     if (bad) report_status(p.status, kStatusBadIndex, 1022, b, 0);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issue
@@ -478,37 +531,48 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
       constexpr uint32_t idesc_s = make_idesc_bf16(PX_BM, PX_BN, 0, 0);
       constexpr uint32_t idesc_pv = make_idesc_bf16(PX_BM, D, 0, 1);
       const uint64_t qa = make_smem_desc(smem_u32(sQ), 0, 1024, kSwizzle128B);
-      auto issue_s = [&](int i) -> bool {
-        const int st = 2 * i % kSlots;
-        if (!px_wait(&kv_full[st], (2 * i / kSlots) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1031, i, 0); *abort_flag = 1; return false; }
-        tc_fence_after_sync();
-        const uint64_t ka = make_smem_desc(smem_u32(sKV + st * SM::kKV), 0, 1024, kSwizzle128B);
+      const uint64_t k_desc = make_smem_desc(smem_u32(sKV), 0, 1024, kSwizzle128B);
+      const uint64_t v_desc = make_smem_desc(smem_u32(sKV + kStages * SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
+      int k_st = 0, v_st = 0;
+      uint32_t k_ph = 0, v_ph = 0;
+      auto wait_for = [&](uint64_t* bar, uint32_t ph, int site, int i) -> bool {
+        if (px_wait(bar, ph, abort_flag)) return true;
+        report_status(p.status, kStatusWaitTimeout, site, i, 0);
+        *abort_flag = 1;
+        return false;
+      };
+      auto issue_s = [&](int i) {                                // S = Q K^T of block i, whose keys are there
+        const uint64_t ka = k_desc + static_cast<uint64_t>(k_st * SM::kKV >> 4);
         const uint32_t d = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
           mma_f16_ss(d, qa + (((j >> 2) * (PX_BM * 128) + (j & 3) * 32) >> 4), ka + (((j >> 2) * (PX_BN * 128) + (j & 3) * 32) >> 4),
                      idesc_s, j != 0 ? 1u : 0u);
         mma_commit(&s_full[i % kBufs]);
-        mma_commit(&kv_empty[st]);
-        return true;
+        mma_commit(&kv_empty[k_st]);
+        if (++k_st == kStages) { k_st = 0; k_ph ^= 1; }
       };
-      bool good = n_blk > 0 && issue_s(0);
+      bool good = n_blk > 0 && wait_for(&kv_full[0], 0, 1031, 0);
+      if (good) { tc_fence_after_sync(); issue_s(0); }
       for (int i = 0; good && i < n_blk; ++i) {
-        if (kBufs == 2 && i + 1 < n_blk) { good = issue_s(i + 1); if (!good) break; }
-        const int st = (2 * i + 1) % kSlots;
-        const uint64_t va = make_smem_desc(smem_u32(sKV + st * SM::kKV), PX_BN * 128, 1024, kSwizzle128B);
-        if (!px_wait(&kv_full[st], ((2 * i + 1) / kSlots) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1038, i, 0); *abort_flag = 1; break; }
-        if (!px_wait(&p_full[i % kBufs], (i / kBufs) & 1, abort_flag)) { report_status(p.status, kStatusWaitTimeout, 1032, i, 0); *abort_flag = 1; break; }
+        const bool more = i + 1 < n_blk;
+        // what is known to come in time is waited for first: only P is on the way from S to S
+        if (more) { good = wait_for(&kv_full[k_st], k_ph, 1031, i + 1); if (!good) break; }
+        if (kBufs == 2 && more) { tc_fence_after_sync(); issue_s(i + 1); }
+        good = wait_for(&kv_full[kStages + v_st], v_ph, 1038, i) && wait_for(&p_full[i % kBufs], (i / kBufs) & 1, 1032, i);
+        if (!good) break;
         tc_fence_after_sync();
+        const uint64_t va = v_desc + static_cast<uint64_t>(v_st * SM::kKV >> 4);
         const uint32_t a_t = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
         for (int j = 0; j < PX_BN / 16; ++j)
           px_mma_ts(tmem_base + kTmemO, a_t + j * 8, va + ((j * 2048) >> 4), idesc_pv, (i | j) != 0 ? 1u : 0u);
-        mma_commit(&kv_empty[st]);
-        if (i + 1 == n_blk) mma_commit(o_full);
+        if (!more) mma_commit(o_full);
         else if (kBufs == 2) mma_commit(pv_done);
         // one buffer: S goes over P once P V has read it (the tensor core takes the products in order)
-        if (kBufs == 1 && i + 1 < n_blk) good = issue_s(i + 1);
+        mma_commit(&kv_empty[kStages + v_st]);
+        if (kBufs == 1 && more) issue_s(i + 1);
+        if (++v_st == kStages) { v_st = 0; v_ph ^= 1; }
       }
     }
     __syncwarp();
@@ -578,25 +642,30 @@ __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas) k_paged
         tmem_st_wait();
       }
       const uint64_t sc2 = px_pack(p.scale_log2, p.scale_log2), nm2 = px_pack(-m, -m);
-      uint64_t rs2[4] = {0, 0, 0, 0};                                        // pairs of partial sums, both halves 0.f
+      uint64_t rs2[2] = {0, 0};                                              // pairs of partial sums, both halves 0.f
       auto exps = [&](uint32_t (&pk)[16]) {
 #pragma unroll
         for (int t = 0; t < 32; t += 2) {
           float x0, x1;
           px_unpack(px_fma2(px_pack(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nm2), x0, x1);
           const float p0 = px_exp2(x0), p1 = px_exp2(x1);
-          rs2[(t >> 1) & 3] = px_add2(rs2[(t >> 1) & 3], px_pack(p0, p1));
+          rs2[(t >> 1) & 1] = px_add2(rs2[(t >> 1) & 1], px_pack(p0, p1));
           pk[t >> 1] = pack_bf16x2(p0, p1);
         }
       };
-      uint32_t pa[16], pb[16];
-      exps(pb);
-      half(0);                                                               // before P goes over it
-      exps(pa);
-      px_tmem_st_x16(s_addr, pa);
-      px_tmem_st_x16(s_addr + 16, pb);
+      {
+        uint32_t pk[16];
+        exps(pk);
+        half(0);                                                             // before P goes over it
+        px_tmem_st_x16(s_addr + 16, pk);
+      }
+      {
+        uint32_t pk[16];
+        exps(pk);
+        px_tmem_st_x16(s_addr, pk);
+      }
       float sa, sb;
-      px_unpack(px_add2(px_add2(rs2[0], rs2[1]), px_add2(rs2[2], rs2[3])), sa, sb);
+      px_unpack(px_add2(rs2[0], rs2[1]), sa, sb);
       l += sa + sb;
       tmem_st_wait();
       tc_fence_before_sync();
@@ -1053,15 +1122,16 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
   if (units > worth) units = worth;
   if (units < 1) units = 1;
   q.splits = 1;
-  // large clusters leave SMs free that do not fill one; the kernel for few rows fits two CTAs best (99k keys: 84 us with 2,
-  // 113 with 8)
-  while (q.splits < (q.nt > 0 ? 2 : 8) && q.splits * 2 <= units) q.splits *= 2;
+  // One cluster does up to 8 splits in one launch.  More of them go to clusters of 2 and a launch that joins these: large
+  // clusters leave SMs free that do not fill one (99k keys of one sequence: 84 us in clusters of 2, 113 in clusters of 8).
+  const int most = may_group && units > 8 ? 2 : 8;
+  while (q.splits * 2 <= most && q.splits * 2 <= units) q.splits *= 2;
   q.groups = may_group && units >= 2 * q.splits ? static_cast<int>(units / q.splits) : 1;
   return q;
 }
 
-template <void (*kern)(ExtendParams)>
-static cudaError_t px_launch(const ExtendParams& p, dim3 grid, int threads, int smem, bool dependent, cudaStream_t st) {
+template <auto kern, typename... More>
+static cudaError_t px_launch(const ExtendParams& p, dim3 grid, int threads, int smem, bool dependent, cudaStream_t st, const More&... more) {
   static std::atomic<unsigned long long> ready{0};               // of this kernel: devices where its shared memory has been raised
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1089,7 +1159,7 @@ static cudaError_t px_launch(const ExtendParams& p, dim3 grid, int threads, int 
     ++n;
   }
   cfg.attrs = at; cfg.numAttrs = n;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
+  e = cudaLaunchKernelEx(&cfg, kern, p, more...);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
@@ -1099,7 +1169,17 @@ static cudaError_t px_few(const ExtendParams& p, dim3 grid, cudaStream_t st) {
 }
 template <int D>
 static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
-  return px_launch<k_paged_extend<D>>(p, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st);
+  // The maps are made for every call: they take a fraction of a microsecond, and nothing is kept by an address.
+  CUtensorMap tk{}, tv{};
+  const uint64_t inner = static_cast<uint64_t>(p.hkv) * D, rows = static_cast<uint64_t>(p.num_blocks) * p.block_size;
+  ExtendParams a = p;
+  a.tma_rows = p.block_size % PX_BN == 0 ? PX_BN : p.block_size >= 8 && PX_BN % p.block_size == 0 ? p.block_size : 0;
+  if (a.tma_rows > 0) {
+    const int rc = make_tensor_map_2d(&tk, p.k_cache, kTmaBf16, inner, rows, inner * 2, 64, a.tma_rows, kTmaSwizzle128) |
+                   make_tensor_map_2d(&tv, p.v_cache, kTmaBf16, inner, rows, inner * 2, 64, a.tma_rows, kTmaSwizzle128);
+    if (rc != 0) a.tma_rows = 0;                                 // then every block is copied by hand
+  }
+  return px_launch<k_paged_extend<D>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st, tk, tv);
 }
 
 static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream_t st) {
