@@ -189,33 +189,41 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) k_verify_draft(const Verify
       }
       int found = -1, last = -1;
       const int e0 = v0 + at_step * per_step, e1 = min(v1, e0 + per_step);
-      for (int v = e0; v < e1 && found < 0; v += 128) {
-        double o[4];
-        const int at = v + lane * 4;
-        float pv[4], qv[4] = {0.f, 0.f, 0.f, 0.f};
-        read4(tp, at, pv);
-        if (dp != nullptr) read4(dp, at, qv);
-        weights(at, pv, qv, o);
-        const double mine = (o[0] + o[1]) + (o[2] + o[3]);
-        double inc = mine;
+      for (int v = e0; v < e1 && found < 0; v += kBatch) {
+        float pv[kVerifyBatch][4], qv[kVerifyBatch][4];
 #pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, inc, k);
-          if (lane >= k) inc += up;
+        for (int u = 0; u < kVerifyBatch; ++u) {
+          read4(tp, v + u * 128 + lane * 4, pv[u]);
+          if (dp != nullptr) read4(dp, v + u * 128 + lane * 4, qv[u]);
+          else qv[u][0] = qv[u][1] = qv[u][2] = qv[u][3] = 0.f;
         }
-        double c = wbase + (inc - mine);
-        int hit = -1, tail = -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c += o[i];
-          if (o[i] > 0.0) tail = at + i;
-          if (hit < 0 && o[i] > 0.0 && c > goal) hit = at + i;
+        for (int u = 0; u < kVerifyBatch; ++u) {
+          if (found >= 0) break;
+          const int at = v + u * 128 + lane * 4;
+          double o[4];
+          weights(at, pv[u], qv[u], o);
+          const double mine = (o[0] + o[1]) + (o[2] + o[3]);
+          double inc = mine;
+#pragma unroll
+          for (int k = 1; k < 32; k <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, inc, k);
+            if (lane >= k) inc += up;
+          }
+          double c = wbase + (inc - mine);
+          int hit = -1, tail = -1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c += o[i];
+            if (o[i] > 0.0) tail = at + i;
+            if (hit < 0 && o[i] > 0.0 && c > goal) hit = at + i;
+          }
+          const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
+          if (who) found = __shfl_sync(0xffffffffu, hit, __ffs(who) - 1);
+          const unsigned any = __ballot_sync(0xffffffffu, tail >= 0);
+          if (any) last = __shfl_sync(0xffffffffu, tail, 31 - __clz(any));
+          wbase += __shfl_sync(0xffffffffu, inc, 31);
         }
-        const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
-        if (who) found = __shfl_sync(0xffffffffu, hit, __ffs(who) - 1);
-        const unsigned any = __ballot_sync(0xffffffffu, tail >= 0);
-        if (any) last = __shfl_sync(0xffffffffu, tail, 31 - __clz(any));
-        wbase += __shfl_sync(0xffffffffu, inc, 31);
       }
       if (lane == 0) p.out[row] = found >= 0 ? found : last;
     } else if (pw < 0 && warp == 0 && lane == 0) {
