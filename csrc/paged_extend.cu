@@ -143,6 +143,13 @@ NMOE_DEVICE void px_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: 
 // x / g for x below g + 128 and 2^22, from 1 / g: (x + 1/2) / g is at least 1 / (2 g) from a whole number
 NMOE_DEVICE int px_div(int x, float inv_g) { return static_cast<int>((static_cast<float>(x) + 0.5f) * inv_g); }
 
+// floor(n * i / of) for i <= of: where the share of unit i starts (a 64-bit division only where 32 bits do not hold it)
+NMOE_DEVICE int px_share(int n, int i, int of) {
+  if (of == 1) return i == 0 ? 0 : n;
+  if (n < 0x7fffffff / (of + 1)) return static_cast<int>(static_cast<unsigned>(n * i) / static_cast<unsigned>(of));
+  return static_cast<int>(static_cast<long long>(n) * i / of);
+}
+
 // Rows of one list: its first row, its number of tokens (0 where the lengths are out of range) and its context.
 NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start, int& n, int& ctx) {
   start = 0;
@@ -166,13 +173,18 @@ constexpr int PX_SORT_MOST = 256;
 template <int kThreads>
 NMOE_DEVICE int px_nth_longest(const ExtendParams& p, int z, int* s_len) {         // s_len: PX_SORT_MOST + 1 words of scratch
   int& s_which = s_len[PX_SORT_MOST];
-  for (int t = threadIdx.x; t < p.n_seqs; t += kThreads)
-    s_len[t] = p.q_lens != nullptr && p.q_lens[t] <= 0 ? -1 : p.context_lens[t];
+  const int n4 = (p.n_seqs + 3) / 4;
+  for (int t = threadIdx.x; t < 4 * n4; t += kThreads)
+    s_len[t] = t >= p.n_seqs ? -0x7fffffff - 1 : p.q_lens != nullptr && p.q_lens[t] <= 0 ? -1 : p.context_lens[t];
   __syncthreads();
   for (int t = threadIdx.x; t < p.n_seqs; t += kThreads) {
     const int mine = s_len[t];
     int rank = 0;
-    for (int u = 0; u < p.n_seqs; ++u) rank += s_len[u] > mine || (s_len[u] == mine && u < t) ? 1 : 0;
+    for (int u = 0; u < n4; ++u) {
+      const int4 v = reinterpret_cast<const int4*>(s_len)[u];
+      rank += (v.x > mine || (v.x == mine && 4 * u < t)) + (v.y > mine || (v.y == mine && 4 * u + 1 < t)) +
+              (v.z > mine || (v.z == mine && 4 * u + 2 < t)) + (v.w > mine || (v.w == mine && 4 * u + 3 < t));
+    }
     if (rank == z) s_which = t;
   }
   __syncthreads();
@@ -416,8 +428,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
   // blocks start on a box of keys, so that all but the first and the last are whole boxes
   const int k_from = p.tma_rows > 0 && k_end > k_begin ? k_begin - k_begin % p.tma_rows : k_begin;
   const int n_blocks_all = k_end > k_begin ? (k_end - k_from + PX_BN - 1) / PX_BN : 0;
-  const int blk0 = static_cast<int>(static_cast<long long>(n_blocks_all) * unit / units);
-  const int n_blk = static_cast<int>(static_cast<long long>(n_blocks_all) * (unit + 1) / units) - blk0;
+  const int blk0 = px_share(n_blocks_all, unit, units), n_blk = px_share(n_blocks_all, unit + 1, units) - blk0;
   const int key0 = n_blk > 0 ? k_from + blk0 * PX_BN : 0;        // first key of this CTA
 
   bool ok = true;
@@ -833,8 +844,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
     }
   }
   const int tiles_all = k_end > k_begin ? (k_end - k_begin + kTile - 1) / kTile : 0;
-  const int tile0 = static_cast<int>(static_cast<long long>(tiles_all) * unit / units);
-  const int n_tiles = static_cast<int>(static_cast<long long>(tiles_all) * (unit + 1) / units) - tile0;
+  const int tile0 = px_share(tiles_all, unit, units), n_tiles = px_share(tiles_all, unit + 1, units) - tile0;
   const int n_mine = n_tiles > warp ? (n_tiles - warp + F::kWarps - 1) / F::kWarps : 0;      // tiles warp, warp + 4, ...
   const int key0 = (tiles_all > 0 ? k_begin : 0) + (tile0 + warp) * kTile;
 
@@ -1046,30 +1056,36 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   px_join<D, F::kThreads>(p, sx, s_ml, start, 0, n_valid, hk, unit);
 }
 
-// Joins the sets of a launch that split the keys over several clusters: a CTA for each row, D / 8 threads for its columns,
-// the others for other sets (dozens of them for a single long context: one after the other they took 32 us).
-template <int D>
+// Joins the sets of the launches that split the keys over several clusters: D / 8 threads for the columns of a row, kParts of
+// such groups for its sets (1 for a few sets and many rows; a CTA a row for the dozens of sets of a single long context,
+// which took 32 us one after the other).
+template <int D, int kParts>
 __global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
-  constexpr int kCols = D / 8, kParts = 128 / kCols;
-  __shared__ float s_max[4], s_acc[kParts][kCols][9];
-  const int b = blockIdx.y, c = threadIdx.x % kCols, part = threadIdx.x / kCols;
-  const int h = static_cast<int>(blockIdx.x) % p.hq, tok = static_cast<int>(blockIdx.x) / p.hq;
+  constexpr int kCols = D / 8, kRows = 128 / (kCols * kParts);
+  static_assert(kParts == 1 || kRows == 1, "the parts of a row are its CTA");
+  __shared__ float s_max[4], s_acc[kParts > 1 ? kParts : 1][kCols][9];
+  const int b = blockIdx.y, c = threadIdx.x % kCols, part = kParts > 1 ? threadIdx.x / kCols : 0;
+  const int i = static_cast<int>(blockIdx.x) * kRows + (kParts > 1 ? 0 : threadIdx.x / kCols), h = i % p.hq, tok = i / p.hq;
   int start, n, ctx;
   px_list(p, b, false, start, n, ctx);
   px_wait_prior_grid();
-  if (tok >= n) return;                                          // the whole CTA
+  if (tok >= n) return;                                          // the whole CTA where it has one row
   const long long row = static_cast<long long>(start + tok) * p.hq + h;
   const float sink = px_sink(p, h);
   float mm = -1e30f;
-  for (int s = threadIdx.x; s < p.n_sets; s += 128) {
+#pragma unroll 4
+  for (int s = kParts > 1 ? threadIdx.x : 0; s < p.n_sets; s += kParts > 1 ? 128 : 1) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
     if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
   }
-  mm = warp_max(mm);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mm;
-  __syncthreads();
+  if constexpr (kParts > 1) {
+    mm = warp_max(mm);
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mm;
+    __syncthreads();
+    mm = fmaxf(px_max3(s_max[0], s_max[1], s_max[2]), s_max[3]);
+  }
   PxSum t;
-  t.start(fmaxf(px_max3(s_max[0], s_max[1], s_max[2]), fmaxf(s_max[3], sink)));
+  t.start(fmaxf(mm, sink));
 #pragma unroll 4
   for (int s = part; s < p.n_sets; s += kParts) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
@@ -1077,16 +1093,18 @@ __global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
     const float4 x = __ldcg(o), y = __ldcg(o + 1);
     if (ml.y > 0.f) t.add(ml, x, y);
   }
+  if constexpr (kParts > 1) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s_acc[part][c][e] = t.acc[e];
-  s_acc[part][c][8] = t.sum;
-  __syncthreads();
-  if (part > 0) return;
+    for (int e = 0; e < 8; ++e) s_acc[part][c][e] = t.acc[e];
+    s_acc[part][c][8] = t.sum;
+    __syncthreads();
+    if (part > 0) return;
 #pragma unroll
-  for (int q = 1; q < kParts; ++q) {
+    for (int q = 1; q < kParts; ++q) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t.acc[e] += s_acc[q][c][e];
-    t.sum += s_acc[q][c][8];
+      for (int e = 0; e < 8; ++e) t.acc[e] += s_acc[q][c][e];
+      t.sum += s_acc[q][c][8];
+    }
   }
   t.store(p.out + row * D + c * 8, sink);
 }
@@ -1101,13 +1119,15 @@ struct PxPlan {
 // `lists` row lists of up to `rows` rows that see at most `keys` keys each; groups only where partial sets may be written.
 static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys, bool may_group) {
   PxPlan q;
-  const int few_most = D == 64 ? 40 : 32;
+  // 64 drafted steps of 5 tokens, 40 rows, D = 64: 72 us against 84 in the kernel for many rows; 32 rows of D = 128 over 99k
+  // keys: 68 against 63
+  const int few_most = D == 64 ? 40 : 16;
   q.nt = 0;
   q.tiles = 1;
   long long slots, least;                  // CTAs the GPU holds at once; keys that make a split worth while
   if (rows <= few_most) {
     const int t = static_cast<int>((rows + 7) / 8);
-    q.nt = D == 64 ? (t == 4 ? 5 : t) : (t == 3 ? 4 : t);
+    q.nt = t == 4 ? 5 : t;
     slots = 148 * (D == 64 ? (q.nt == 1 ? 4 : q.nt == 2 ? 3 : 2) : (q.nt == 1 ? 3 : 2));
     least = 128;
   } else {
@@ -1201,28 +1221,34 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
     switch (q.nt) {
       case 0: e = px_many<128>(p, grid, st); break;
       case 1: e = px_few<128, 1>(p, grid, st); break;
-      case 2: e = px_few<128, 2>(p, grid, st); break;
-      default: e = px_few<128, 4>(p, grid, st); break;
+      default: e = px_few<128, 2>(p, grid, st); break;
     }
   }
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
 
+// The launches of a call.  One row list a sequence: `own`, and a join where its keys are split over several clusters.  A shared
+// prefix: `pre` for its keys, then `own` for each sequence's, whose CTAs join pre's sets.  (Letting own run beside pre and
+// joining both in a third launch gained nothing: 128 sequences behind 1504 keys 45 -> 46 us, pre leaves few places free.)
 struct PxCall {
-  PxPlan first, second;      // second: each sequence's own keys behind a shared prefix
+  PxPlan own, pre;
+  bool shared, join;
+  int sets;
 };
 
 static PxCall px_call(int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int max_q_len, int window, int prefix_len) {
-  const long long capacity = static_cast<long long>(max_blocks) * block_size;
+  const long long capacity = static_cast<long long>(max_blocks) * block_size, seen = prefix_len > 0 ? capacity - prefix_len : capacity;
+  const long long reach = window > 0 ? static_cast<long long>(window) + max_q_len : seen, keys = reach < seen ? reach : seen;
   const int g = Hq / Hkv;
-  PxCall c;
-  if (prefix_len <= 0) {
-    const long long keys = window > 0 && window + static_cast<long long>(max_q_len) < capacity ? window + max_q_len : capacity;
-    c.first = c.second = px_plan(D, Hkv, static_cast<long long>(max_q_len) * g, B, keys, true);
+  PxCall c{};
+  c.shared = prefix_len > 0;
+  c.own = px_plan(D, Hkv, static_cast<long long>(max_q_len) * g, B, keys, !c.shared);
+  if (c.shared) {
+    c.pre = px_plan(D, Hkv, static_cast<long long>(B) * g, 1, prefix_len, true);
+    c.sets = c.pre.groups;
   } else {
-    const long long own = capacity - prefix_len;
-    c.first = px_plan(D, Hkv, static_cast<long long>(B) * g, 1, prefix_len, true);
-    c.second = px_plan(D, Hkv, g, B, window > 0 && window < own ? window : own, false);
+    c.join = c.own.groups > 1;
+    c.sets = c.join ? c.own.groups : 0;
   }
   return c;
 }
@@ -1235,9 +1261,15 @@ using namespace nmoe;
 extern "C" long long nmoe_paged_extend_workspace(int n_rows, int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
                                                  int max_q_len, int window, int prefix_len) {
   if (Hkv < 1 || Hq < Hkv) return 0;
+  return px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len).sets * static_cast<long long>(n_rows) * Hq * (D + 2);
+}
+
+// Kernels that such a call launches.
+extern "C" int nmoe_paged_extend_launches(int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int max_q_len, int window,
+                                          int prefix_len) {
+  if (Hkv < 1 || Hq < Hkv) return 0;
   const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
-  if (prefix_len <= 0 && c.first.groups == 1) return 0;
-  return static_cast<long long>(c.first.groups) * n_rows * Hq * (D + 2);
+  return 1 + (c.shared ? 1 : 0) + (c.join ? 1 : 0);
 }
 
 // q [n_rows, Hq, D] (rows q_stride apart), out [n_rows, Hq, D]; caches [num_blocks, block_size, Hkv, D]; block_tables [B] rows
@@ -1258,7 +1290,7 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
   if (prefix_len > 0 && (q_starts != nullptr || q_lens != nullptr)) return -5;
   if (workspace_floats < nmoe_paged_extend_workspace(n_rows, B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len)) return -6;
   const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
-  ExtendParams p;
+  ExtendParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q); p.k_cache = static_cast<const __nv_bfloat16*>(k_cache);
   p.v_cache = static_cast<const __nv_bfloat16*>(v_cache); p.out = static_cast<__nv_bfloat16*>(out);
   p.block_tables = block_tables; p.context_lens = context_lens; p.q_starts = q_starts; p.q_lens = q_lens; p.sinks = sinks;
@@ -1272,25 +1304,32 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
   p.max_q_len = max_q_len; p.window = window; p.sinks_fp32 = sinks_fp32;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.set_rows = static_cast<long long>(n_rows) * Hq;
-  p.n_sets = c.first.groups;
+  p.n_sets = c.sets;
   p.part_o = workspace;
   p.part_ml = workspace != nullptr ? workspace + p.n_sets * p.set_rows * D : nullptr;
-  p.key_begin = 0; p.key_end = 0x7fffffff; p.flat = 0; p.part_mode = 0;
-  if (prefix_len <= 0) {
-    if (c.first.groups == 1) return px_run(p, c.first, D, B, st);
-    p.part_mode = 1;
-    const int rc = px_run(p, c.first, D, B, st);
+  p.key_end = 0x7fffffff;
+  if (c.shared) {
+    ExtendParams f = p;
+    f.flat = 1; f.part_mode = 1; f.key_end = prefix_len;
+    const int rc = px_run(f, c.pre, D, 1, st);
     if (rc != 0) return rc;
+    p.key_begin = prefix_len;
     p.part_mode = 2;
-    p.splits = 1;
-    const dim3 grid(static_cast<unsigned>(max_q_len) * Hq, B);
-    const cudaError_t e = D == 64 ? px_launch<k_paged_join<64>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128>>(p, grid, 128, 0, true, st);
-    return e == cudaSuccess ? 0 : static_cast<int>(e);
+  } else if (c.join) {
+    p.part_mode = 1;
   }
-  ExtendParams f = p;
-  f.flat = 1; f.part_mode = 1; f.key_end = prefix_len;
-  const int rc = px_run(f, c.first, D, 1, st);
-  if (rc != 0) return rc;
-  p.part_mode = 2; p.key_begin = prefix_len;
-  return px_run(p, c.second, D, B, st);
+  const int rc = px_run(p, c.own, D, B, st);
+  if (rc != 0 || !c.join) return rc;
+  p.splits = 1;
+  const long long rows = static_cast<long long>(max_q_len) * Hq;
+  cudaError_t e;
+  if (p.n_sets > 8) {
+    const dim3 grid(static_cast<unsigned>(rows), B);
+    e = D == 64 ? px_launch<k_paged_join<64, 16>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128, 8>>(p, grid, 128, 0, true, st);
+  } else {
+    const int each = 128 / (D / 8);
+    const dim3 grid(static_cast<unsigned>((rows + each - 1) / each), B);
+    e = D == 64 ? px_launch<k_paged_join<64, 1>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128, 1>>(p, grid, 128, 0, true, st);
+  }
+  return e == cudaSuccess ? 0 : static_cast<int>(e);
 }

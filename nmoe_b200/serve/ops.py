@@ -111,9 +111,10 @@ def _stream(device: torch.device) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _attend_workspace(*sizes: int) -> int:
-  """Floats of partial results of a call of these sizes; a function of the sizes alone."""
-  return _fn("nmoe_paged_extend_workspace", "iiiiiiiiii", ctypes.c_longlong)(*sizes)
+def _attend_plan(N: int, *sizes: int) -> Tuple[int, int]:
+  """Floats of partial results and number of launches of a call of these sizes; a function of the sizes alone."""
+  return (_fn("nmoe_paged_extend_workspace", "iiiiiiiiii", ctypes.c_longlong)(N, *sizes),
+          _fn("nmoe_paged_extend_launches", "iiiiiiiii")(*sizes))
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, Hkv: int, D: int) -> None:
@@ -277,14 +278,14 @@ def _attend(what, q, k_cache, v_cache, block_tables, context_lens, q_starts, q_l
   N, Hq, D = q.shape
   num_blocks, block_size, Hkv, _ = k_cache.shape
   B, width, dev = context_lens.size(0), block_tables.size(1), q.device
-  need = _attend_workspace(N, B, Hq, Hkv, D, block_size, width, max_q_len, window, prefix_len)
+  need, launches = _attend_plan(N, B, Hq, Hkv, D, block_size, width, max_q_len, window, prefix_len)
   # partial results (O, m, l) where the keys of a row are split over more CTAs than exchange them directly
   work = torch.empty((need,), dtype=torch.float32, device=dev) if need else None
   L.check(_fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifiplpp")(
     q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
     context_lens.data_ptr(), _p(q_starts), _p(q_lens), _p(sinks), sinks is not None and sinks.dtype == torch.float32, out.data_ptr(),
     N, B, Hq, Hkv, D, block_size, num_blocks, width, max_q_len, window, scale, prefix_len, _p(work), need,
-    status_buffer(dev).data_ptr(), _stream(dev)), what, 2 if need else 1)
+    status_buffer(dev).data_ptr(), _stream(dev)), what, launches)
 
 
 def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
