@@ -50,7 +50,7 @@ struct ExtendParams {
   long long q_stride, bt_stride;
   int n_rows, n_seqs, hq, hkv, group, block_size, block_shift, num_blocks, capacity, max_q_len, window, sinks_fp32;
   int key_begin, key_end;             // only keys in [key_begin, key_end) count here
-  int flat;                           // 1: the tokens of all sequences are one list that reads the first sequence's pages
+  int flat;                           // 1: the tokens of all sequences are one list that reads the pages of one of them
   int splits, groups;                 // the keys of a row list are divided over groups x splits CTAs, splits = a cluster
   int sorted;                         // 1: lists by falling context
   int part_mode;                      // 0 none, 1 write partial results (one set per group), 2 join those of the launch before
@@ -191,6 +191,17 @@ NMOE_DEVICE int px_nth_longest(const ExtendParams& p, int z, int* s_len) {      
   const int which = s_which;
   __syncthreads();                                               // the scratch may be used for something else
   return which;
+}
+// Whose pages hold the keys of a list that all sequences share: the first sequence that reaches its end (a padding row does
+// not), else the longest.
+NMOE_DEVICE int px_owner(const ExtendParams& p) {
+  int best = 0, most = -1;
+  for (int t = 0; t < p.n_seqs; ++t) {
+    const int c = p.context_lens[t];
+    if (c >= p.key_end) return t;
+    if (c > most) { most = c; best = t; }
+  }
+  return best;
 }
 // Keys [lo, hi) that a token of the list sees.
 NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool speaker, int& lo, int& hi) {
@@ -364,7 +375,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     if (p.part_mode == 2) px_wait_prior_grid();
     return;
   }
-  const int* table = p.block_tables + b * p.bt_stride;
+  const int* table = p.block_tables + (p.flat ? px_owner(p) : b) * p.bt_stride;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kStages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -818,7 +829,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
     return;
   }
   if (p.part_mode == 1) px_launch_dependents();
-  const int* table = p.block_tables + b * p.bt_stride;
+  const int* table = p.block_tables + (p.flat ? px_owner(p) : b) * p.bt_stride;
 
   // keys of the list, and the bounds inside which no row needs a mask
   int k_begin, k_end, w_lo, w_hi;
@@ -1260,14 +1271,14 @@ using namespace nmoe;
 // Floats of workspace that nmoe_paged_extend needs for a call of these sizes (0: none).
 extern "C" long long nmoe_paged_extend_workspace(int n_rows, int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
                                                  int max_q_len, int window, int prefix_len) {
-  if (Hkv < 1 || Hq < Hkv) return 0;
+  if (B < 1 || n_rows < 1 || max_q_len < 1 || Hkv < 1 || Hq < Hkv || max_blocks < 0 || block_size < 1) return 0;
   return px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len).sets * static_cast<long long>(n_rows) * Hq * (D + 2);
 }
 
 // Kernels that such a call launches.
 extern "C" int nmoe_paged_extend_launches(int B, int Hq, int Hkv, int D, int block_size, int max_blocks, int max_q_len, int window,
                                           int prefix_len) {
-  if (Hkv < 1 || Hq < Hkv) return 0;
+  if (B < 1 || max_q_len < 1 || Hkv < 1 || Hq < Hkv || max_blocks < 0 || block_size < 1) return 0;
   const PxCall c = px_call(B, Hq, Hkv, D, block_size, max_blocks, max_q_len, window, prefix_len);
   return 1 + (c.shared ? 1 : 0) + (c.join ? 1 : 0);
 }
@@ -1282,7 +1293,7 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
                                  int max_q_len, int window, float scale, int prefix_len, float* workspace,
                                  long long workspace_floats, void* status, cudaStream_t st) {
   if (B == 0 || n_rows == 0 || max_q_len == 0) return 0;
-  if (Hkv < 1 || Hkv > 65535 || Hq % Hkv != 0 || block_size < 1 || B < 0 || B > 65535 || !(scale > 0.f)) return -1;
+  if (n_rows < 0 || max_q_len < 0 || max_blocks < 0 || num_blocks < 0 || Hkv < 1 || Hkv > 65535 || Hq < Hkv || Hq % Hkv != 0 || block_size < 1 || B < 0 || B > 65535 || !(scale > 0.f)) return -1;
   if (D != 64 && D != 128) return -2;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 != 0 || (n_rows > 1 && q_stride % 8 != 0)) return -3;

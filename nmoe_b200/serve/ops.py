@@ -296,9 +296,11 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   q [N, Hq, D]: the tokens of sequence b are rows q_starts[b] .. q_starts[b] + q_lens[b] - 1 (sequences do not overlap; gaps
   are fine); its token j stands at position context_lens[b] - q_lens[b] + j and sees the keys at or before it, of those the
   last ``window`` if that is positive.  sinks [Hq]: a logit per head that only enters the denominator.  A token that sees no
-  key gives zeros.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].
+  key gives zeros.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].  K and V of the
+  positions before ``context_lens[b]`` (within the window of the first new token) are finite; what else the pages hold does not matter.
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.
-  Lengths or pages outside their tensors are skipped and show up in ``check_status``."""
+  Sequences whose rows lie outside q or exceed ``max_q_len`` are skipped, contexts longer than their table are cut, pages
+  outside the cache count as zeros: all three show up in ``check_status``."""
   given = q
   q, sinks = _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, scale, window)
   dev, N = q.device, q.size(0)
@@ -328,7 +330,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          context_lens: torch.Tensor, prefix_len: int, sinks: Optional[torch.Tensor], scale: float,
                          window: int = 0) -> torch.Tensor:
   """``paged_decode`` for a batch whose sequences all start with the same ``prefix_len`` tokens: their keys and values are
-  read once for the whole batch, through the first sequence's pages, instead of once per sequence.
+  read once for the whole batch, through the pages of the first sequence that has them all, instead of once per sequence.
 
   q [B, Hq, D] -> [B, Hq, D]; block_tables [B, n] hold every sequence's whole table (prefix pages included; where the prefix
   ends inside a page, each table may have its own copy of that page).  ``context_lens`` counts the current token; a sequence

@@ -116,3 +116,36 @@ def test_status_record_made_in_inference_mode_can_be_reset():
     G.check_status(dev)
   finally:
     G._STATUS.pop(dev, None)
+
+
+def test_c_entries_refuse_sizes_that_are_none():
+  """Empty and senseless sizes come back as numbers from the C entries (no GPU is asked for anything)."""
+  import ctypes
+  from nmoe_b200.ops import _lib as L
+  if not L.available():
+    pytest.skip("library not built")
+  lib = L.lib()
+  ws = lib.nmoe_paged_extend_workspace
+  ws.restype = ctypes.c_longlong
+  for n_rows, B, Hq, Hkv, D, bs, width, mq in ((0, 0, 8, 2, 64, 16, 3, 0), (3, 0, 8, 2, 64, 16, 3, 1), (3, 2, 8, 0, 64, 16, 3, 3), (3, 2, 8, 2, 64, 0, 3, 3),
+                                               (3, 2, 1, 2, 64, 16, 3, 3), (3, 2, 8, 2, 64, 16, 0, 3)):
+    assert ws(n_rows, B, Hq, Hkv, D, bs, width, mq, 0, 0) == 0
+    assert lib.nmoe_paged_extend_launches(B, Hq, Hkv, D, bs, width, mq, 0, 0) in (0, 1)
+  call = S._fn("nmoe_paged_extend", "plppplppppipiiiiiiiiiifiplpp")
+  args = lambda **kw: [{**dict(q=0, qs=512, k=0, v=0, bt=0, bts=3, ctx=0, st=0, ln=0, sk=0, sf=0, out=0, n=3, B=2, Hq=8, Hkv=2, D=64, bs=16, nb=4, w=3, mq=3,
+                               win=0, scale=1.0, pre=0, ws=0, wf=0, status=0, stream=0), **kw}[k] for k in
+                       "q qs k v bt bts ctx st ln sk sf out n B Hq Hkv D bs nb w mq win scale pre ws wf status stream".split()]
+  assert call(*args(B=0)) == 0 and call(*args(n=0)) == 0 and call(*args(mq=0)) == 0
+  for bad, rc in ((dict(Hkv=0), -1), (dict(Hq=9), -1), (dict(Hq=1), -1), (dict(bs=0), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(n=-1), -1),
+                  (dict(D=96), -2), (dict(q=8), -3), (dict(out=2), -3), (dict(qs=100), -3), (dict(nb=1 << 30), -4), (dict(pre=5, st=16), -5),
+                  (dict(w=100000, B=1), -6), (dict(pre=48), -6)):
+    assert call(*args(**bad)) == rc, bad
+  rope = S._fn("nmoe_rope_append", "plpipfppplpppiiiipp")
+  r = lambda **kw: [{**dict(x=0, xs=768, pos=0, p64=1, inv=0, conc=1.0, slots=0, k=0, v=0, ns=0, q=0, ko=0, vo=0, n=1, hq=8, hkv=2, d=64, status=0, stream=0),
+                     **kw}[k] for k in "x xs pos p64 inv conc slots k v ns q ko vo n hq hkv d status stream".split()]
+  assert rope(*r(n=0)) == 0
+  for bad, rc in ((dict(n=-1), -1), (dict(hq=0), -1), (dict(d=8), -1), (dict(d=520), -1), (dict(xs=100), -1), (dict(slots=16), -2), (dict(x=8), -3), (dict(k=4), -3)):
+    assert rope(*r(**bad)) == rc, bad
+  ver = S._fn("nmoe_verify_draft", "plplpippppp" + "iiipp")
+  assert ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, 3, 0, 5, 0, 0) == 0
+  assert ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, 3, 2, 0, 0, 0) == -1 and ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, -3, 2, 5, 0, 0) == -1

@@ -137,6 +137,67 @@ def test_paged_extend_ignores_what_lies_outside(what):
   within(out, want, bound)
 
 
+@pytest.mark.parametrize("bs", [8, 16, 32, 48, 64, 128, 192, 7])
+@pytest.mark.parametrize("D,hq,hkv,window", [(64, 8, 2, 0), (128, 8, 2, 0), (64, 16, 2, 150)])
+def test_paged_extend_page_sizes(bs, D, hq, hkv, window):
+  """Pages that hold whole boxes of a block, or more than a block, or neither; many rows, few rows."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(bs)
+  lens, ctx = [100, 3, 37], [500, 777, 65]
+  k, v, tables = paged(ctx, bs, hkv, D, g)
+  for b in range(3):                                # behind the context: nothing that may be read into a product
+    for t in range(ctx[b], (ctx[b] + bs - 1) // bs * bs):
+      k[tables[b, t // bs].long(), t % bs] = float("nan")
+      v[tables[b, t // bs].long(), t % bs] = float("nan")
+  starts = [0, 100, 103]
+  q = torch.randn(140, hq, D, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, starts, lens, None, D ** -0.5, window)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, D ** -0.5, window)
+  within(out, want, bound)
+
+
+def test_paged_extend_strided_operands():
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(8)
+  lens, ctx = [2, 50], [300, 50]
+  k, v, tables = paged(ctx, 16, 2, 64, g)
+  q = torch.randn(52, 8, 64, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, [0, 2], lens, None, 0.125, 0)
+  kd, vd = k.to(DEV), v.to(DEV)
+  rest = (i32(ctx), i32([0, 2]), i32(lens), None, 0.125)
+  base = S.paged_extend(q.to(DEV), kd, vd, tables.to(DEV), *rest)
+  within(base, want, bound)
+  fused = torch.zeros(52, 12 * 64 + 8, dtype=torch.bfloat16, device=DEV)
+  for off in (0, 8, 1):                             # q heads inside a fused projection; misaligned rows are copied once
+    view = fused[:, off:off + 512].view(52, 8, 64) if off == 0 else fused[:, off:off + 512].unflatten(1, (8, 64))
+    view.copy_(q)
+    assert torch.equal(S.paged_extend(view, kd, vd, tables.to(DEV), *rest), base)
+  heads_first = q.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)
+  assert torch.equal(S.paged_extend(heads_first, kd, vd, tables.to(DEV), *rest), base)
+  wide = torch.zeros(2, tables.size(1) + 5, dtype=torch.int32, device=DEV)
+  wide[:, :tables.size(1)] = tables.to(DEV)
+  assert torch.equal(S.paged_extend(q.to(DEV), kd, vd, wide[:, :tables.size(1)], *rest), base)
+  pairs = torch.stack((i32(ctx), i32(lens)), 1)     # every second number
+  assert torch.equal(S.paged_extend(q.to(DEV), kd, vd, tables.to(DEV), pairs[:, 0], i32([0, 2]), pairs[:, 1], None, 0.125), base)
+
+
+def test_empty_calls():
+  from nmoe_b200.serve import ops as S
+  kc = torch.zeros(2, 16, 2, 64, device=DEV, dtype=torch.bfloat16)
+  none, t0 = i32([]), torch.zeros(0, 3, dtype=torch.int32, device=DEV)
+  q = torch.zeros(0, 8, 64, device=DEV, dtype=torch.bfloat16)
+  assert S.paged_extend(q, kc, kc, t0, none, none, none, None, 0.125).shape == (0, 8, 64)
+  assert S.shared_prefix_decode(q, kc, kc, t0, none, 0, None, 0.125).shape == (0, 8, 64)
+  q3 = torch.ones(3, 8, 64, device=DEV, dtype=torch.bfloat16)
+  t = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+  assert (S.paged_extend(q3, kc, kc, t, i32([0, 4]), i32([0, 3]), i32([0, 0]), None, 0.125) == 0).all()
+  qq, k, v = S.rope_append(torch.zeros(0, 12 * 64, device=DEV, dtype=torch.bfloat16), torch.zeros(0, device=DEV, dtype=torch.long),
+                           torch.ones(32, device=DEV), 1.0, 8, 2, kc, kc.clone(), none, need_kv=True)
+  assert qq.shape == (0, 8, 64) and k.shape == v.shape == (0, 2, 64)
+  out, n = S.verify_draft(torch.zeros(0, 5, device=DEV), torch.zeros(0, device=DEV, dtype=torch.long), torch.zeros(0, device=DEV), i32([0]), i32([0]))
+  assert out.numel() == 0 and n.tolist() == [0]
+
+
 def test_paged_extend_large_scores_and_extreme_sinks():
   from nmoe_b200.serve import ops as S
   g = torch.Generator().manual_seed(6)
@@ -194,13 +255,28 @@ def test_shared_prefix_decode_many_rows_and_odd_contexts():
   g = torch.Generator().manual_seed(9)
   prefix, hq, hkv, D = 700, 16, 2, 64
   ctx = [prefix + 1 + (7 * b) % 90 for b in range(70)]
-  ctx[3], ctx[20], ctx[69], ctx[40] = 0, 5, 700, 650
+  ctx[0], ctx[3], ctx[20], ctx[69], ctx[40] = 0, 0, 5, 700, 650
   k, v, tables = paged([max(c, prefix) for c in ctx], 16, hkv, D, g, shared=prefix)
+  tables[0] = -1                                    # a padding row has no pages, in the first place neither
   q = torch.randn(70, hq, D, generator=g).bfloat16()
   sinks = torch.randn(hq, generator=g).bfloat16()
   want, bound, _ = attend(q, k, v, tables, ctx, list(range(70)), [1 if c else 0 for c in ctx], sinks, 0.125, 0)
-  out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix, sinks.to(DEV), 0.125)
-  within(out, want, bound + 1e-30)
+  for lo, hi in ((0, 70), (0, 3), (18, 22)):        # as a whole, a few rows, a few among them shorter than the prefix
+    out = S.shared_prefix_decode(q[lo:hi].to(DEV), k.to(DEV), v.to(DEV), tables[lo:hi].to(DEV), i32(ctx[lo:hi]), prefix, sinks.to(DEV), 0.125)
+    within(out, want[lo:hi], bound[lo:hi] + 1e-30)
+
+
+@pytest.mark.parametrize("B,prefix,suffix", [(2, 6000, 40), (3, 100, 5000), (300, 130, 20)])
+def test_shared_prefix_decode_long_and_wide(B, prefix, suffix):
+  """A long prefix of few sequences (split over many CTAs), long ends behind a short one, more sequences than are ranked."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(B)
+  ctx = [prefix + suffix + b % 7 for b in range(B)]
+  k, v, tables = paged(ctx, 16, 1, 64, g, shared=prefix)
+  q = torch.randn(B, 4, 64, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, list(range(B)), [1] * B, None, 0.125, 0)
+  out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix, None, 0.125)
+  within(out, want, bound)
 
 
 # ------------------------------------------------------------------------------------------------ drafted tokens
