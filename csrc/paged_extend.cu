@@ -6,19 +6,24 @@
 // head of the group, 128 rows to a tile, so every K/V block is read once for all of them.  Each row carries its own
 // bounds [lo, hi) of visible keys (causal end, window, shared part); a block that lies inside all of them needs no mask.
 //
-// Pipeline of a CTA (one tile), 64 keys at a time: two loader warps gather the block's K and V rows from their pages with
-// cp.async (16 bytes a lane, any page size, zero fill outside the CTA's keys, so that what lies there cannot reach the
-// products), one thread issues the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back to
-// tensor memory as the A operand of P V.  A block is a chain of latencies (S, softmax, P V) of some 1900 cycles in which a
-// warp keeps no unit busy, so the SM is filled with chains: three CTAs for D = 64 (S single-buffered to fit tensor
-// memory), two for D = 128.  The running maximum is
-// raised only when it grows by more than 2^8; the stale one is exact after the final division.  P is rounded to bf16
-// because the tensor core multiplies it with bf16 values; the sum l takes the unrounded p.
+// Many rows (k_paged_extend), a tile a CTA, 64 keys at a time.  Two loader warps, one for K and one for V, bring a block's
+// rows from their pages, by TMA where whole boxes of keys lie in a page, else with cp.async (16 bytes a lane, any page
+// size); both leave zeros where the CTA has no keys, so that what lies there cannot reach the products.  One thread issues
+// the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back to tensor memory as the A operand
+// of P V.  The maximum is raised only when it grows by more than 2^8; the stale one is exact after the final division.  P is
+// rounded to bf16 because the tensor core multiplies it with bf16 values; the sum l takes the unrounded p.
+// A block is a chain of latencies (S 430 cycles, softmax 1050 alone and 1400 in company, P V and the way to the next S 400)
+// in which no unit is busy, so an SM is filled with chains: three CTAs for D = 64, whose S has a single buffer to fit tensor
+// memory, two for D = 128.  8 prompts of 200..1750 new tokens behind 1300..3500 cached ones, 64/8 heads of 64: 715 us, 560
+// TFLOP/s (issue slots half full, special function unit half, tensor cores a quarter).  What did not help: part of the
+// exponentials by polynomial, two warps for 32 rows, two tiles a CTA (788 us), turns between warps, polling barriers.
 //
-// Few rows: the keys are split over the CTAs of a cluster, whose (m, l, O) meet in distributed shared memory: no
-// workspace, no atomics, one launch, the same bits on every run.  Shared prefix: one launch for the prefix (rows of all
-// sequences, partial (m, l, O) to a workspace), a dependent launch for each sequence's own keys that starts while the
-// first one drains and joins its rows at the end.
+// Few rows (k_paged_few, below): decode steps and drafts, bound by the bytes of K and V.
+//
+// Few CTAs: the keys are split over the CTAs of a cluster, whose (m, l, O) meet in distributed shared memory: no workspace,
+// no atomics, one launch; beyond eight splits over several clusters and a launch that joins their sets.  Shared prefix: one
+// launch for the prefix (rows of all sequences, sets to a workspace), a dependent launch for each sequence's own keys that
+// starts while the first one drains and joins its rows at the end.  All of it gives the same bits on every run.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -773,6 +778,9 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 // barrier is needed.  Each of four warps streams its own tiles of 16 or 32 keys through a ring of its own,
 // with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
 // movmatrix; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
+// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 64 us, 4.1 TB/s (the stream itself runs at 5.5; the
+// rest is 5 us of start-up latencies a CTA and the last wave).  Equal shares of all keys for 296 CTAs, with pieces joined
+// afterwards, took 95 us: a start-up for every piece, and heads of one page no longer read together.
 template <int D, int NT>
 struct PxFew {
   static constexpr int kWarps = 4, kThreads = 128;
