@@ -241,7 +241,7 @@ struct PxSum {
     acc[4] += w * d.x; acc[5] += w * d.y; acc[6] += w * d.z; acc[7] += w * d.w;
   }
   NMOE_DEVICE void store(__nv_bfloat16* dst, float sink) const {
-    const float f = sum > 0.f ? 1.f / (sum + px_exp2(sink - top)) : 0.f;
+    const float f = sum != 0.f ? 1.f / (sum + px_exp2(sink - top)) : 0.f;     // no key: zeros; a NaN in q stays one
     int4 v;
     uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
@@ -275,12 +275,12 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
     }
 #pragma unroll
     for (int s = 0; s < 8; ++s)
-      if (ml[s].y > 0.f) mm = fmaxf(mm, ml[s].x);
+      if (ml[s].y != 0.f) mm = fmaxf(mm, ml[s].x);
     if (p.part_mode == 2)
 #pragma unroll 8
       for (int s = 0; s < p.n_sets; ++s) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-        if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+        if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
       }
     PxSum t;
     t.start(fmaxf(mm, sink));
@@ -297,7 +297,7 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
         }
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        if (s0 + s < splits && ml[s0 + s].y > 0.f) t.add(ml[s0 + s], x[s], y[s]);
+        if (s0 + s < splits && ml[s0 + s].y != 0.f) t.add(ml[s0 + s], x[s], y[s]);
     }
     if (p.part_mode == 2) {
 #pragma unroll 4
@@ -305,7 +305,7 @@ NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int star
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
         const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
         const float4 x = __ldcg(o), y = __ldcg(o + 1);
-        if (ml.y > 0.f) t.add(ml, x, y);
+        if (ml.y != 0.f) t.add(ml, x, y);
       }
     }
     if (p.part_mode == 1) {
@@ -724,7 +724,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     if (direct && my_row < n_valid) {
       const int rr = row0 + my_row, tok = rr / g, h = hk * g + rr - tok * g;
       const float sk = px_sink(p, h), mm = fmaxf(m, sk);
-      f = l > 0.f ? px_exp2(m - mm) / (l * px_exp2(m - mm) + px_exp2(sk - mm)) : 0.f;
+      f = l != 0.f ? px_exp2(m - mm) / (l * px_exp2(m - mm) + px_exp2(sk - mm)) : 0.f;
       orow = p.out + (static_cast<long long>(start + tok) * p.hq + h) * D;
     }
 #pragma unroll 1
@@ -746,7 +746,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               vv[e] = pack_bf16x2(__uint_as_float(o[8 * t + 2 * e]) * f, __uint_as_float(o[8 * t + 2 * e + 1]) * f);
-            if (!(f > 0.f)) v = make_int4(0, 0, 0, 0);
+            if (f == 0.f) v = make_int4(0, 0, 0, 0);
             reinterpret_cast<int4*>(orow + c * 32)[t] = v;
           }
         }
@@ -1054,14 +1054,14 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
 #pragma unroll
     for (int w = 0; w < F::kWarps; ++w) {
       ml[w] = *reinterpret_cast<const float2*>(smem + w * F::kRing + F::kRows * F::kOStride * 4 + r * 8);
-      if (ml[w].y > 0.f) mm = fmaxf(mm, ml[w].x);
+      if (ml[w].y != 0.f) mm = fmaxf(mm, ml[w].x);
     }
     PxSum t;
     t.start(fmaxf(mm, sink));
 #pragma unroll
     for (int w = 0; w < F::kWarps; ++w) {
       const float4* src = reinterpret_cast<const float4*>(smem + w * F::kRing + (r * F::kOStride + c * 8) * 4);
-      if (ml[w].y > 0.f) t.add(ml[w], src[0], src[1]);
+      if (ml[w].y != 0.f) t.add(ml[w], src[0], src[1]);
     }
     if (direct) {
       t.store(p.out + (static_cast<long long>(start + tok) * p.hq + h) * D + c * 8, sink);
@@ -1095,7 +1095,7 @@ __global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
 #pragma unroll 4
   for (int s = kParts > 1 ? threadIdx.x : 0; s < p.n_sets; s += kParts > 1 ? 128 : 1) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-    if (ml.y > 0.f) mm = fmaxf(mm, ml.x);
+    if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
   }
   if constexpr (kParts > 1) {
     mm = warp_max(mm);
@@ -1110,7 +1110,7 @@ __global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
     const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
     const float4 x = __ldcg(o), y = __ldcg(o + 1);
-    if (ml.y > 0.f) t.add(ml, x, y);
+    if (ml.y != 0.f) t.add(ml, x, y);
   }
   if constexpr (kParts > 1) {
 #pragma unroll

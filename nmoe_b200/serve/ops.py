@@ -230,7 +230,7 @@ def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_st
       seen = seen & (pos > at - window)
     s = s.masked_fill(~seen, float("-inf"))
     sk = torch.full((Hq, n, 1), float("-inf"), device=q.device) if sinks is None else sinks.float().view(Hq, 1, 1).expand(Hq, n, 1)
-    p = torch.softmax(torch.cat((s, sk), dim=-1), dim=-1)[..., :-1].nan_to_num(0.0)       # a row that sees nothing gives zeros
+    p = torch.softmax(torch.cat((s, sk), dim=-1), dim=-1)[..., :-1].masked_fill(~seen.any(-1).unsqueeze(-1), 0.0)
     out[s0:s0 + n] = torch.einsum("hnk,khd->nhd", p, v).to(out.dtype)
   return out
 

@@ -30,6 +30,17 @@ def test_paged_extend_plain(window):
   assert torch.equal(keep[owned], out[owned]) and (keep[~owned] == 2.0).all()
 
 
+def test_a_nan_in_q_stays_in_its_row():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  args = (k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25)
+  clean = S.paged_extend(q, *args)
+  q[4, 1, 0] = float("nan")
+  out = S.paged_extend(q, *args)
+  assert out[4, 1].isnan().all()
+  out[4, 1] = clean[4, 1]
+  assert torch.equal(out, clean)
+
+
 def test_shared_prefix_decode_plain_equals_paged_decode():
   g = torch.Generator().manual_seed(0)
   ctx = [21, 40, 0, 33, 12]

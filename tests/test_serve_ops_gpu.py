@@ -211,6 +211,39 @@ def test_paged_extend_large_scores_and_extreme_sinks():
   within(out, want, bound)
 
 
+@pytest.mark.parametrize("lens,ctx,D", [([5], [700], 64), ([1], [30_000], 64), ([1] * 9, [90] * 9, 128), ([140], [900], 64),
+                                        ([90], [140], 128), ([60], [9000], 128), ([3, 0, 2], [3, 0, 50], 64)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_paged_extend_a_nan_in_q_stays_in_its_row(lens, ctx, D, window):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(D)
+  k, v, tables = paged(ctx, 16, 2, D, g)
+  starts = [sum(lens[:b]) for b in range(len(lens))]
+  q = torch.randn(sum(lens), 8, D, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, starts, lens, None, D ** -0.5, window)
+  r = sum(lens) // 2
+  q[r, 2, 7], q[r, 5] = float("nan"), float("inf")
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, D ** -0.5, window).cpu()
+  assert out[r, [2, 5]].isnan().all()
+  out[r, [2, 5]] = want[r, [2, 5]].bfloat16()
+  within(out, want, bound)
+
+
+def test_shared_prefix_decode_a_nan_in_q_stays_in_its_row():
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(1)
+  for B, hq in ((3, 8), (40, 8)):
+    ctx = [200 + 3 * b for b in range(B)]
+    k, v, tables = paged(ctx, 16, 2, 64, g, shared=160)
+    q = torch.randn(B, hq, 64, generator=g).bfloat16()
+    want, bound, _ = attend(q, k, v, tables, ctx, list(range(B)), [1] * B, None, 0.125, 0)
+    q[1, 3, 0] = float("nan")
+    out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), 160, None, 0.125).cpu()
+    assert out[1, 3].isnan().all()
+    out[1, 3] = want[1, 3].bfloat16()
+    within(out, want, bound)
+
+
 def test_paged_extend_reports_bad_pages_and_lengths():
   from nmoe_b200.ops import tc_gemm as G
   from nmoe_b200.ops._lib import NativeLibraryError
