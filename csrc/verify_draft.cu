@@ -249,7 +249,7 @@ extern "C" int nmoe_verify_draft(const float* target, long long target_stride, c
                                  const int* q_lens, int* out, int* n_out, int n_rows, int n_seqs, int vocab, void* status,
                                  cudaStream_t st) {
   if (n_seqs == 0) return 0;
-  if (n_seqs < 0 || n_rows < 0 || vocab < 1) return -1;
+  if (n_seqs < 0 || n_rows < 0 || vocab < 1 || vocab > 1 << 30) return -1;     // indices of a stretch stay within 32 bits
   VerifyParams p;
   p.target = target; p.draft = draft; p.tokens = tokens; p.uniforms = uniforms; p.q_starts = q_starts; p.q_lens = q_lens;
   p.out = out; p.n_out = n_out; p.status = static_cast<StatusRecord*>(status);

@@ -252,8 +252,8 @@ def _check_attention(q, k_cache, v_cache, block_tables, context_lens, sinks, sca
     raise ValueError("block_tables must be [B, n], context_lens [B]")
   if sinks is not None and (sinks.shape != (Hq,) or sinks.device != dev):
     raise ValueError("sinks must be [Hq] on q's device")
-  if window < 0:
-    raise ValueError("window must not be negative")
+  if not 0 <= window < 2 ** 31:
+    raise ValueError("window must not be negative, nor pass 32 bits")
   if not scale > 0:
     raise ValueError("scale must be positive")
   if not q.is_cuda:
@@ -404,8 +404,8 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
   Returns (out [N] int32: the emitted tokens from row q_starts[b] on, -1 behind them; n_out [B] int32: how many, at least 1
   for a sequence with rows).  Rows of no sequence are -1, or left as they were in a given ``out``.  A drafted token outside
   the vocabulary fails and shows up in ``check_status``."""
-  if target_probs.dim() != 2 or target_probs.size(1) == 0:
-    raise ValueError("target_probs must be [N, V]")
+  if target_probs.dim() != 2 or not 0 < target_probs.size(1) <= 2 ** 30:
+    raise ValueError("target_probs must be [N, V], V up to 2^30")
   N, V = target_probs.shape
   dev = target_probs.device
   if target_probs.dtype != torch.float32:
@@ -424,6 +424,9 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
     _check_int32(out, dev, "out")
     if out.shape != (N,) or not out.is_contiguous():
       raise ValueError("out must be a contiguous [N]")
+    first, ends = tokens.data_ptr(), ((N - 1) * tokens.stride(0) + 1) * tokens.element_size()
+    if N > 0 and first < out.data_ptr() + 4 * N and out.data_ptr() < first + ends:
+      raise ValueError("out must not overlap tokens, which are read while it is written")
   if not target_probs.is_cuda:
     return verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, draft_probs, out)
   if target_probs.stride(1) != 1 and V > 1:

@@ -113,6 +113,29 @@ def test_refusals():
       S.verify_draft(**{**ok, **bad})
 
 
+def test_verify_draft_refuses_to_write_over_its_tokens():
+  t, u, one = torch.rand(4, 9), torch.rand(4), i32([0])
+  room = torch.zeros(9, dtype=torch.int32)
+  for at in (0, 3, 4, 5):                           # tokens are room[4:8] (the last one has its own place)
+    if at in (0,):
+      S.verify_draft(t, room[4:8], u, one, i32([4]), out=room[0:4])
+    else:
+      with pytest.raises(ValueError, match="overlap"):
+        S.verify_draft(t, room[4:8], u, one, i32([4]), out=room[at:at + 4])
+  with pytest.raises(ValueError, match="overlap"):
+    S.verify_draft(t, room[1:9:2], u, one, i32([4]), out=room[4:8])
+
+
+def test_sizes_past_32_bits_are_refused():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  S.paged_extend(q, k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, 2 ** 31 - 1)
+  with pytest.raises(ValueError, match="32 bits"):
+    S.paged_extend(q, k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, 2 ** 32 + 5)
+  t = torch.rand(1, 1).expand(2, 2 ** 30 + 1)
+  with pytest.raises(ValueError, match="2\\^30"):
+    S.verify_draft(t, i32([0, 0]), torch.rand(2), i32([0]), i32([2]))
+
+
 def test_status_record_made_in_inference_mode_can_be_reset():
   from nmoe_b200.ops import tc_gemm as G
   from nmoe_b200.ops._lib import NativeLibraryError
