@@ -244,6 +244,62 @@ def test_shared_prefix_decode_a_nan_in_q_stays_in_its_row():
     within(out, want, bound)
 
 
+def test_a_cache_past_32_bits():
+  """Pages behind the first 2^32 bytes and 2^31 elements of a cache give what the same pages give in a small one."""
+  from nmoe_b200.serve import ops as S
+  bs, hkv, D, far = 64, 8, 64, 2 ** 31 // (64 * 8 * 64) + 3
+  g = torch.Generator().manual_seed(2)
+  ctx, lens, starts = [640, 130], [60, 3], [0, 60]
+  k, v, tables = paged(ctx, bs, hkv, D, g, shared=64)
+  n = k.size(0)
+  big = [torch.empty(far + n, bs, hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+  for c, small in zip(big, (k, v)):
+    c[far:] = small.to(DEV)
+  small = (k.to(DEV), v.to(DEV))
+  t_small = tables.to(DEV)
+  t_big = torch.where(t_small >= 0, t_small + far, t_small)
+  q = torch.randn(63, 64, D, generator=g).bfloat16().to(DEV)
+  call = lambda c, t: (S.paged_extend(q, *c, t, i32(ctx), i32(starts), i32(lens), None, 0.125),
+                       S.paged_extend(q[60:], *c, t[1:], i32(ctx[1:]), i32([0]), i32([3]), None, 0.125),
+                       S.shared_prefix_decode(q[:2], *c, t, i32(ctx), 64, None, 0.125))
+  for a, b in zip(call(small, t_small), call(big, t_big)):
+    assert torch.equal(a, b)
+  qkv = torch.randn(5, 80 * D, generator=g).bfloat16().to(DEV)
+  slots = i32([0, 7, n * bs - 1, -1, bs])
+  pos, inv = torch.arange(5, device=DEV), torch.ones(32, device=DEV)
+  S.rope_append(qkv, pos, inv, 1.0, 64, 8, *small, slots)
+  S.rope_append(qkv, pos, inv, 1.0, 64, 8, *big, torch.where(slots >= 0, slots + far * bs, slots))
+  assert all(torch.equal(c[far:], s) for c, s in zip(big, small))
+
+
+def test_calls_on_two_streams_at_once():
+  """Calls with workspaces and clusters beside each other, as two engines in one process make them."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(3)
+  cases = []
+  for ctx, lens in (([30_000], [1]), ([900, 4000, 80], [70, 5, 80])):
+    k, v, tables = paged(ctx, 16, 2, 64, g)
+    starts = [sum(lens[:b]) for b in range(len(lens))]
+    q = torch.randn(sum(lens), 8, 64, generator=g).bfloat16().to(DEV)
+    cases.append((q, k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, 0.125))
+  ctx = [2000 + b for b in range(30)]
+  k, v, tables = paged(ctx, 16, 2, 64, g, shared=1600)
+  shared = (torch.randn(30, 8, 64, generator=g).bfloat16().to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), 1600, None, 0.125)
+  step = lambda: [S.paged_extend(*c) for c in cases] + [S.shared_prefix_decode(*shared)]
+  want = step()
+  streams = [torch.cuda.Stream() for _ in range(2)]
+  got = [[], []]
+  torch.cuda.synchronize()
+  for _ in range(5):
+    for i, s in enumerate(streams):
+      with torch.cuda.stream(s):
+        got[i].append(step())
+  torch.cuda.synchronize()
+  for runs in got:
+    for run in runs:
+      assert all(torch.equal(a, b) for a, b in zip(run, want))
+
+
 def test_paged_extend_reports_bad_pages_and_lengths():
   from nmoe_b200.ops import tc_gemm as G
   from nmoe_b200.ops._lib import NativeLibraryError
