@@ -308,7 +308,7 @@ class Transformer(nn.Module):
     start = 0 if from_layer is None else max(0, min(L, int(from_layer)))
     stop = L if up_to_layer is None else max(start, min(L, int(up_to_layer)))
     x = hidden_in if (start > 0 and hidden_in is not None) else ops.embedding(input_ids, self.embed, 1.0)
-    rot = (self.inv_freq, self.conc)
+    rot = (self.inv_freq.float(), self.conc)                    # Module.to(dtype) casts the buffer too
     taps: Dict[int, torch.Tensor] = {}
     mode = "prefill" if is_prefill else "decode" if cache.q_lens is None else "extend"
     for i in range(start, stop):

@@ -90,3 +90,17 @@ def test_generate_with_drafts_and_a_shared_rubric(models, temperature, top_k, mo
   assert all(len(o) == 30 and all(0 <= t < 512 for t in o) for o in out)
   assert eng.steps["drafted"] > 0 and eng.pool.n_free == eng.num_blocks
   G.check_status()
+
+
+def test_a_model_cast_as_a_whole_still_runs(models):
+  """Module.to casts the rotary frequencies with the weights; the step takes them as they are."""
+  mg, _ = models
+  ids = torch.arange(24, device="cuda").view(1, 24)
+  pos = torch.arange(24, device="cuda").view(1, 24)
+  want, kept = mg(ids, pos), mg.inv_freq
+  try:
+    mg.inv_freq = kept.bfloat16()
+    got = mg(ids, pos)
+  finally:
+    mg.inv_freq = kept
+  assert got.shape == want.shape and _cos(got, want) > 0.9      # frequencies rounded to 8 bits: up to 24 * 2^-9 radians off
