@@ -173,40 +173,51 @@ NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start,
   }
 }
 // The list of blocks with index z: the z-th longest context where one wave of CTAs does not hold them all, so that the long
-// ones start first and the short ones fill the end.  Every CTA ranks the contexts for itself.
+// ones start first and the short ones fill the end (64 drafted steps: 102 -> 74 us).  Every CTA ranks the contexts for itself,
+// as numbers that also hold the index, so that no two are the same and one comparison does (contexts from 2^23 on count alike).
 constexpr int PX_SORT_MOST = 256;
 template <int kThreads>
-NMOE_DEVICE int px_nth_longest(const ExtendParams& p, int z, int* s_len) {         // s_len: PX_SORT_MOST + 1 words of scratch
-  int& s_which = s_len[PX_SORT_MOST];
+NMOE_DEVICE int px_nth_longest(const ExtendParams& p, int z, int* s_key) {         // s_key: PX_SORT_MOST + 1 words of scratch
+  constexpr int kEach = (PX_SORT_MOST + kThreads - 1) / kThreads;
   const int n4 = (p.n_seqs + 3) / 4;
-  for (int t = threadIdx.x; t < 4 * n4; t += kThreads)
-    s_len[t] = t >= p.n_seqs ? -0x7fffffff - 1 : p.q_lens != nullptr && p.q_lens[t] <= 0 ? -1 : p.context_lens[t];
-  __syncthreads();
-  for (int t = threadIdx.x; t < p.n_seqs; t += kThreads) {
-    const int mine = s_len[t];
-    int rank = 0;
-    for (int u = 0; u < n4; ++u) {
-      const int4 v = reinterpret_cast<const int4*>(s_len)[u];
-      rank += (v.x > mine || (v.x == mine && 4 * u < t)) + (v.y > mine || (v.y == mine && 4 * u + 1 < t)) +
-              (v.z > mine || (v.z == mine && 4 * u + 2 < t)) + (v.w > mine || (v.w == mine && 4 * u + 3 < t));
-    }
-    if (rank == z) s_which = t;
+  int key[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int t = threadIdx.x + k * kThreads;
+    const bool in = t < p.n_seqs;
+    const int len = in && !(p.q_lens != nullptr && p.q_lens[t] <= 0) ? min(max(p.context_lens[t], 0), 0x7fffff) : 0;
+    key[k] = in ? len * PX_SORT_MOST + (PX_SORT_MOST - 1 - t) : -1;
+    if (t < 4 * n4) s_key[t] = key[k];
   }
   __syncthreads();
-  const int which = s_which;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int t = threadIdx.x + k * kThreads;
+    if (t >= p.n_seqs) break;
+    int rank = 0;
+    for (int u = 0; u < n4; ++u) {
+      const int4 v = reinterpret_cast<const int4*>(s_key)[u];
+      rank += (v.x > key[k]) + (v.y > key[k]) + (v.z > key[k]) + (v.w > key[k]);
+    }
+    if (rank == z) s_key[PX_SORT_MOST] = t;
+  }
+  __syncthreads();
+  const int which = s_key[PX_SORT_MOST];
   __syncthreads();                                               // the scratch may be used for something else
   return which;
 }
 // Whose pages hold the keys of a list that all sequences share: the first sequence that reaches its end (a padding row does
-// not), else the longest.
-NMOE_DEVICE int px_owner(const ExtendParams& p) {
+// not), else the longest.  By a whole warp.
+NMOE_DEVICE int px_owner(const ExtendParams& p, int lane) {
   int best = 0, most = -1;
-  for (int t = 0; t < p.n_seqs; ++t) {
-    const int c = p.context_lens[t];
-    if (c >= p.key_end) return t;
+  for (int t0 = 0; t0 < p.n_seqs; t0 += 32) {
+    const int t = t0 + lane, c = t < p.n_seqs ? p.context_lens[t] : -1;
+    const unsigned all = __ballot_sync(0xffffffffu, t < p.n_seqs && c >= p.key_end);
+    if (all != 0) return t0 + __ffs(all) - 1;
     if (c > most) { most = c; best = t; }
   }
-  return best;
+  const int top = __reduce_max_sync(0xffffffffu, most);
+  return __reduce_min_sync(0xffffffffu, most == top ? best : 0x7fffffff);
 }
 // Keys [lo, hi) that a token of the list sees.
 NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool speaker, int& lo, int& hi) {
@@ -225,100 +236,140 @@ NMOE_DEVICE float px_sink(const ExtendParams& p, int h) {         // log2 units
                                              : __bfloat162float(static_cast<const __nv_bfloat16*>(p.sinks)[h]));
 }
 
-// Sum of (m, l, O) pieces relative to a common maximum, 8 columns a thread.
+NMOE_DEVICE void px_store(__nv_bfloat16* dst, float4 a, float f) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f));
+}
+// what scales a sum relative to `top` to the result: 1 / (sum + sink's part); no key: zeros; a NaN in q stays one
+NMOE_DEVICE float px_factor(float top, float sum, float sink) {
+  const float high = fmaxf(top, sink), e = px_exp2(top - high);
+  return sum != 0.f ? e / (sum * e + px_exp2(sink - high)) : 0.f;
+}
+NMOE_DEVICE void px_axpy(float4& y, float w, float4 x) { y.x += w * x.x; y.y += w * x.y; y.z += w * x.z; y.w += w * x.w; }
+// Sum of (m, l, O) pieces relative to a common maximum, 4 columns a thread.
 struct PxSum {
-  float top, sum, acc[8];
+  float top, sum;
+  float4 acc;
   NMOE_DEVICE void start(float t) {
     top = t;
     sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  NMOE_DEVICE void add(float2 ml, float4 a, float4 d) {
+  NMOE_DEVICE void add(float2 ml, float4 a) {
     const float w = px_exp2(ml.x - top);
     sum += w * ml.y;
-    acc[0] += w * a.x; acc[1] += w * a.y; acc[2] += w * a.z; acc[3] += w * a.w;
-    acc[4] += w * d.x; acc[5] += w * d.y; acc[6] += w * d.z; acc[7] += w * d.w;
+    px_axpy(acc, w, a);
   }
-  NMOE_DEVICE void store(__nv_bfloat16* dst, float sink) const {
-    const float f = sum != 0.f ? 1.f / (sum + px_exp2(sink - top)) : 0.f;     // no key: zeros; a NaN in q stays one
-    int4 v;
-    uint32_t* vv = reinterpret_cast<uint32_t*>(&v);
+  // the sets first, first + step, ... of a row, kAtOnce of them on their way; rows without keys hold zeros
+  template <int D, int kAtOnce>
+  NMOE_DEVICE void add_sets(const ExtendParams& p, long long row, int c, int first, int step) {
+    for (int s0 = first; s0 < p.n_sets; s0 += kAtOnce * step) {
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) vv[e] = pack_bf16x2(acc[2 * e] * f, acc[2 * e + 1] * f);
-    *reinterpret_cast<int4*>(dst) = v;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int s = s0 + u * step;
+        ml[u] = make_float2(0.f, 0.f);
+        if (s < p.n_sets) {
+          ml[u] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
+          x[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + c);
+        }
+      }
+      float high = top;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (ml[u].y != 0.f) high = fmaxf(high, ml[u].x);
+      const float w = px_exp2(top - high);
+      top = high;
+      sum *= w;
+      acc.x *= w; acc.y *= w; acc.z *= w; acc.w *= w;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (ml[u].y != 0.f) add(ml[u], x[u]);
+    }
   }
+  NMOE_DEVICE void store(__nv_bfloat16* dst, float sink) const { px_store(dst, acc, px_factor(top, sum, sink)); }
 };
 
-// Joins what the CTAs of a cluster hold for the rows row0 .. row0 + n_valid (sx [rows][D] fp32 in 16-byte pieces swizzled
-// by row, s_ml [rows][2]) and, in part_mode 2, the sets of the launch before.  Every CTA takes a run of the rows.
-template <int D, int kThreads>
-NMOE_DEVICE void px_join(const ExtendParams& p, float* sx, float* s_ml, int start, int row0, int n_valid, int hk, int unit) {
+// Joins what the kS CTAs of a cluster hold for the rows row0 .. row0 + n_valid (sx [rows][D] fp32 in 16-byte pieces swizzled
+// by row, s_ml [rows][2]) and, in part_mode 2, the sets of the launch before.  Every CTA takes a run of the rows: a thread a
+// row works out what each part counts for (s_w, [rows][kS + 3]), then all threads sum the columns, with the loads of several
+// sums in flight, since a remote read takes some hundred cycles (doing both per column took 7 us where this takes 3).
+template <int D, int kThreads, int kS>
+NMOE_DEVICE void px_join_of(const ExtendParams& p, const float* sx, const float* s_ml, float* s_w, int start, int row0, int n_valid, int hk, int unit) {
   cg::cluster_group cl = cg::this_cluster();
-  const int splits = p.splits, rank = unit % splits, group = unit / splits, g = p.group;
-  if (splits > 1) cl.sync();
+  constexpr int kW = kS + 3;                                     // weights, maximum, sum, row of the result
+  const int rank = unit % kS, group = unit / kS, g = p.group;
+  if (kS > 1) cl.sync();
   else __syncthreads();
-  if (p.part_mode == 2) px_wait_prior_grid();
-  const int per = (n_valid + splits - 1) / splits;
-  const int ra = rank * per, rb = min(n_valid, ra + per);
-  for (int i = threadIdx.x; i < (rb - ra) * (D / 8); i += kThreads) {
-    const int r = ra + i / (D / 8), c = i % (D / 8);
-    const int rr = row0 + r, tok = rr / g, h = hk * g + rr - tok * g;
+  const int per = (n_valid + kS - 1) / kS;
+  const int ra = rank * per, n_mine = max(min(n_valid, ra + per) - ra, 0);
+  auto of = [&](const float* at, int s) -> const float* { return kS > 1 ? cl.map_shared_rank(const_cast<float*>(at), s) : at; };
+  for (int i = threadIdx.x; i < n_mine; i += kThreads) {
+    const int r = ra + i, rr = row0 + r, tok = rr / g, h = hk * g + rr - tok * g;
     const long long row = static_cast<long long>(start + tok) * p.hq + h;
-    const float sink = p.part_mode == 1 ? -INFINITY : px_sink(p, h);
-    float mm = -1e30f;
-    float2 ml[8];                                                // all loads before the first use: a remote read takes some 200 cycles
+    float2 ml[kS];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      ml[s] = make_float2(0.f, 0.f);
-      if (s < splits) ml[s] = *reinterpret_cast<const float2*>(splits > 1 ? cl.map_shared_rank(s_ml + 2 * r, s) : s_ml + 2 * r);
+    for (int s = 0; s < kS; ++s) ml[s] = *reinterpret_cast<const float2*>(of(s_ml + 2 * r, s));
+    float top = -1e30f, sum = 0.f, w[kS], f = 1.f;
+#pragma unroll
+    for (int s = 0; s < kS; ++s)
+      if (ml[s].y != 0.f) top = fmaxf(top, ml[s].x);
+#pragma unroll
+    for (int s = 0; s < kS; ++s) {
+      w[s] = ml[s].y != 0.f ? px_exp2(ml[s].x - top) : 0.f;
+      sum += w[s] * ml[s].y;
+    }
+    if (p.part_mode == 0) f = px_factor(top, sum, px_sink(p, h));
+    else if (p.part_mode == 1) reinterpret_cast<float2*>(p.part_ml)[group * p.set_rows + row] = make_float2(top, sum);
+#pragma unroll
+    for (int s = 0; s < kS; ++s) s_w[i * kW + s] = w[s] * f;
+    s_w[i * kW + kS] = top;
+    s_w[i * kW + kS + 1] = sum;
+    s_w[i * kW + kS + 2] = __int_as_float(static_cast<int>(row));
+  }
+  if (p.part_mode == 2) px_wait_prior_grid();
+  __syncthreads();
+  constexpr int kCols = D / 4, kItems = kS <= 2 ? 4 : kS == 4 ? 2 : 1;             // up to eight pieces of 16 bytes on their way
+  const int n_items = n_mine * kCols;
+  for (int i0 = threadIdx.x; i0 < n_items; i0 += kThreads * kItems) {
+    float4 x[kItems][kS];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int i = min(i0 + k * kThreads, n_items - 1), r = ra + i / kCols, c = i % kCols;
+#pragma unroll
+      for (int s = 0; s < kS; ++s) x[k][s] = reinterpret_cast<const float4*>(of(sx + r * D, s))[c ^ (r & 7)];
     }
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (ml[s].y != 0.f) mm = fmaxf(mm, ml[s].x);
-    if (p.part_mode == 2)
-#pragma unroll 8
-      for (int s = 0; s < p.n_sets; ++s) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-        if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
+    for (int k = 0; k < kItems; ++k) {
+      const int i = i0 + k * kThreads, c = i % kCols;
+      if (i >= n_items) break;
+      const float* w = s_w + i / kCols * kW;
+      const long long row = __float_as_int(w[kS + 2]);
+      PxSum t;
+      t.start(w[kS]);
+      t.sum = w[kS + 1];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) px_axpy(t.acc, w[s], x[k][s]);
+      if (p.part_mode == 0) {
+        px_store(p.out + row * D + c * 4, t.acc, 1.f);
+      } else if (p.part_mode == 1) {
+        reinterpret_cast<float4*>(p.part_o + (group * p.set_rows + row) * D)[c] = t.acc;
+      } else {
+        t.add_sets<D, 4>(p, row, c, 0, 1);
+        t.store(p.out + row * D + c * 4, px_sink(p, static_cast<int>(row % p.hq)));
       }
-    PxSum t;
-    t.start(fmaxf(mm, sink));
-#pragma unroll
-    for (int s0 = 0; s0 < 8; s0 += 4) {
-      if (s0 >= splits) break;
-      float4 x[4], y[4];
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (s0 + s < splits) {
-          const float4* xr = reinterpret_cast<const float4*>(splits > 1 ? cl.map_shared_rank(sx + r * D, s0 + s) : sx + r * D);
-          x[s] = xr[(2 * c) ^ (r & 7)];
-          y[s] = xr[(2 * c + 1) ^ (r & 7)];
-        }
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (s0 + s < splits && ml[s0 + s].y != 0.f) t.add(ml[s0 + s], x[s], y[s]);
-    }
-    if (p.part_mode == 2) {
-#pragma unroll 4
-      for (int s = 0; s < p.n_sets; ++s) {                       // rows without keys hold zeros: nothing here waits for a comparison
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-        const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
-        const float4 x = __ldcg(o), y = __ldcg(o + 1);
-        if (ml.y != 0.f) t.add(ml, x, y);
-      }
-    }
-    if (p.part_mode == 1) {
-      const long long at = group * p.set_rows + row;
-      float4* o = reinterpret_cast<float4*>(p.part_o + at * D) + 2 * c;
-      o[0] = make_float4(t.acc[0], t.acc[1], t.acc[2], t.acc[3]);
-      o[1] = make_float4(t.acc[4], t.acc[5], t.acc[6], t.acc[7]);
-      if (c == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(t.top, t.sum);
-    } else {
-      t.store(p.out + row * D + c * 8, sink);
     }
   }
-  if (splits > 1) cl.sync();                                     // nobody leaves while its rows may still be read
+  if (kS > 1) cl.sync();                                         // nobody leaves while its rows may still be read
+}
+template <int D, int kThreads>
+NMOE_DEVICE void px_join(const ExtendParams& p, const float* sx, const float* s_ml, float* s_w, int start, int row0, int n_valid, int hk, int unit) {
+  switch (p.splits) {
+    case 1: px_join_of<D, kThreads, 1>(p, sx, s_ml, s_w, start, row0, n_valid, hk, unit); break;
+    case 2: px_join_of<D, kThreads, 2>(p, sx, s_ml, s_w, start, row0, n_valid, hk, unit); break;
+    case 4: px_join_of<D, kThreads, 4>(p, sx, s_ml, s_w, start, row0, n_valid, hk, unit); break;
+    default: px_join_of<D, kThreads, 8>(p, sx, s_ml, s_w, start, row0, n_valid, hk, unit); break;
+  }
 }
 
 // Layout of shared memory.  The exchange of partial results reuses the stages (O as fp32, 16-byte pieces swizzled by row).
@@ -338,7 +389,7 @@ struct PxSmem {
   static constexpr uint32_t kTmemCols = kBufs * PX_BN + D;
 };
 
-template <int D>
+template <int D, bool kDirect>
 __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas)
 k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using SM = PxSmem<D>;
@@ -358,9 +409,9 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
   uint64_t* p_full = s_full + kBufs;         // [kBufs]
   uint64_t* pv_done = p_full + kBufs;
   uint64_t* o_full = pv_done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  uint64_t* q_full = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_range = reinterpret_cast<int*>(tmem_slot + 2);          // [2] first key, end of keys
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the keys are divided over units = groups x splits CTAs, the splits of a group being a cluster
@@ -380,15 +431,12 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     if (p.part_mode == 2) px_wait_prior_grid();
     return;
   }
-  const int* table = p.block_tables + (p.flat ? px_owner(p) : b) * p.bt_stride;
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kStages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
     for (int i = 0; i < kBufs; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], (n_valid + 31) / 32); }
     mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
-    s_range[0] = 0x7fffffff;
-    s_range[1] = 0;
+    mbar_init(q_full, 4);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -396,56 +444,91 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     tmem_alloc(tmem_slot, SM::kTmemCols);
     tmem_relinquish();
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
-  // Row r of the tile lies in lane r + 32 * turn of tensor memory (modulo 128), the turn differing between the CTAs of an
-  // SM: the busy warps of tiles with few rows then sit on different schedulers.
-  const int turn = static_cast<int>((tmem_base & 511u) / SM::kTmemCols) * (4 / SM::kBufs / 2 + 1) & 3;
-  // rows of Q, 128-byte swizzle, K-major; rows that do not exist are zero
+  // keys that the tile sees, worked out by every warp for itself
+  int k_begin = 0x7fffffff, k_end = 0;
   {
-    constexpr int kPieces = PX_BM * (D / 8), kEach = (kPieces + kThreads - 1) / kThreads;
-    const int tok0 = row0 / g, rem0 = row0 - tok0 * g;
-    int4 v[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {                            // all loads of a thread before the first store
-      const int i = threadIdx.x + k * kThreads, r = i / (D / 8), c = i % (D / 8);
-      v[k] = make_int4(0, 0, 0, 0);
-      if (i < kPieces && r < n_valid) {
-        const int dt = px_div(rem0 + r, inv_g), h = hk * g + rem0 + r - dt * g;
-        v[k] = ld_nc_v4(p.q + (start + tok0 + dt) * p.q_stride + static_cast<long long>(h) * D + c * 8);
+    const int tok_a = row0 / g, tok_b = (row0 + n_valid - 1) / g;
+    if (p.flat) {
+      for (int t = tok_a + lane; t <= tok_b; t += 32) {
+        int from, to;
+        px_bounds(p, t, n, ctx, false, from, to);
+        if (from < to) { k_begin = min(k_begin, from); k_end = max(k_end, to); }
       }
-    }
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int i = threadIdx.x + k * kThreads, r = i / (D / 8), c = i % (D / 8), at = (r + 32 * turn) & 127;
-      if (i < kPieces)
-        *reinterpret_cast<int4*>(sQ + (c >> 3) * (PX_BM * 128) + at * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
-    }
-  }
-  fence_proxy_async_smem();
-  // every CTA holds its tensor memory before a dependent launch may ask for some
-  if (p.part_mode == 1) px_launch_dependents();
-
-  // bounds of this thread's row
-  int lo = 0, hi = 0;
-  const int quad_row = (((warp & 3) - turn) & 3) * 32, my_row = quad_row + lane;         // softmax threads: row of the tile
-  const bool softmax_warp = warp < kMmaWarp && quad_row < n_valid;
-  if (softmax_warp && my_row < n_valid) {
-    px_bounds(p, (row0 + my_row) / g, n, ctx, hk == 0 && unit == 0 && (row0 + my_row) % g == 0, lo, hi);
-    if (lo < hi) {
-      atomicMin(&s_range[0], lo);
-      atomicMax(&s_range[1], hi);
+      k_begin = __reduce_min_sync(0xffffffffu, k_begin);
+      k_end = __reduce_max_sync(0xffffffffu, k_end);
+    } else {                                                     // both bounds grow from token to token
+      int skip;
+      px_bounds(p, tok_a, n, ctx, false, k_begin, skip);
+      px_bounds(p, tok_b, n, ctx, false, skip, k_end);
     }
   }
-  __syncthreads();
-  const int k_begin = s_range[0], k_end = s_range[1];
   // blocks start on a box of keys, so that all but the first and the last are whole boxes
   const int k_from = p.tma_rows > 0 && k_end > k_begin ? k_begin - k_begin % p.tma_rows : k_begin;
   const int n_blocks_all = k_end > k_begin ? (k_end - k_from + PX_BN - 1) / PX_BN : 0;
   const int blk0 = px_share(n_blocks_all, unit, units), n_blk = px_share(n_blocks_all, unit + 1, units) - blk0;
   const int key0 = n_blk > 0 ? k_from + blk0 * PX_BN : 0;        // first key of this CTA
+
+  // What a loader looks up: a page and a place in it; they become a row only when the block's turn comes, so that nothing waits
+  // for the page table meanwhile.  -1: zeros, -2: no such page.
+  struct Spot { int page, in_page; };
+  const int rows = p.tma_rows, n_box = rows > 0 ? PX_BN / rows : 0;
+  const int* table = nullptr;
+  Spot next[2];
+  auto whole = [&](int i) -> bool {
+    const int k0 = key0 + i * PX_BN;
+    return rows > 0 && k0 >= k_begin && k0 + PX_BN <= k_end;
+  };
+  auto spot_of = [&](int key) -> Spot {
+    if (key < k_begin || key >= k_end) return {-1, -1};
+    const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
+    return {__ldg(table + pi), key - pi * p.block_size};
+  };
+  auto look_up = [&](int i) {                                    // this lane's box, or its two keys, of block i
+    next[0] = next[1] = {-1, -1};
+    if (i >= n_blk) return;
+    const int k0 = key0 + i * PX_BN;
+    if (whole(i)) {
+      if (lane < n_box) next[0] = spot_of(k0 + lane * rows);
+    } else {
+      next[0] = spot_of(k0 + lane);
+      next[1] = spot_of(k0 + 32 + lane);
+    }
+  };
+  if (warp > kMmaWarp) {
+    table = p.block_tables + (p.flat ? px_owner(p, lane) : b) * p.bt_stride;
+    look_up(0);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  // every CTA holds its tensor memory before a dependent launch may ask for some
+  if (p.part_mode == 1) px_launch_dependents();
+  const uint32_t tmem_base = *tmem_slot;
+  // Row r of the tile lies in lane r + 32 * turn of tensor memory (modulo 128), the turn differing between the CTAs of an
+  // SM: the busy warps of tiles with few rows then sit on different schedulers.
+  const int turn = static_cast<int>((tmem_base & 511u) / SM::kTmemCols) * (4 / SM::kBufs / 2 + 1) & 3;
+  const int quad_row = (((warp & 3) - turn) & 3) * 32, my_row = quad_row + lane;         // softmax threads: row of the tile
+  const bool softmax_warp = warp < kMmaWarp && quad_row < n_valid;
+  int lo = 0, hi = 0;                                            // bounds of this thread's row
+  if (warp < kMmaWarp) {
+    // rows of Q, 128-byte swizzle, K-major; rows that do not exist are zero
+    const int tok0 = row0 / g, rem0 = row0 - tok0 * g, c = threadIdx.x % (D / 8);
+    const uint32_t dst = smem_u32(sQ) + (c >> 3) * (PX_BM * 128);
+#pragma unroll
+    for (int r = threadIdx.x / (D / 8); r < PX_BM; r += 128 / (D / 8)) {
+      const bool in = r < n_valid;
+      const int dt = in ? px_div(rem0 + r, inv_g) : 0, h = hk * g + (in ? rem0 + r - dt * g : 0);
+      px_cp16(dst + ((r + 32 * turn) & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+              p.q + (start + tok0 + dt) * p.q_stride + static_cast<long long>(h) * D + c * 8, in ? 16u : 0u);
+    }
+    px_cp_commit();
+    px_cp_wait<0>();
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    if (softmax_warp && my_row < n_valid)
+      px_bounds(p, (row0 + my_row) / g, n, ctx, hk == 0 && unit == 0 && (row0 + my_row) % g == 0, lo, hi);
+  }
 
   bool ok = true;
   float m = -1e30f, l = 0.f;
@@ -464,35 +547,9 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     const CUtensorMap* map = is_v ? &tm_v : &tm_k;
     uint64_t *full = kv_full + (is_v ? kStages : 0), *empty = kv_empty + (is_v ? kStages : 0);
     uint8_t* ring = sKV + (is_v ? kStages * SM::kKV : 0);
-    const int rows = p.tma_rows, n_box = rows > 0 ? PX_BN / rows : 0;
-    auto whole = [&](int i) -> bool {
-      const int k0 = key0 + i * PX_BN;
-      return rows > 0 && k0 >= k_begin && k0 + PX_BN <= k_end;
-    };
-    // A lookup is a page and a place in it; they become a row only when the block's turn comes, so that nothing waits for
-    // the page table meanwhile.  -1: zeros, -2: no such page.
-    struct Spot { int page, in_page; };
-    auto spot_of = [&](int key) -> Spot {
-      if (key < k_begin || key >= k_end) return {-1, -1};
-      const int pi = p.block_shift >= 0 ? key >> p.block_shift : key / p.block_size;
-      return {__ldg(table + pi), key - pi * p.block_size};
-    };
     auto row_of = [&](Spot s) -> int {
       return s.in_page < 0 ? -1 : s.page < 0 || s.page >= p.num_blocks ? -2 : s.page * p.block_size + s.in_page;
     };
-    Spot next[2];
-    auto look_up = [&](int i) {                                  // this lane's box, or its two keys, of block i
-      next[0] = next[1] = {-1, -1};
-      if (i >= n_blk) return;
-      const int k0 = key0 + i * PX_BN;
-      if (whole(i)) {
-        if (lane < n_box) next[0] = spot_of(k0 + lane * rows);
-      } else {
-        next[0] = spot_of(k0 + lane);
-        next[1] = spot_of(k0 + 32 + lane);
-      }
-    };
-    look_up(0);
     bool bad = false;
     int told = 0, st = 0;                                        // blocks announced so far; stage
     uint32_t ph = 1;
@@ -579,7 +636,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
         mma_commit(&kv_empty[k_st]);
         if (++k_st == kStages) { k_st = 0; k_ph ^= 1; }
       };
-      bool good = n_blk > 0 && wait_for(&kv_full[0], 0, 1031, 0);
+      bool good = n_blk > 0 && wait_for(q_full, 0, 1039, 0) && wait_for(&kv_full[0], 0, 1031, 0);
       if (good) { tc_fence_after_sync(); issue_s(0); }
       for (int i = 0; good && i < n_blk; ++i) {
         const bool more = i + 1 < n_blk;
@@ -713,18 +770,16 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
   }
 
   // ---------------------------------------------------------------- results
-  const bool direct = p.splits == 1 && p.part_mode == 0;
   float* sx = reinterpret_cast<float*>(sKV);                     // [PX_BM][D], 16-byte pieces swizzled by row
   float* s_ml = sx + PX_BM * D;                                  // [PX_BM][2]
-  if (!direct) __syncthreads();                                  // every MMA of the CTA is done: the stages are free
+  if (!kDirect) __syncthreads();                                  // every MMA of the CTA is done: the stages are free
   if (softmax_warp) {
     const uint32_t tmem_o = tmem_base + kTmemO + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float f = 1.f;
     __nv_bfloat16* orow = nullptr;
-    if (direct && my_row < n_valid) {
+    if (kDirect && my_row < n_valid) {
       const int rr = row0 + my_row, tok = rr / g, h = hk * g + rr - tok * g;
-      const float sk = px_sink(p, h), mm = fmaxf(m, sk);
-      f = l != 0.f ? px_exp2(m - mm) / (l * px_exp2(m - mm) + px_exp2(sk - mm)) : 0.f;
+      f = px_factor(m, l, px_sink(p, h));
       orow = p.out + (static_cast<long long>(start + tok) * p.hq + h) * D;
     }
 #pragma unroll 1
@@ -737,7 +792,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 #pragma unroll
         for (int t = 0; t < 32; ++t) o[t] = 0u;
       }
-      if (direct) {
+      if (kDirect) {
         if (my_row < n_valid) {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
@@ -757,7 +812,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
               make_uint4(o[4 * t], o[4 * t + 1], o[4 * t + 2], o[4 * t + 3]);
       }
     }
-    if (!direct && my_row < n_valid) reinterpret_cast<float2*>(s_ml)[my_row] = make_float2(m, l);
+    if (!kDirect && my_row < n_valid) reinterpret_cast<float2*>(s_ml)[my_row] = make_float2(m, l);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -765,9 +820,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, SM::kTmemCols);
   }
-  if (direct) return;
-
-  px_join<D, kThreads>(p, sx, s_ml, start, row0, n_valid, hk, unit);
+  if constexpr (!kDirect) px_join<D, kThreads>(p, sx, s_ml, reinterpret_cast<float*>(sQ), start, row0, n_valid, hk, unit);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -790,7 +843,7 @@ struct PxFew {
   static constexpr int kKV = kTile * D * 2;
   static constexpr int kRows = 8 * NT;
   static constexpr int kOStride = D + 4;                   // floats; a warp leaves its O in its ring
-  static constexpr int kJoined = kRows * (D + 2) * 4;
+  static constexpr int kJoined = kRows * (D + 2 + kWarps) * 4;
   static constexpr int kRingMost = ((232448 / kCtas - 1024 - 128 - kJoined) / kWarps) & ~127;
   static constexpr int kStages = kRingMost / (2 * kKV) < 6 ? kRingMost / (2 * kKV) : 6;
   static constexpr int kRing = kStages * 2 * kKV;          // of a warp
@@ -825,6 +878,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   float* sx = reinterpret_cast<float*>(smem + F::kWarps * F::kRing);       // [rows][D], joined over the warps
   float* s_ml = sx + F::kRows * D;
+  float* s_w = s_ml + F::kRows * 2;                                        // [rows][warps] what each warp's part counts for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.splits * p.groups, unit = blockIdx.x, hk = blockIdx.y, g = p.group;
   const int b = p.flat ? 0 : p.sorted ? px_nth_longest<F::kThreads>(p, blockIdx.z, reinterpret_cast<int*>(smem)) : blockIdx.z;
@@ -837,7 +891,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
     return;
   }
   if (p.part_mode == 1) px_launch_dependents();
-  const int* table = p.block_tables + (p.flat ? px_owner(p) : b) * p.bt_stride;
+  const int* table = p.block_tables + (p.flat ? px_owner(p, lane) : b) * p.bt_stride;
 
   // keys of the list, and the bounds inside which no row needs a mask
   int k_begin, k_end, w_lo, w_hi;
@@ -882,6 +936,9 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   int ahead[kStages];
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ahead[i] = look_up(i);       // all the first tiles at once
+  const bool direct = p.splits == 1 && p.part_mode == 0;         // nothing to join but the warps
+  const int my_tok = px_div(threadIdx.x, inv_g);                 // thread r has the sink of row r ready for the end
+  const float my_sink = direct && threadIdx.x < n_valid ? px_sink(p, hk * g + threadIdx.x - my_tok * g) : -INFINITY;
   // Q^T as B operands: column = row of the list, k = dims
   uint32_t qf[KS][NT][2];
 #pragma unroll
@@ -1045,87 +1102,73 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
       }
     }
   __syncthreads();
-  const bool direct = p.splits == 1 && p.part_mode == 0;         // nothing to join but the warps
-  for (int i = threadIdx.x; i < n_valid * (D / 8); i += F::kThreads) {
-    const int r = i / (D / 8), c = i % (D / 8), tok = px_div(r, inv_g), h = hk * g + r - tok * g;
-    const float sink = direct ? px_sink(p, h) : -INFINITY;
-    float mm = -1e30f;
+  if (const int r = threadIdx.x; r < n_valid) {
     float2 ml[F::kWarps];
+    float top = -1e30f, sum = 0.f, w[F::kWarps], f = 1.f;
 #pragma unroll
-    for (int w = 0; w < F::kWarps; ++w) {
-      ml[w] = *reinterpret_cast<const float2*>(smem + w * F::kRing + F::kRows * F::kOStride * 4 + r * 8);
-      if (ml[w].y != 0.f) mm = fmaxf(mm, ml[w].x);
+    for (int k = 0; k < F::kWarps; ++k) {
+      ml[k] = *reinterpret_cast<const float2*>(smem + k * F::kRing + F::kRows * F::kOStride * 4 + r * 8);
+      if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
     }
-    PxSum t;
-    t.start(fmaxf(mm, sink));
 #pragma unroll
-    for (int w = 0; w < F::kWarps; ++w) {
-      const float4* src = reinterpret_cast<const float4*>(smem + w * F::kRing + (r * F::kOStride + c * 8) * 4);
-      if (ml[w].y != 0.f) t.add(ml[w], src[0], src[1]);
+    for (int k = 0; k < F::kWarps; ++k) {
+      w[k] = ml[k].y != 0.f ? px_exp2(ml[k].x - top) : 0.f;
+      sum += w[k] * ml[k].y;
     }
-    if (direct) {
-      t.store(p.out + (static_cast<long long>(start + tok) * p.hq + h) * D + c * 8, sink);
-      continue;
-    }
-    reinterpret_cast<float4*>(sx + r * D)[(2 * c) ^ (r & 7)] = make_float4(t.acc[0], t.acc[1], t.acc[2], t.acc[3]);
-    reinterpret_cast<float4*>(sx + r * D)[(2 * c + 1) ^ (r & 7)] = make_float4(t.acc[4], t.acc[5], t.acc[6], t.acc[7]);
-    if (c == 0) reinterpret_cast<float2*>(s_ml)[r] = make_float2(mm, t.sum);
+    if (direct) f = px_factor(top, sum, my_sink);
+    else reinterpret_cast<float2*>(s_ml)[r] = make_float2(top, sum);
+#pragma unroll
+    for (int k = 0; k < F::kWarps; ++k) s_w[r * F::kWarps + k] = w[k] * f;
+  }
+  __syncthreads();
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n_valid * (D / 4); i += F::kThreads) {
+    const int r = i / (D / 4), c = i % (D / 4), tok = px_div(r, inv_g), h = hk * g + r - tok * g;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < F::kWarps; ++k)
+      px_axpy(acc, s_w[r * F::kWarps + k], *reinterpret_cast<const float4*>(smem + k * F::kRing + (r * F::kOStride + c * 4) * 4));
+    if (direct) px_store(p.out + (static_cast<long long>(start + tok) * p.hq + h) * D + c * 4, acc, 1.f);
+    else reinterpret_cast<float4*>(sx + r * D)[c ^ (r & 7)] = acc;
   }
   if (direct) return;
-  px_join<D, F::kThreads>(p, sx, s_ml, start, 0, n_valid, hk, unit);
+  px_join<D, F::kThreads>(p, sx, s_ml, reinterpret_cast<float*>(smem), start, 0, n_valid, hk, unit);
 }
 
-// Joins the sets of the launches that split the keys over several clusters: D / 8 threads for the columns of a row, kParts of
+// Joins the sets of the launches that split the keys over several clusters: D / 4 threads for the columns of a row, kParts of
 // such groups for its sets (1 for a few sets and many rows; a CTA a row for the dozens of sets of a single long context,
 // which took 32 us one after the other).
 template <int D, int kParts>
-__global__ void __launch_bounds__(128) k_paged_join(const ExtendParams p) {
-  constexpr int kCols = D / 8, kRows = 128 / (kCols * kParts);
-  static_assert(kParts == 1 || kRows == 1, "the parts of a row are its CTA");
-  __shared__ float s_max[4], s_acc[kParts > 1 ? kParts : 1][kCols][9];
-  const int b = blockIdx.y, c = threadIdx.x % kCols, part = kParts > 1 ? threadIdx.x / kCols : 0;
-  const int i = static_cast<int>(blockIdx.x) * kRows + (kParts > 1 ? 0 : threadIdx.x / kCols), h = i % p.hq, tok = i / p.hq;
+struct PxJoin {
+  static constexpr int kCols = D / 4, kThreads = kParts > 1 ? kCols * kParts : 128, kRows = kThreads / (kCols * kParts);
+};
+template <int D, int kParts>
+__global__ void __launch_bounds__(PxJoin<D, kParts>::kThreads) k_paged_join(const ExtendParams p) {
+  using J = PxJoin<D, kParts>;
+  const int b = blockIdx.y, c = threadIdx.x % J::kCols, part = kParts > 1 ? threadIdx.x / J::kCols : 0;
+  const int i = static_cast<int>(blockIdx.x) * J::kRows + (kParts > 1 ? 0 : threadIdx.x / J::kCols), h = i % p.hq, tok = i / p.hq;
   int start, n, ctx;
   px_list(p, b, false, start, n, ctx);
   px_wait_prior_grid();
   if (tok >= n) return;                                          // the whole CTA where it has one row
   const long long row = static_cast<long long>(start + tok) * p.hq + h;
-  const float sink = px_sink(p, h);
-  float mm = -1e30f;
-#pragma unroll 4
-  for (int s = kParts > 1 ? threadIdx.x : 0; s < p.n_sets; s += kParts > 1 ? 128 : 1) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-    if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
-  }
-  if constexpr (kParts > 1) {
-    mm = warp_max(mm);
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mm;
-    __syncthreads();
-    mm = fmaxf(px_max3(s_max[0], s_max[1], s_max[2]), s_max[3]);
-  }
   PxSum t;
-  t.start(fmaxf(mm, sink));
-#pragma unroll 4
-  for (int s = part; s < p.n_sets; s += kParts) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + s * p.set_rows + row);
-    const float4* o = reinterpret_cast<const float4*>(p.part_o + (s * p.set_rows + row) * D) + 2 * c;
-    const float4 x = __ldcg(o), y = __ldcg(o + 1);
-    if (ml.y != 0.f) t.add(ml, x, y);
-  }
+  t.start(-1e30f);
+  t.add_sets<D, (kParts > 1 ? 4 : 8)>(p, row, c, part, kParts);
   if constexpr (kParts > 1) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s_acc[part][c][e] = t.acc[e];
-    s_acc[part][c][8] = t.sum;
+    __shared__ float4 s_acc[kParts][J::kCols];
+    __shared__ float2 s_ml[kParts];
+    s_acc[part][c] = t.acc;
+    if (c == 0) s_ml[part] = make_float2(t.top, t.sum);
     __syncthreads();
     if (part > 0) return;
+    t.start(-1e30f);
 #pragma unroll
-    for (int q = 1; q < kParts; ++q) {
+    for (int q = 0; q < kParts; ++q) t.top = fmaxf(t.top, s_ml[q].x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t.acc[e] += s_acc[q][c][e];
-      t.sum += s_acc[q][c][8];
-    }
+    for (int q = 0; q < kParts; ++q) t.add(s_ml[q], s_acc[q][c]);
   }
-  t.store(p.out + row * D + c * 8, sink);
+  t.store(p.out + row * D + c * 4, px_sink(p, h));
 }
 
 // How a call is cut: which kernel, tiles a list, CTAs the keys of a tile are split over.
@@ -1218,7 +1261,15 @@ static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
                    make_tensor_map_2d(&tv, p.v_cache, kTmaBf16, inner, rows, inner * 2, 64, a.tma_rows, kTmaSwizzle128);
     if (rc != 0) a.tma_rows = 0;                                 // then every block is copied by hand
   }
-  return px_launch<k_paged_extend<D>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st, tk, tv);
+  return p.splits == 1 && p.part_mode == 0
+             ? px_launch<k_paged_extend<D, true>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, false, st, tk, tv)
+             : px_launch<k_paged_extend<D, false>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st, tk, tv);
+}
+
+template <int D, int kParts>
+static cudaError_t px_join_launch(const ExtendParams& p, long long rows, int B, cudaStream_t st) {
+  using J = PxJoin<D, kParts>;
+  return px_launch<k_paged_join<D, kParts>>(p, dim3(static_cast<unsigned>((rows + J::kRows - 1) / J::kRows), B), J::kThreads, 0, true, st);
 }
 
 static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream_t st) {
@@ -1342,13 +1393,7 @@ extern "C" int nmoe_paged_extend(const void* q, long long q_stride, const void* 
   p.splits = 1;
   const long long rows = static_cast<long long>(max_q_len) * Hq;
   cudaError_t e;
-  if (p.n_sets > 8) {
-    const dim3 grid(static_cast<unsigned>(rows), B);
-    e = D == 64 ? px_launch<k_paged_join<64, 16>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128, 8>>(p, grid, 128, 0, true, st);
-  } else {
-    const int each = 128 / (D / 8);
-    const dim3 grid(static_cast<unsigned>((rows + each - 1) / each), B);
-    e = D == 64 ? px_launch<k_paged_join<64, 1>>(p, grid, 128, 0, true, st) : px_launch<k_paged_join<128, 1>>(p, grid, 128, 0, true, st);
-  }
+  if (p.n_sets > 8) e = D == 64 ? px_join_launch<64, 16>(p, rows, B, st) : px_join_launch<128, 8>(p, rows, B, st);
+  else e = D == 64 ? px_join_launch<64, 1>(p, rows, B, st) : px_join_launch<128, 1>(p, rows, B, st);
   return e == cudaSuccess ? 0 : static_cast<int>(e);
 }
