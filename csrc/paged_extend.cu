@@ -375,11 +375,11 @@ NMOE_DEVICE void px_join(const ExtendParams& p, const float* sx, const float* s_
 // Layout of shared memory.  The exchange of partial results reuses the stages (O as fp32, 16-byte pieces swizzled by row).
 template <int D>
 struct PxSmem {
-  static constexpr int kCtas = D == 64 ? 3 : 2;            // of an SM: 66 KB and 100 KB of shared memory, 128 and 256 columns of tensor memory
+  static constexpr int kCtas = D == 64 ? 4 : 2;            // of an SM: all of tensor memory, 128 and 256 columns each
   static constexpr int kBufs = D == 64 ? 1 : 2;            // S buffers of 64 columns
-  static constexpr int kLoaders = 64;                      // threads
-  static constexpr int kThreads = 4 * 32 + 32 + kLoaders;
-  static constexpr int kStages = D == 64 ? 3 : 2;          // of K and of V
+  static constexpr int kLoaders = D == 64 ? 1 : 2;         // warps; with one more four CTAs have no registers
+  static constexpr int kThreads = 4 * 32 + 32 + 32 * kLoaders;
+  static constexpr int kStages = 2;                        // of K and of V
   static constexpr int kQ = PX_BM * D * 2;
   static constexpr int kKV = PX_BN * D * 2;                // a stage of one of them
   static constexpr int kRing = 2 * kStages * kKV;
@@ -540,13 +540,10 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     // once they have landed, normally kLag blocks after they were asked for, all at once when the ring is full, since what
     // would make room may be waiting for one of them.
     constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
-    const bool is_v = warp == kMmaWarp + 2;
+    // K (0) and V (1) by a warp each, or both by one
+    const int kv0 = SM::kLoaders == 2 ? warp - kMmaWarp - 1 : 0, kv1 = SM::kLoaders == 2 ? kv0 + 1 : 2;
     const int c = lane % kChunks, rp = lane / kChunks;
-    const long long row_bytes = static_cast<long long>(p.hkv) * D * 2;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache) + (static_cast<long long>(hk) * D + c * 8) * 2;
-    const CUtensorMap* map = is_v ? &tm_v : &tm_k;
-    uint64_t *full = kv_full + (is_v ? kStages : 0), *empty = kv_empty + (is_v ? kStages : 0);
-    uint8_t* ring = sKV + (is_v ? kStages * SM::kKV : 0);
+    const long long row_bytes = static_cast<long long>(p.hkv) * D * 2, piece = (static_cast<long long>(hk) * D + c * 8) * 2;
     auto row_of = [&](Spot s) -> int {
       return s.in_page < 0 ? -1 : s.page < 0 || s.page >= p.num_blocks ? -2 : s.page * p.block_size + s.in_page;
     };
@@ -557,16 +554,11 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0)
-        for (int t = told; t < upto; ++t) mbar_arrive(&full[t % kStages]);
+        for (int t = told; t < upto; ++t)
+          for (int kv = kv0; kv < kv1; ++kv) mbar_arrive(&kv_full[kv * kStages + t % kStages]);
       told = upto;
     };
     for (int i = 0; i < n_blk && ok; ++i) {
-      if (!__all_sync(0xffffffffu, px_test(&empty[st], ph))) {
-        if (told < i) { px_cp_wait<0>(); announce(i); }
-        ok = px_wait(&empty[st], ph, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, is_v); *abort_flag = 1; break; }
-      }
       int mine[2] = {row_of(next[0]), row_of(next[1])};
       bool boxes = whole(i);
       if (boxes && __any_sync(0xffffffffu, mine[0] == -2)) {     // a bad page among boxes: its keys become zeros
@@ -576,31 +568,46 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
       }
       bad = bad || mine[0] == -2 || mine[1] == -2;
       look_up(i + 1);
-      uint8_t* slot = ring + st * SM::kKV;
-      if (boxes) {
-        if (told < i) { px_cp_wait<0>(); announce(i); }
-        int row[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) row[x] = __shfl_sync(0xffffffffu, mine[0], x);
-        if (elect_one()) {
-          mbar_expect_tx(&full[st], SM::kKV);
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            if (x < n_box) {
-#pragma unroll
-              for (int d = 0; d < D / 64; ++d) tma_load_2d(slot + d * (PX_BN * 128) + x * rows * 128, map, &full[st], hk * D + d * 64, row[x]);
-            }
+      if (boxes && told < i) { px_cp_wait<0>(); announce(i); }
+      for (int kv = kv0; kv < kv1; ++kv) {
+        uint64_t *full = &kv_full[kv * kStages + st], *empty = &kv_empty[kv * kStages + st];
+        if (!__all_sync(0xffffffffu, px_test(empty, ph))) {
+          if (told < i) { px_cp_wait<0>(); announce(i); }
+          ok = px_wait(empty, ph, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) { if (lane == 0) report_status(p.status, kStatusWaitTimeout, 1030, i, kv); *abort_flag = 1; break; }
         }
-        __syncwarp();
+        uint8_t* slot = sKV + (kv * kStages + st) * SM::kKV;
+        if (boxes) {
+          const CUtensorMap* map = kv ? &tm_v : &tm_k;
+          int row[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) row[x] = __shfl_sync(0xffffffffu, mine[0], x);
+          if (elect_one()) {
+            mbar_expect_tx(full, SM::kKV);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (x < n_box) {
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d) tma_load_2d(slot + d * (PX_BN * 128) + x * rows * 128, map, full, hk * D + d * 64, row[x]);
+              }
+          }
+          __syncwarp();
+        } else {
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(kv ? p.v_cache : p.k_cache) + piece;
+          const uint32_t dst = smem_u32(slot);
+#pragma unroll
+          for (int s = 0; s < PX_BN / kRowsPass; ++s) {
+            const int r = s * kRowsPass + rp;
+            const int row = __shfl_sync(0xffffffffu, mine[s >= PX_BN / kRowsPass / 2], r & 31);
+            px_cp16(dst + (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + max(row, 0) * row_bytes, row >= 0 ? 16u : 0u);
+          }
+        }
+      }
+      if (!ok) break;
+      if (boxes) {
         told = i + 1;
       } else {
-        const uint32_t dst = smem_u32(slot);
-#pragma unroll
-        for (int s = 0; s < PX_BN / kRowsPass; ++s) {
-          const int r = s * kRowsPass + rp;
-          const int row = __shfl_sync(0xffffffffu, mine[s >= PX_BN / kRowsPass / 2], r & 31);
-          px_cp16(dst + (c >> 3) * (PX_BN * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + max(row, 0) * row_bytes, row >= 0 ? 16u : 0u);
-        }
         px_cp_commit();
         if (i - kLag >= told) { px_cp_wait<kLag>(); announce(i - kLag + 1); }
       }
@@ -686,15 +693,21 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
       auto half = [&](int hf) {
         tmem_ld_32x32b_x32(s_addr + hf * 32, r);
         tmem_ld_wait();
-        if (edge) {
+      };
+      if (edge) {                                                            // masked scores go back, so that what follows stays short
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          half(hf);
           const int from = lo - k0 - hf * 32, to = hi - k0 - hf * 32;
 #pragma unroll
           for (int t = 0; t < 32; ++t)
             if (t < from || t >= to) r[t] = 0xff800000u;                     // -inf
+          tmem_st_32x32b_x32(s_addr + hf * 32, r);
         }
-      };
+        tmem_st_wait();
+      }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};           // four chains: one would be 32 latencies long
-#pragma unroll
+#pragma unroll 1
       for (int hf = 0; hf < 2; ++hf) {
         half(hf);
 #pragma unroll
@@ -737,16 +750,12 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
           pk[t >> 1] = pack_bf16x2(p0, p1);
         }
       };
-      {
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
         uint32_t pk[16];
+        half(hf);
         exps(pk);
-        half(0);                                                             // before P goes over it
-        px_tmem_st_x16(s_addr + 16, pk);
-      }
-      {
-        uint32_t pk[16];
-        exps(pk);
-        px_tmem_st_x16(s_addr, pk);
+        px_tmem_st_x16(s_addr + hf * 16, pk);
       }
       float sa, sb;
       px_unpack(px_add2(rs2[0], rs2[1]), sa, sb);
@@ -1194,7 +1203,7 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
     least = 128;
   } else {
     q.tiles = (rows + PX_BM - 1) / PX_BM;
-    slots = D == 64 ? 3 * 148 : 2 * 148;
+    slots = D == 64 ? 4 * 148 : 2 * 148;
     least = 4 * PX_BN;
   }
   q.slots = slots;
