@@ -6,17 +6,20 @@
 // head of the group, 128 rows to a tile, so every K/V block is read once for all of them.  Each row carries its own
 // bounds [lo, hi) of visible keys (causal end, window, shared part); a block that lies inside all of them needs no mask.
 //
-// Many rows (k_paged_extend), a tile a CTA, 64 keys at a time.  Two loader warps, one for K and one for V, bring a block's
+// Many rows (k_paged_extend), a tile a CTA, 64 keys at a time.  A loader warp (D = 128: one for K, one for V) brings a block's
 // rows from their pages, by TMA where whole boxes of keys lie in a page, else with cp.async (16 bytes a lane, any page
-// size); both leave zeros where the CTA has no keys, so that what lies there cannot reach the products.  One thread issues
-// the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back to tensor memory as the A operand
-// of P V.  The maximum is raised only when it grows by more than 2^8; the stale one is exact after the final division.  P is
-// rounded to bf16 because the tensor core multiplies it with bf16 values; the sum l takes the unrounded p.
-// A block is a chain of latencies (S 430 cycles, softmax 1050 alone and 1400 in company, P V and the way to the next S 400)
-// in which no unit is busy, so an SM is filled with chains: three CTAs for D = 64, whose S has a single buffer to fit tensor
-// memory, two for D = 128.  8 prompts of 200..1750 new tokens behind 1300..3500 cached ones, 64/8 heads of 64: 715 us, 560
-// TFLOP/s (issue slots half full, special function unit half, tensor cores a quarter).  What did not help: part of the
-// exponentials by polynomial, two warps for 32 rows, two tiles a CTA (788 us), turns between warps, polling barriers.
+// size; 8 prompts: 725 us by TMA where 770 by hand); both leave zeros where the CTA has no keys, so that what lies there cannot
+// reach the products.  One thread issues the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back
+// to tensor memory as the A operand of P V.  The maximum is raised only when it grows by more than 2^8; the stale one is exact
+// after the final division.  P is rounded to bf16 because the tensor core multiplies it with bf16 values; the sum l takes the
+// unrounded p.
+// A block is a chain of latencies (S, softmax, P V and the way to the next S) in which no unit is busy, so an SM is filled with
+// chains: four CTAs for D = 64, whose S has a single buffer to fit tensor memory, two for D = 128.  Code that is run once or
+// seldom stays rolled: with the softmax of 64 keys in one piece, 55 % of the instruction cache's request rate was the bound and
+// the fourth CTA gained nothing (699 us; loops over 32 keys: 625; loaders and start of a CTA rolled too: 597; three CTAs: 700).
+// 8 prompts of 200..1750 new tokens behind 1300..3500 cached ones, 64/8 heads of 64: 597 us, 670 TFLOP/s (issue slots 56 %,
+// special function unit 62 %, tensor cores 31 %).  What did not help: part of the exponentials by polynomial, two warps for 32
+// rows, two tiles a CTA, 16 keys at a time (631 us), keeping half of the scores between maximum and exponentials (679 us).
 //
 // Few rows (k_paged_few, below): decode steps and drafts, bound by the bytes of K and V.
 //
@@ -514,7 +517,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
     // rows of Q, 128-byte swizzle, K-major; rows that do not exist are zero
     const int tok0 = row0 / g, rem0 = row0 - tok0 * g, c = threadIdx.x % (D / 8);
     const uint32_t dst = smem_u32(sQ) + (c >> 3) * (PX_BM * 128);
-#pragma unroll
+#pragma unroll 2
     for (int r = threadIdx.x / (D / 8); r < PX_BM; r += 128 / (D / 8)) {
       const bool in = r < n_valid;
       const int dt = in ? px_div(rem0 + r, inv_g) : 0, h = hk * g + (in ? rem0 + r - dt * g : 0);
@@ -533,9 +536,9 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
   bool ok = true;
   float m = -1e30f, l = 0.f;
   if (warp > kMmaWarp) {
-    // ------------------------------------------------------------ loaders: one warp for K, one for V
-    // Where pages hold whole boxes of 8 to 64 keys, a block without keys outside [k_begin, k_end) comes by TMA, one box after
-    // the other from one lane.  Other blocks are copied by hand: every lane looks up two of the 64 keys (a block ahead, so
+    // ------------------------------------------------------------ loaders
+    // Where pages hold whole boxes of 8 to 64 keys, a block without keys outside [k_begin, k_end) comes by TMA, a box a
+    // lane.  Other blocks are copied by hand: every lane looks up two of the 64 keys (a block ahead, so
     // that the page table's latency is covered) and the warp shares the rows by shuffle; such copies are announced in order
     // once they have landed, normally kLag blocks after they were asked for, all at once when the ring is full, since what
     // would make room may be waiting for one of them.
@@ -580,23 +583,17 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
         uint8_t* slot = sKV + (kv * kStages + st) * SM::kKV;
         if (boxes) {
           const CUtensorMap* map = kv ? &tm_v : &tm_k;
-          int row[8];
+          if (lane == 0) mbar_expect_tx(full, SM::kKV);
+          __syncwarp();
+          if (lane < n_box) {                                    // a box a lane
 #pragma unroll
-          for (int x = 0; x < 8; ++x) row[x] = __shfl_sync(0xffffffffu, mine[0], x);
-          if (elect_one()) {
-            mbar_expect_tx(full, SM::kKV);
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              if (x < n_box) {
-#pragma unroll
-                for (int d = 0; d < D / 64; ++d) tma_load_2d(slot + d * (PX_BN * 128) + x * rows * 128, map, full, hk * D + d * 64, row[x]);
-              }
+            for (int d = 0; d < D / 64; ++d) tma_load_2d(slot + d * (PX_BN * 128) + lane * rows * 128, map, full, hk * D + d * 64, mine[0]);
           }
           __syncwarp();
         } else {
           const uint8_t* src = reinterpret_cast<const uint8_t*>(kv ? p.v_cache : p.k_cache) + piece;
           const uint32_t dst = smem_u32(slot);
-#pragma unroll
+#pragma unroll 4
           for (int s = 0; s < PX_BN / kRowsPass; ++s) {
             const int r = s * kRowsPass + rp;
             const int row = __shfl_sync(0xffffffffu, mine[s >= PX_BN / kRowsPass / 2], r & 31);
@@ -840,7 +837,7 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 // barrier is needed.  Each of four warps streams its own tiles of 16 or 32 keys through a ring of its own,
 // with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
 // movmatrix; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
-// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 64 us, 4.1 TB/s (the stream itself runs at 5.5; the
+// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 62 us, 4.2 TB/s (the stream itself runs at 5.5; the
 // rest is 5 us of start-up latencies a CTA and the last wave).  Equal shares of all keys for 296 CTAs, with pieces joined
 // afterwards, took 95 us: a start-up for every piece, and heads of one page no longer read together.
 template <int D, int NT>
