@@ -1187,12 +1187,14 @@ struct PxPlan {
 // `lists` row lists of up to `rows` rows that see at most `keys` keys each; groups only where partial sets may be written.
 static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys, bool may_group) {
   PxPlan q;
-  // 64 drafted steps of 5 tokens, 40 rows, D = 64: 72 us against 84 in the kernel for many rows; 32 rows of D = 128 over 99k
-  // keys: 68 against 63
+  // 64 sequences over 300..4096 keys, D = 64: 40 rows 74 us against 89 in the kernel for many rows, 24 rows 59 against 77 (one
+  // context of 100000 keys, 40 rows: 52 against 47); D = 128 over 99k keys: 16 rows 41 against 41, 32 rows 68 against 63
   const int few_most = D == 64 ? 40 : 16;
   q.nt = 0;
   q.tiles = 1;
-  long long slots, least;                  // CTAs the GPU holds at once; keys that make a split worth while
+  // CTAs the GPU holds at once; keys that make a split worth while (few rows, 3 sequences of 900..1000 keys: 8.0 us, with half of
+  // that 9.2, with twice as many 9.7; many rows, 4 sequences of 2000..3000 keys: 18.3 us, 24.2 and 20.3)
+  long long slots, least;
   if (rows <= few_most) {
     const int t = static_cast<int>((rows + 7) / 8);
     q.nt = t == 4 ? 5 : t;
@@ -1205,6 +1207,8 @@ static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys,
   }
   q.slots = slots;
   const long long base = q.tiles * lists * hkv;
+  // Rounded down: a second wave of a few CTAs costs as much as a first one.  (32 sequences of 3000 keys each, 16 rows: 41 us,
+  // rounded up 55; of 1000..8000 keys 82 and 64, but the lengths are not known here.)
   long long units = slots / (base > slots ? slots : base);
   const long long worth = keys / least;
   if (units > worth) units = worth;

@@ -256,6 +256,8 @@ extern "C" int nmoe_verify_draft(const float* target, long long target_stride, c
   p.target_stride = target_stride; p.draft_stride = draft_stride; p.n_rows = n_rows; p.vocab = vocab; p.tok64 = tok64;
   p.vec = (reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) % 16 == 0 &&
           (target_stride | draft_stride) % 4 == 0;
+  // As many CTAs a row as keep the batch within two an SM: one sequence 12.4 us with 16 of them, 14.4 with 8, 18.5 with 4, 43 with
+  // one; 64 sequences 30 us with 4, 38 with 8, 54 with one.
   int cluster = 1;
   while (cluster < kVerifyMaxCluster && n_seqs * cluster * 2 <= 296 && vocab >= cluster * 2 * 4096) cluster *= 2;
   cudaLaunchConfig_t cfg = {};

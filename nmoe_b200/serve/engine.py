@@ -14,7 +14,7 @@ sequence by one token.  ``generate`` wraps the loop for greedy / top-k sampling;
 runs prompts through the first layers only (the probe / judge taps of the curation stack).
 
 Two things shorten decoding.  Blocks that every running sequence has in common (a grading rubric, a
-few-shot header) are attended to once per step for the whole batch.  And with ``draft_tokens`` > 0
+few-shot header) are attended to once per step for the whole batch (steps without drafts).  And with ``draft_tokens`` > 0
 ``generate`` lets each sequence propose that many tokens per step by looking its last tokens up in
 its own text (answers that quote their prompt, structured output); one pass scores them all and
 those that fit are kept.  Greedy output is what it would be without drafts, sampled output has the
@@ -38,7 +38,8 @@ from .kv import BlockPool, SeqStatus, Sequence
 from .model import CacheView, Transformer
 
 
-# A shared prefix of fewer tokens is left to the per-sequence decode kernel.
+# A shared prefix of fewer tokens is left to the per-sequence decode kernel.  With 64 shared tokens two sequences of 64 more take
+# 9.3 us against 13.0; with 32 shared ones two take 9.5 against 10.8 and eight 10.9 against 10.9.
 MIN_SHARED_TOKENS = 64
 
 
