@@ -17,8 +17,8 @@ Two things shorten decoding.  Blocks that every running sequence has in common (
 few-shot header) are attended to once per step for the whole batch (steps without drafts).  And with ``draft_tokens`` > 0
 ``generate`` lets each sequence propose that many tokens per step by looking its last tokens up in
 its own text (answers that quote their prompt, structured output); one pass scores them all and
-those that fit are kept.  Greedy output is what it would be without drafts, sampled output has the
-same distribution.
+those that fit are kept.  Greedy output is what it would be without drafts (on the GPU as far as the
+rounding of two kernels leaves near-ties alone), sampled output has the same distribution.
 
 Behavioural counterpart: ``BatchedGenerator`` (nmoe/data/model.py:650-790).  Differences: prefix
 blocks found in the cache are really attended to during prefill, the host-side batch assembly is

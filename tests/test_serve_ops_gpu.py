@@ -156,6 +156,24 @@ def test_paged_extend_page_sizes(bs, D, hq, hkv, window):
   within(out, want, bound)
 
 
+@pytest.mark.parametrize("bs", [2, 4, 6, 12, 20, 24, 36, 80])
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 0), (64, 150)])
+def test_paged_extend_pages_of_small_boxes(bs, D, window):
+  """Pages of an even number of keys that is no power of two, or a small one: many rows, contexts that end inside a page."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(bs)
+  lens, ctx = [100, 1, 37], [501, 777, 65]
+  k, v, tables = paged(ctx, bs, 2, D, g)
+  for b in range(3):
+    for t in range(ctx[b], (ctx[b] + bs - 1) // bs * bs):
+      k[tables[b, t // bs].long(), t % bs] = float("nan")
+      v[tables[b, t // bs].long(), t % bs] = float("nan")
+  q = torch.randn(138, 8, D, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, [0, 100, 101], lens, None, D ** -0.5, window)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, 100, 101]), i32(lens), None, D ** -0.5, window)
+  within(out, want, bound)
+
+
 def test_paged_extend_strided_operands():
   from nmoe_b200.serve import ops as S
   g = torch.Generator().manual_seed(8)
