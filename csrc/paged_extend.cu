@@ -11,8 +11,14 @@
 // size; 8 prompts: 597 us by TMA where 982 by hand); both leave zeros where the CTA has no keys, so that what lies there cannot
 // reach the products.  One thread issues the MMAs, four warps own 32 rows each: running maximum and sum in fp32, P as bf16 back
 // to tensor memory as the A operand of P V.  The maximum is raised only when it grows by more than 2^8; the stale one is exact
-// after the final division.  P is rounded to bf16 because the tensor core multiplies it with bf16 values; the sum l takes the
-// unrounded p.
+// after the final division.  The sum l takes the unrounded p.
+//
+// Roundings of P.  The tensor core multiplies it with bf16 values, so it has to be bf16 too.  Steps of a few tokens (the kernel for
+// few rows, lists of one tile, a shared prefix) take it in two parts, its bf16 value and the bf16 value of what that leaves, at
+// twice the products of P V: what comes out is rounded once, as paged_decode's results are (which has P in fp32), whichever kernel a
+// sequence's step happens to run on.  Error of the result relative to its norm 1.7e-3, with one part 2.4e-3.  Prompts of several
+// tiles take one part, as the dense attention of a prompt without a cached prefix does (8 prompts: 597 us, in two parts 795).
+//
 // A block is a chain of latencies (S, softmax, P V and the way to the next S) in which no unit is busy, so an SM is filled with
 // chains: four CTAs for D = 64, whose S has a single buffer to fit tensor memory, two for D = 128.  Code that is run once or
 // seldom stays rolled: with the softmax of 64 keys in one piece, 55 % of the instruction cache's request rate was the bound and
@@ -138,6 +144,12 @@ NMOE_DEVICE uint64_t px_add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+// two probabilities as bf16 values and, in a second pair, what these leave of them: together they hold 2^-16 of each
+NMOE_DEVICE void px_split(float a, float b, uint32_t& high, uint32_t& rest) {
+  high = pack_bf16x2(a, b);
+  const float2 h = unpack_bf16x2(high);
+  rest = pack_bf16x2(a - h.x, b - h.y);
 }
 NMOE_DEVICE void px_cp16(uint32_t dst, const void* src, uint32_t bytes) {      // bytes 0: the 16 bytes become zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -392,7 +404,7 @@ struct PxSmem {
   static constexpr uint32_t kTmemCols = kBufs * PX_BN + D;
 };
 
-template <int D, bool kDirect>
+template <int D, bool kDirect, bool kFine>
 __global__ void __launch_bounds__(PxSmem<D>::kThreads, PxSmem<D>::kCtas)
 k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using SM = PxSmem<D>;
@@ -653,8 +665,16 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
         const uint64_t va = v_desc + static_cast<uint64_t>(v_st * SM::kKV >> 4);
         const uint32_t a_t = tmem_base + (i % kBufs) * PX_BN;
 #pragma unroll
-        for (int j = 0; j < PX_BN / 16; ++j)
-          px_mma_ts(tmem_base + kTmemO, a_t + j * 8, va + ((j * 2048) >> 4), idesc_pv, (i | j) != 0 ? 1u : 0u);
+        for (int j = 0; j < PX_BN / 16; ++j) {
+          const uint64_t v16 = va + ((j * 2048) >> 4);
+          if constexpr (kFine) {                                 // 32 keys: 16 columns of P, 16 of what its rounding left
+            const uint32_t a16 = a_t + (j >> 1) * 32 + (j & 1) * 8;
+            px_mma_ts(tmem_base + kTmemO, a16, v16, idesc_pv, (i | j) != 0 ? 1u : 0u);
+            px_mma_ts(tmem_base + kTmemO, a16 + 16, v16, idesc_pv, 1u);
+          } else {
+            px_mma_ts(tmem_base + kTmemO, a_t + j * 8, v16, idesc_pv, (i | j) != 0 ? 1u : 0u);
+          }
+        }
         if (!more) mma_commit(o_full);
         else if (kBufs == 2) mma_commit(pv_done);
         // one buffer: S goes over P once P V has read it (the tensor core takes the products in order)
@@ -744,7 +764,8 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
           px_unpack(px_fma2(px_pack(__uint_as_float(r[t]), __uint_as_float(r[t + 1])), sc2, nm2), x0, x1);
           const float p0 = px_exp2(x0), p1 = px_exp2(x1);
           rs2[(t >> 1) & 1] = px_add2(rs2[(t >> 1) & 1], px_pack(p0, p1));
-          pk[t >> 1] = pack_bf16x2(p0, p1);
+          if constexpr (kFine) px_split(p0, p1, pk[t >> 1], r[t >> 1]);
+          else pk[t >> 1] = pack_bf16x2(p0, p1);
         }
       };
 #pragma unroll 1
@@ -752,7 +773,12 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
         uint32_t pk[16];
         half(hf);
         exps(pk);
-        px_tmem_st_x16(s_addr + hf * 16, pk);
+        if constexpr (kFine) {
+          px_tmem_st_x16(s_addr + hf * 32, pk);                  // over the scores that were just read
+          px_tmem_st_x16(s_addr + hf * 32 + 16, r);
+        } else {
+          px_tmem_st_x16(s_addr + hf * 16, pk);
+        }
       }
       float sa, sb;
       px_unpack(px_add2(rs2[0], rs2[1]), sa, sb);
@@ -836,9 +862,9 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 // its own share (a tcgen05 tile gives a whole row of 64 keys to one lane: 1350 cycles a block for one busy warp), and no
 // barrier is needed.  Each of four warps streams its own tiles of 16 or 32 keys through a ring of its own,
 // with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
-// movmatrix; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
-// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 62 us, 4.2 TB/s (the stream itself runs at 5.5; the
-// rest is 5 us of start-up latencies a CTA and the last wave).  Equal shares of all keys for 296 CTAs, with pieces joined
+// movmatrix, in its two parts; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
+// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 69 us, 3.7 TB/s (62 with P in one part, when the stream
+// itself ran at 5.5 TB/s; 73 with 40 rows for every list; the rest is 5 us of start-up latencies a CTA and the last wave).  Equal shares of all keys for 296 CTAs, with pieces joined
 // afterwards, took 95 us: a start-up for every piece, and heads of one page no longer read together.
 template <int D, int NT>
 struct PxFew {
@@ -875,28 +901,16 @@ NMOE_DEVICE void px_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const ExtendParams p) {
-  using F = PxFew<D, NT>;
+// one list, its rows in NT columns of 8; F: the layout of the kernel it runs in
+template <int D, int NT, typename F>
+NMOE_DEVICE void px_few_list(const ExtendParams& p, uint8_t* smem, int b, int start, int n, int ctx, int n_valid) {
   constexpr int kTile = F::kTile, kStages = F::kStages, MT = kTile / 16, KS = D / 16;
   const float inv_g = 1.f / static_cast<float>(p.group);
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   float* sx = reinterpret_cast<float*>(smem + F::kWarps * F::kRing);       // [rows][D], joined over the warps
   float* s_ml = sx + F::kRows * D;
   float* s_w = s_ml + F::kRows * 2;                                        // [rows][warps] what each warp's part counts for
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.splits * p.groups, unit = blockIdx.x, hk = blockIdx.y, g = p.group;
-  const int b = p.flat ? 0 : p.sorted ? px_nth_longest<F::kThreads>(p, blockIdx.z, reinterpret_cast<int*>(smem)) : blockIdx.z;
-  int start, n, ctx;
-  px_list(p, b, unit == 0 && hk == 0 && threadIdx.x == 0, start, n, ctx);
-  const int n_valid = min(F::kRows, n * g);                      // the host launches this kernel only where all rows fit
-  if (n_valid <= 0) {                                            // uniform over the cluster
-    if (p.part_mode == 1) px_launch_dependents();
-    if (p.part_mode == 2) px_wait_prior_grid();
-    return;
-  }
-  if (p.part_mode == 1) px_launch_dependents();
   const int* table = p.block_tables + (p.flat ? px_owner(p, lane) : b) * p.bt_stride;
 
   // keys of the list, and the bounds inside which no row needs a mask
@@ -1063,7 +1077,7 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      uint32_t pf[NT][2];
+      uint32_t pf[NT][2], pr[NT][2];                             // P as a bf16 value and what it leaves, both as operands
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float e4[4];
@@ -1071,8 +1085,13 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
         for (int e = 0; e < 4; ++e) e4[e] = px_exp2(fmaf(s[mt][nt][e], p.scale_log2, -m[nt][e & 1]));
         l[nt][0] += e4[0] + e4[2];
         l[nt][1] += e4[1] + e4[3];
-        pf[nt][0] = px_transpose(pack_bf16x2(e4[0], e4[1]));
-        pf[nt][1] = px_transpose(pack_bf16x2(e4[2], e4[3]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t high, rest;
+          px_split(e4[2 * h], e4[2 * h + 1], high, rest);
+          pf[nt][h] = px_transpose(high);
+          pr[nt][h] = px_transpose(rest);
+        }
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -1081,6 +1100,8 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
         px_ldm_t(vs_addr + r * (D * 2) + (((ks * 2 + vc) ^ (r & 7)) << 4), a);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) px_mma(o[ks][nt], a, pf[nt][0], pf[nt][1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) px_mma(o[ks][nt], a, pr[nt][0], pr[nt][1]);
       }
     }
     __syncwarp();                                                // the stage may be filled again
@@ -1141,6 +1162,27 @@ __global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const Ex
   px_join<D, F::kThreads>(p, sx, s_ml, reinterpret_cast<float*>(smem), start, 0, n_valid, hk, unit);
 }
 
+template <int D, int NT>
+__global__ void __launch_bounds__(128, PxFew<D, NT>::kCtas) k_paged_few(const ExtendParams p) {
+  using F = PxFew<D, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  const int b = p.flat ? 0 : p.sorted ? px_nth_longest<F::kThreads>(p, blockIdx.z, reinterpret_cast<int*>(smem)) : blockIdx.z;
+  int start, n, ctx;
+  px_list(p, b, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0, start, n, ctx);
+  const int n_valid = min(F::kRows, n * p.group);                // the host launches this kernel only where all rows fit
+  if (n_valid <= 0) {                                            // uniform over the cluster
+    if (p.part_mode == 1) px_launch_dependents();
+    if (p.part_mode == 2) px_wait_prior_grid();
+    return;
+  }
+  if (p.part_mode == 1) px_launch_dependents();
+  if constexpr (NT == 5) {                                       // a list with few of the rows that the longest one may have
+    if (n_valid <= 24) { px_few_list<D, 3, F>(p, smem, b, start, n, ctx, n_valid); return; }
+  }
+  px_few_list<D, NT, F>(p, smem, b, start, n, ctx, n_valid);
+}
+
 // Joins the sets of the launches that split the keys over several clusters: D / 4 threads for the columns of a row, kParts of
 // such groups for its sets (1 for a few sets and many rows; a CTA a row for the dozens of sets of a single long context,
 // which took 32 us one after the other).
@@ -1187,8 +1229,9 @@ struct PxPlan {
 // `lists` row lists of up to `rows` rows that see at most `keys` keys each; groups only where partial sets may be written.
 static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys, bool may_group) {
   PxPlan q;
-  // 64 sequences over 300..4096 keys, D = 64: 40 rows 74 us against 89 in the kernel for many rows, 24 rows 59 against 77 (one
-  // context of 100000 keys, 40 rows: 52 against 47); D = 128 over 99k keys: 16 rows 41 against 41, 32 rows 68 against 63
+  // 64 sequences over 300..4096 keys, D = 64: 40 rows 84 us against 100 in the kernel for many rows, 24 rows 62 against 91 (one
+  // context of 100000 keys: 40 rows 65 against 54, 24 rows 49 and 49); D = 128: 16 rows 76 against 74 (99k keys: 44 against 43), 8
+  // rows 65 against 74 (42 against 43)
   const int few_most = D == 64 ? 40 : 16;
   q.nt = 0;
   q.tiles = 1;
@@ -1260,7 +1303,7 @@ static cudaError_t px_few(const ExtendParams& p, dim3 grid, cudaStream_t st) {
   return px_launch<k_paged_few<D, NT>>(p, grid, PxFew<D, NT>::kThreads, PxFew<D, NT>::kBytes, p.part_mode == 2, st);
 }
 template <int D>
-static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
+static cudaError_t px_many(const ExtendParams& p, dim3 grid, bool fine, cudaStream_t st) {
   // The maps are made for every call: they take a fraction of a microsecond, and nothing is kept by an address.
   CUtensorMap tk{}, tv{};
   const uint64_t inner = static_cast<uint64_t>(p.hkv) * D, rows = static_cast<uint64_t>(p.num_blocks) * p.block_size;
@@ -1274,9 +1317,13 @@ static cudaError_t px_many(const ExtendParams& p, dim3 grid, cudaStream_t st) {
                    make_tensor_map_2d(&tv, p.v_cache, kTmaBf16, inner, rows, inner * 2, 64, a.tma_rows, kTmaSwizzle128);
     if (rc != 0) a.tma_rows = 0;                                 // then every block is copied by hand
   }
-  return p.splits == 1 && p.part_mode == 0
-             ? px_launch<k_paged_extend<D, true>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, false, st, tk, tv)
-             : px_launch<k_paged_extend<D, false>>(a, grid, PxSmem<D>::kThreads, PxSmem<D>::kBytes, p.part_mode == 2, st, tk, tv);
+  const int threads = PxSmem<D>::kThreads, smem = PxSmem<D>::kBytes;
+  const bool direct = p.splits == 1 && p.part_mode == 0, dependent = p.part_mode == 2;
+  if (fine)
+    return direct ? px_launch<k_paged_extend<D, true, true>>(a, grid, threads, smem, false, st, tk, tv)
+                  : px_launch<k_paged_extend<D, false, true>>(a, grid, threads, smem, dependent, st, tk, tv);
+  return direct ? px_launch<k_paged_extend<D, true, false>>(a, grid, threads, smem, false, st, tk, tv)
+                : px_launch<k_paged_extend<D, false, false>>(a, grid, threads, smem, dependent, st, tk, tv);
 }
 
 template <int D, int kParts>
@@ -1291,10 +1338,12 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
   p.groups = q.groups;
   p.sorted = !p.flat && lists > 1 && lists <= PX_SORT_MOST && q.tiles * q.splits * q.groups * p.hkv * lists > q.slots;
   const dim3 grid(static_cast<unsigned>(q.tiles) * q.splits * q.groups, p.hkv, lists);
+  // steps of a few tokens: P in two parts, see the head of this file
+  const bool fine = p.flat || q.tiles == 1;
   cudaError_t e;
   if (D == 64) {
     switch (q.nt) {
-      case 0: e = px_many<64>(p, grid, st); break;
+      case 0: e = px_many<64>(p, grid, fine, st); break;
       case 1: e = px_few<64, 1>(p, grid, st); break;
       case 2: e = px_few<64, 2>(p, grid, st); break;
       case 3: e = px_few<64, 3>(p, grid, st); break;
@@ -1302,7 +1351,7 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
     }
   } else {
     switch (q.nt) {
-      case 0: e = px_many<128>(p, grid, st); break;
+      case 0: e = px_many<128>(p, grid, fine, st); break;
       case 1: e = px_few<128, 1>(p, grid, st); break;
       default: e = px_few<128, 2>(p, grid, st); break;
     }

@@ -548,3 +548,50 @@ def test_results_do_not_change_between_runs(window, D, hq, hkv):
     assert torch.equal(S.paged_extend(*args), first)
     assert torch.equal(S.shared_prefix_decode(*one), shared)
   G.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ probabilities of decode steps
+def _once_rounded(q, k, v, tables, ctx, starts, lens, sinks, scale, window):
+  """(out, bound, owned) where only the result is rounded to bf16: ``attend`` with its allowance for rounded probabilities
+  (half a step, 2^-8 of sum p |v|) taken out again.  What is left of it: probabilities that hold 2^-15 of themselves, and a sum
+  over the keys in steps of 8 whose fp32 additions each lose 2^-22 of sum p |v|."""
+  from serve_oracle import BF16
+  want, bound, owned = attend(q, k, v, tables, ctx, starts, lens, sinks, scale, window)
+  a = attend(q, k, v.abs(), tables, ctx, starts, lens, sinks, scale, window)[0]
+  return want, bound + a * (2.0 ** -15 + max(ctx) / 8 * 2.0 ** -22 - BF16), owned
+
+
+@pytest.mark.parametrize("hq,hkv,D,lens,ctx,window", [
+  (8, 2, 64, [1, 2, 1], [300, 77, 1000], 0), (16, 2, 64, [1, 2, 0, 1], [300, 500, 9, 64], 150), (24, 3, 64, [3, 1], [700, 20], 0),
+  (16, 2, 64, [5, 4], [600, 130], 0), (64, 8, 64, [1] * 5, [400, 90, 1, 33, 700], 128), (8, 2, 128, [2, 1], [300, 500], 0),
+  (16, 2, 128, [2, 1], [300, 500], 0), (32, 4, 128, [4], [5000], 0), (32, 4, 128, [4, 5], [900, 300], 100), (64, 8, 64, [9, 16], [700, 900], 0),
+  (8, 1, 64, [2], [9000], 0), (70, 1, 64, [1, 1], [500, 90], 0)])
+@pytest.mark.parametrize("use_sinks", [False, True])
+def test_a_few_tokens_are_rounded_once(hq, hkv, D, lens, ctx, window, use_sinks):
+  """Decode steps and drafted ones keep what ``paged_decode`` gives: probabilities in more than the type of the values."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(hq + len(ctx))
+  k, v, tables = paged(ctx, 16, hkv, D, g)
+  starts = [sum(lens[:b]) for b in range(len(lens))]
+  q = torch.randn(sum(lens), hq, D, generator=g).bfloat16()
+  sinks = torch.randn(hq, generator=g) if use_sinks else None
+  want, bound, _ = _once_rounded(q, k, v, tables, ctx, starts, lens, sinks, D ** -0.5, window)
+  sd = None if sinks is None else sinks.to(DEV)
+  out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), sd, D ** -0.5, window,
+                       max_q_len=max(lens))
+  within(out, want, bound)
+  if max(lens) == 1 and min(lens) == 1:
+    within(S.paged_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), sd, D ** -0.5, window), want, bound, "paged_decode")
+
+
+@pytest.mark.parametrize("hq,hkv,D,B,prefix,window", [(8, 2, 64, 3, 300, 0), (64, 8, 64, 20, 160, 0), (64, 8, 64, 20, 160, 100), (16, 16, 128, 2, 333, 0),
+                                                      (32, 4, 128, 9, 1000, 0), (48, 1, 64, 3, 500, 0), (16, 1, 128, 40, 4000, 0)])
+def test_a_shared_prefix_is_rounded_once(hq, hkv, D, B, prefix, window):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(B)
+  ctx = [prefix + 1 + 13 * b for b in range(B)]
+  k, v, tables = paged(ctx, 16, hkv, D, g, shared=prefix)
+  q, sinks = torch.randn(B, hq, D, generator=g).bfloat16(), torch.randn(hq, generator=g)
+  want, bound, _ = _once_rounded(q, k, v, tables, ctx, list(range(B)), [1] * B, sinks, D ** -0.5, window)
+  out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix, sinks.to(DEV), D ** -0.5, window)
+  within(out, want, bound)
