@@ -242,7 +242,7 @@ NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool 
     if (c > p.capacity && speaker) report_status(p.status, kStatusBadIndex, 1021, tok, c);
     pos = min(c, p.capacity) - 1;
   }
-  lo = max(p.window > 0 ? max(0, pos - p.window + 1) : 0, p.key_begin);
+  lo = max(p.window > 0 ? max(0, max(pos, 0) - p.window + 1) : 0, p.key_begin);    // before position 0: stays within 32 bits
   hi = min(pos + 1, p.key_end);
 }
 NMOE_DEVICE float px_sink(const ExtendParams& p, int h) {         // log2 units

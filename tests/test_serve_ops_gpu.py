@@ -595,3 +595,19 @@ def test_a_shared_prefix_is_rounded_once(hq, hkv, D, B, prefix, window):
   want, bound, _ = _once_rounded(q, k, v, tables, ctx, list(range(B)), [1] * B, sinks, D ** -0.5, window)
   out = S.shared_prefix_decode(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), prefix, sinks.to(DEV), D ** -0.5, window)
   within(out, want, bound)
+
+
+# ------------------------------------------------------------------------------------------------ bounds at the ends of 32 bits
+@pytest.mark.parametrize("n,hq", [(6, 8), (40, 8), (200, 8), (9, 1)])
+def test_the_largest_window_hides_nothing(n, hq):
+  """More new tokens than context: those before position 0 see nothing, the others everything, whatever the window's size."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(n)
+  ctx, lens = [n - 4, n + 30], [n, n]
+  k, v, tables = paged(ctx, 16, 1, 64, g)
+  q = torch.randn(2 * n, hq, 64, generator=g).bfloat16()
+  want, bound, _ = attend(q, k, v, tables, ctx, [0, n], lens, None, 0.125, 0)
+  for window in (2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30, 0):
+    out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, n]), i32(lens), None, 0.125, window, max_q_len=n)
+    within(out, want, bound, f"window {window}")
+  assert (out[:4] == 0).all()
