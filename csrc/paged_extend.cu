@@ -186,6 +186,7 @@ NMOE_DEVICE void px_list(const ExtendParams& p, int b, bool speaker, int& start,
     if (speaker) report_status(p.status, kStatusBadIndex, 1021, b, ctx);
     ctx = p.capacity;
   }
+  ctx = max(ctx, 0);                                             // a negative length is none: positions must not wrap below
 }
 // The list of blocks with index z: the z-th longest context where one wave of CTAs does not hold them all, so that the long
 // ones start first and the short ones fill the end (64 drafted steps: 102 -> 74 us).  Every CTA ranks the contexts for itself,
@@ -240,7 +241,7 @@ NMOE_DEVICE void px_bounds(const ExtendParams& p, int tok, int n, int ctx, bool 
   if (p.flat) {
     const int c = p.context_lens[tok];
     if (c > p.capacity && speaker) report_status(p.status, kStatusBadIndex, 1021, tok, c);
-    pos = min(c, p.capacity) - 1;
+    pos = min(max(c, 0), p.capacity) - 1;
   }
   lo = max(p.window > 0 ? max(0, max(pos, 0) - p.window + 1) : 0, p.key_begin);    // before position 0: stays within 32 bits
   hi = min(pos + 1, p.key_end);

@@ -216,7 +216,7 @@ def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_st
   g = Hq // Hkv
   out = torch.zeros_like(q) if out is None else out
   for b in range(context_lens.numel()):
-    s0, n, ctx = int(q_starts[b]), int(q_lens[b]), int(context_lens[b])
+    s0, n, ctx = int(q_starts[b]), int(q_lens[b]), max(int(context_lens[b]), 0)
     if n == 0:
       continue
     pos = torch.arange(ctx, device=q.device)
@@ -296,7 +296,7 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   q [N, Hq, D]: the tokens of sequence b are rows q_starts[b] .. q_starts[b] + q_lens[b] - 1 (sequences do not overlap; gaps
   are fine); its token j stands at position context_lens[b] - q_lens[b] + j and sees the keys at or before it, of those the
   last ``window`` if that is positive.  sinks [Hq]: a logit per head that only enters the denominator.  A token that sees no
-  key gives zeros.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].  K and V of the
+  key gives zeros, a context below 0 counts as 0.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].  K and V of the
   positions before ``context_lens[b]`` (within the window of the first new token) are finite; what else the pages hold does not matter.
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.
   Sequences whose rows lie outside q or exceed ``max_q_len`` are skipped, contexts longer than their table are cut, pages
@@ -343,7 +343,7 @@ def shared_prefix_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
   if not q.is_cuda:
     one = torch.ones_like(context_lens)
     return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, torch.cumsum(one, 0) - 1,
-                                  torch.minimum(one, context_lens), sinks, scale, window)
+                                  context_lens.clamp(0, 1), sinks, scale, window)
   with _on(q.device):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _attend("shared_prefix_decode", q, k_cache, v_cache, block_tables, context_lens.contiguous(), None, None, sinks, out, scale, window,

@@ -183,3 +183,13 @@ def test_c_entries_refuse_sizes_that_are_none():
   ver = S._fn("nmoe_verify_draft", "plplpippppp" + "iiipp")
   assert ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, 3, 0, 5, 0, 0) == 0
   assert ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, 3, 2, 0, 0, 0) == -1 and ver(0, 5, 0, 0, 0, 1, 0, 0, 0, 0, 0, -3, 2, 5, 0, 0) == -1
+
+
+def test_contexts_below_zero_are_empty():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  args = (k, v, tables, i32([ctx[0], 0, ctx[2], ctx[3]]), i32(starts), i32(lens), sinks, 0.25)
+  want = S.paged_extend(q, *args)
+  low = S.paged_extend(q, *args[:3], i32([ctx[0], -2 ** 31, ctx[2], ctx[3]]), *args[4:])
+  assert torch.equal(low, want) and (low[10:13] == 0).all()
+  out = S.shared_prefix_decode(q[:4], k, v, tables, i32([5, -2 ** 31, -1, 30]), 0, sinks, 0.25)
+  assert torch.equal(out, S.shared_prefix_decode(q[:4], k, v, tables, i32([5, 0, 0, 30]), 0, sinks, 0.25)) and (out[1:3] == 0).all()

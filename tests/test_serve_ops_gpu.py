@@ -611,3 +611,26 @@ def test_the_largest_window_hides_nothing(n, hq):
     out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([0, n]), i32(lens), None, 0.125, window, max_q_len=n)
     within(out, want, bound, f"window {window}")
   assert (out[:4] == 0).all()
+
+
+@pytest.mark.parametrize("D,hq,hkv", [(64, 8, 2), (64, 64, 1), (128, 32, 4)])
+def test_contexts_below_zero_are_empty(D, hq, hkv):
+  """However far below: no position may wrap around to one that looks past the block table."""
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(D)
+  low = -2 ** 31
+  ctx, lens = [50, low, -1, low + 1, 90, low + 3], [2, 2, 3, 1, 2, 4]
+  k, v, tables = paged([max(c, 0) for c in ctx], 16, hkv, D, g, shared=32)
+  starts = [sum(lens[:b]) for b in range(6)]
+  q = torch.randn(sum(lens), hq, D, generator=g).bfloat16()
+  real = [max(c, 0) for c in ctx]
+  for window in (0, 7):
+    want, bound, _ = attend(q, k, v, tables, real, starts, lens, None, D ** -0.5, window)
+    for most in (4, sum(lens)):
+      out = S.paged_extend(q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, D ** -0.5, window, max_q_len=most)
+      within(out, want, bound)
+    want, bound, _ = attend(q[:6], k, v, tables, real, list(range(6)), [1 if c > 0 else 0 for c in ctx], None, D ** -0.5, window)
+    out = S.shared_prefix_decode(q[:6].to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), 32, None, D ** -0.5, window)
+    within(out, want, bound)
+  G.check_status()
