@@ -101,15 +101,16 @@ class CacheView:
     self.q_starts, self.q_lens, self.max_q_len = q_starts, q_lens, max_q_len   # extend: rows of each sequence (int32 [B]), their most
     self.shared_len = shared_len                            # decode: leading tokens whose blocks are the same in every table
 
-  def describe_prefill(self) -> None:
-    """Rows and contexts of a padded prefill batch in the packed form that ``paged_extend`` takes, once per step."""
-    if self.q_lens is None:
-      B, S = self.slots.shape
-      dev = self.slots.device
-      self.q_lens = (self.slots >= 0).sum(1, dtype=torch.int32)
-      self.q_starts = torch.arange(0, B * S, S, dtype=torch.int32, device=dev)
-      self.context_lens = self.q_lens + torch.tensor(self.prefix_lens, dtype=torch.int32).to(dev)
-      self.max_q_len = S
+  def prefill_rows(self) -> Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]:
+    """(q_starts, q_lens, context_lens) of a padded prefill batch in the packed form that ``paged_extend`` takes, None where no
+    sequence has cached tokens.  Worked out from what the view holds now, once per pass: nothing of it stays in the view."""
+    if self.prefix_lens is None or not any(p > 0 for p in self.prefix_lens):
+      return None
+    B, S = self.slots.shape
+    dev = self.slots.device
+    q_lens = (self.slots >= 0).sum(1, dtype=torch.int32)
+    return (torch.arange(0, B * S, S, dtype=torch.int32, device=dev), q_lens,
+            q_lens + torch.tensor(self.prefix_lens, dtype=torch.int32).to(dev))
 
 
 class Attention(nn.Module):
@@ -145,16 +146,17 @@ class Attention(nn.Module):
   def _out(self, x, o):
     return x + ops.linear(o.reshape(*x.shape[:-1], self.nq * self.d), self.out_w, self.out_b)
 
-  def prefill(self, x, pos, rot, cache: Optional[CacheView]):
+  def prefill(self, x, pos, rot, cache: Optional[CacheView], rows=None):
     """x [B,S,H]; positions [B,S] (absolute).  Sequences with a cached prefix attend to it through
-    the pages of the cache (their own rows are written first)."""
+    the pages of the cache (their own rows are written first); ``rows``: what ``cache.prefill_rows()`` gave for this pass."""
     B, S, _ = x.shape
-    has_prefix = cache is not None and cache.prefix_lens is not None and any(p > 0 for p in cache.prefix_lens)
-    q, k, v = self._qkv(x, pos, rot, cache, need_kv=not has_prefix)
-    if has_prefix:
-      cache.describe_prefill()
-      o = sops.paged_extend(q, cache.k_cache[self.layer], cache.v_cache[self.layer], cache.block_tables, cache.context_lens,
-                            cache.q_starts, cache.q_lens, self.sinks, self.scale, self.window, max_q_len=cache.max_q_len)
+    if rows is None and cache is not None:
+      rows = cache.prefill_rows()
+    q, k, v = self._qkv(x, pos, rot, cache, need_kv=rows is None)
+    if rows is not None:
+      starts, lens, ctx = rows
+      o = sops.paged_extend(q, cache.k_cache[self.layer], cache.v_cache[self.layer], cache.block_tables, ctx, starts, lens, self.sinks,
+                            self.scale, self.window, max_q_len=S)
     else:
       o = self._dense_attention(q.view(B, S, self.nq, self.d), k.view(B, S, self.nkv, self.d), v.reshape(B, S, self.nkv, self.d))
     return self._out(x, o)
@@ -311,8 +313,9 @@ class Transformer(nn.Module):
     rot = (self.inv_freq.float(), self.conc)                    # Module.to(dtype) casts the buffer too
     taps: Dict[int, torch.Tensor] = {}
     mode = "prefill" if is_prefill else "decode" if cache.q_lens is None else "extend"
+    args = (cache.prefill_rows() if cache is not None else None,) if is_prefill else ()
     for i in range(start, stop):
-      x = getattr(self.attn[i], mode)(x, positions, rot, cache)
+      x = getattr(self.attn[i], mode)(x, positions, rot, cache, *args)
       x = self.mlp[i](x)
       if return_hidden_states and (i + 1) in (self.cfg.probe_layer, self.cfg.judge_layer):
         taps[i + 1] = x.detach()

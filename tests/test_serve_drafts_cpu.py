@@ -101,3 +101,23 @@ def test_a_shared_prefix_is_found_and_changes_nothing(model, monkeypatch):
 def test_draft_arguments():
   with pytest.raises(ValueError):
     Engine.generate(None, [], draft_tokens=-1)
+
+
+def test_a_cache_view_can_be_used_again(model):
+  """A prompt in chunks through one view whose slots, tables and lengths the caller moves on, then decode with it: every pass
+  sees what the view holds when it is called."""
+  from nmoe_b200.serve.model import CacheView
+  cfg, bs, n = model.cfg, 4, 23
+  shape = (cfg.num_hidden_layers, 8, bs, cfg.num_key_value_heads, cfg.head_dim)
+  ids = torch.tensor([(7 * i + 3) % 64 for i in range(n + 1)])
+  want = model(ids.view(1, -1), torch.arange(n + 1).view(1, -1))[0]
+  view = CacheView(torch.zeros(shape), torch.zeros(shape), None, block_tables=torch.arange(8, dtype=torch.int32).view(1, 8), block_size=bs)
+  at = 0
+  for m in (8, 4, 11):
+    view.slots, view.prefix_lens = torch.arange(at, at + m, dtype=torch.int32).view(1, m), [at]
+    got = model(ids[at:at + m].view(1, m), torch.arange(at, at + m).view(1, m), cache=view)[0]
+    assert torch.allclose(got, want[at:at + m], atol=1e-4)       # fp32 throughout, logits of order one
+    at += m
+  view.slots, view.context_lens = torch.tensor([n], dtype=torch.int32), torch.tensor([n + 1], dtype=torch.int32)
+  got = model(ids[n:], torch.tensor([n]), cache=view, is_prefill=False)
+  assert got.shape == (1, 64) and torch.allclose(got[0], want[n], atol=1e-4)
