@@ -284,6 +284,15 @@ class Transformer(nn.Module):
       for m in self.mlp:
         m.rdep = self.rdep
 
+  def _apply(self, fn, recurse=True):
+    """``Module.to`` and its kin move the rotary frequencies but leave them in fp32: rounded to bf16 they are off by 2^-8, which
+    is 0.8 radians at position 500."""
+    kept = self.inv_freq
+    super()._apply(fn, recurse)
+    if kept.dtype == torch.float32 and self.inv_freq.dtype != torch.float32:
+      self.inv_freq = kept.to(self.inv_freq.device)
+    return self
+
   @torch.no_grad()
   def init_weights(self, std: float = 0.02, seed: int = 0) -> None:
     from ..models.init import normal_
@@ -310,7 +319,7 @@ class Transformer(nn.Module):
     start = 0 if from_layer is None else max(0, min(L, int(from_layer)))
     stop = L if up_to_layer is None else max(start, min(L, int(up_to_layer)))
     x = hidden_in if (start > 0 and hidden_in is not None) else ops.embedding(input_ids, self.embed, 1.0)
-    rot = (self.inv_freq.float(), self.conc)                    # Module.to(dtype) casts the buffer too
+    rot = (self.inv_freq.float(), self.conc)
     taps: Dict[int, torch.Tensor] = {}
     mode = "prefill" if is_prefill else "decode" if cache.q_lens is None else "extend"
     args = (cache.prefill_rows() if cache is not None else None,) if is_prefill else ()

@@ -121,3 +121,16 @@ def test_a_cache_view_can_be_used_again(model):
   view.slots, view.context_lens = torch.tensor([n], dtype=torch.int32), torch.tensor([n + 1], dtype=torch.int32)
   got = model(ids[n:], torch.tensor([n]), cache=view, is_prefill=False)
   assert got.shape == (1, 64) and torch.allclose(got[0], want[n], atol=1e-4)
+
+
+def test_a_cast_model_keeps_its_rotary_frequencies(model):
+  """A model that is cast as a whole says what one of that type with the same weights says, at far positions too."""
+  import copy
+  ids, pos = torch.arange(20).view(1, 20), torch.arange(500, 520).view(1, 20)
+  for dtype in (torch.bfloat16, torch.float64):
+    want = Transformer(model.cfg, dtype=dtype)
+    want.load_state_dict({k: v.to(dtype) for k, v in model.state_dict().items()})
+    cast = copy.deepcopy(model).to(dtype)
+    assert cast.embed.dtype == dtype and torch.equal(cast.inv_freq, model.inv_freq) and cast.inv_freq.dtype == torch.float32
+    assert torch.equal(cast(ids, pos), want(ids, pos))
+  assert torch.equal(copy.deepcopy(model).bfloat16().float().inv_freq, model.inv_freq)
