@@ -357,12 +357,15 @@ def verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, dra
   out = torch.full((tokens.numel(),), -1, dtype=torch.int32) if out is None else out
   n_out = torch.zeros(q_lens.numel(), dtype=torch.int32)
   u = uniforms.double()
+  V = target_probs.size(1)
   for b, (s0, n) in enumerate(zip(q_starts.tolist(), q_lens.tolist())):
     if n == 0:
       continue
     j = 1
     while j < n:
       x = int(tokens[s0 + j])
+      if not 0 <= x < V:
+        break
       qx = 1.0 if draft_probs is None else float(draft_probs[s0 + j, x])
       if not float(u[s0 + j]) * qx < float(target_probs[s0 + j - 1, x]):
         break
@@ -372,7 +375,8 @@ def verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, dra
     if j < n:
       if draft_probs is None:
         w = p.clone()
-        w[int(tokens[s0 + j])] = 0.0
+        if 0 <= int(tokens[s0 + j]) < V:
+          w[int(tokens[s0 + j])] = 0.0
       else:
         w = (p - draft_probs[s0 + j].double()).clamp_(min=0.0)
       if not float(w.sum()) > 0.0:

@@ -193,3 +193,22 @@ def test_contexts_below_zero_are_empty():
   assert torch.equal(low, want) and (low[10:13] == 0).all()
   out = S.shared_prefix_decode(q[:4], k, v, tables, i32([5, -2 ** 31, -1, 30]), 0, sinks, 0.25)
   assert torch.equal(out, S.shared_prefix_decode(q[:4], k, v, tables, i32([5, 0, 0, 30]), 0, sinks, 0.25)) and (out[1:3] == 0).all()
+
+
+OUTSIDE = [-1, -8, 8, 2 ** 31 - 1, -2 ** 31, 2 ** 32 + 3, -2 ** 63]
+
+
+@pytest.mark.parametrize("x", OUTSIDE)
+@pytest.mark.parametrize("dist", [False, True])
+def test_a_drafted_token_outside_the_vocabulary_fails(x, dist):
+  """Whatever the row holds at either end: the token is not emitted, and the redraw takes the whole row."""
+  target = torch.tensor([[0.25, 0, 0, 0, 0, 0, 0, 1.0]]).repeat(4, 1)
+  draft = torch.zeros(4, 8) if dist else None
+  for u, new in ((0.0, 0), (0.19, 0), (0.21, 7), (0.99, 7)):       # the first entry holds a fifth of the row
+    for at in (1, 3):
+      toks = torch.tensor([0, 7, 7, 7])
+      toks[at] = x
+      uni = torch.zeros(4)
+      uni[0] = u
+      out, n = S.verify_draft(target, toks, uni, i32([0]), i32([4]), draft)
+      assert out.tolist() == [7] * (at - 1) + [new] + [-1] * (4 - at) and n.tolist() == [at]

@@ -634,3 +634,24 @@ def test_contexts_below_zero_are_empty(D, hq, hkv):
     out = S.shared_prefix_decode(q[:6].to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), 32, None, D ** -0.5, window)
     within(out, want, bound)
   G.check_status()
+
+
+@pytest.mark.parametrize("dist", [False, True])
+def test_verify_draft_tokens_outside_the_vocabulary_fail(dist):
+  """Negative, just past the end, and numbers that 32 bits would cut to one inside."""
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  from nmoe_b200.serve import ops as S
+  G.check_status()
+  target = torch.tensor([[0.25, 0, 0, 0, 0, 0, 0, 1.0]]).repeat(4, 1)
+  draft = torch.zeros(4, 8) if dist else None
+  for x in (-1, -8, 8, 2 ** 31 - 1, -2 ** 31, 2 ** 32 + 3, -2 ** 63):
+    for u in (0.0, 0.19, 0.21, 0.99):
+      for at in (1, 3):
+        toks, uni = torch.tensor([0, 7, 7, 7]), torch.zeros(4)
+        toks[at], uni[0] = x, u
+        want, count = S.verify_draft(target, toks, uni, i32([0]).cpu(), i32([4]).cpu(), draft)
+        out, n = S.verify_draft(target.to(DEV), toks.to(DEV), uni.to(DEV), i32([0]), i32([4]), None if draft is None else draft.to(DEV))
+        with pytest.raises(NativeLibraryError, match="code=2 where=1011"):
+          G.check_status()
+        assert out.tolist() == want.tolist() and n.tolist() == count.tolist() == [at]
