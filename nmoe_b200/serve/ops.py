@@ -138,6 +138,13 @@ def _check_int32(t: torch.Tensor, device: torch.device, what: str) -> None:
     raise ValueError(f"{what} must be int32 on {device}")
 
 
+def _report(device: torch.device, where: int, a: int, b: int = 0) -> None:
+  """An index that a plain statement skips, in the status record of its device (code 2, as the kernels write it)."""
+  rec = status_buffer(device)
+  if int(rec[0]) == 0:
+    rec.copy_(torch.tensor([2, where, a, b]).clamp(-2 ** 31, 2 ** 31 - 1))
+
+
 # ------------------------------------------------------------------ rotate and append
 def rope_append_reference(qkv, positions, inv_freq, conc, n_heads, n_kv_heads, k_cache=None, v_cache=None, slots=None):
   """Plain statement of ``rope_append`` (angles in fp64, the rest in fp32): rotated q, rotated k, v."""
@@ -209,20 +216,34 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tens
 
 
 # ------------------------------------------------------------------ several query tokens per sequence
-def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window=0, out=None):
+def paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window=0, out=None,
+                           max_q_len=None):
   """Plain statement of ``paged_extend`` in fp32, sequence by sequence."""
   N, Hq, D = q.shape
-  _, bs, Hkv, _ = k_cache.shape
+  num_blocks, bs, Hkv, _ = k_cache.shape
   g = Hq // Hkv
   out = torch.zeros_like(q) if out is None else out
+  capacity = block_tables.size(1) * bs
   for b in range(context_lens.numel()):
     s0, n, ctx = int(q_starts[b]), int(q_lens[b]), max(int(context_lens[b]), 0)
+    if s0 < 0 or n < 0 or s0 + n > N or (max_q_len is not None and n > max_q_len):
+      _report(q.device, 1020, b, s0)
+      continue
     if n == 0:
       continue
-    pos = torch.arange(ctx, device=q.device)
-    slot = block_tables[b, pos // bs].long() * bs + pos % bs
-    k = k_cache.view(-1, Hkv, D)[slot].float().repeat_interleave(g, dim=1)                # [ctx, Hq, D]
-    v = v_cache.view(-1, Hkv, D)[slot].float().repeat_interleave(g, dim=1)
+    if ctx > capacity:
+      _report(q.device, 1021, b, ctx)
+      ctx = capacity
+    first = max(0, ctx - n - window + 1) if window > 0 else 0                             # the oldest key that any of them sees
+    pos = torch.arange(first, ctx, device=q.device)
+    page = block_tables[b, pos // bs].long()
+    there = (page >= 0) & (page < num_blocks)
+    if not bool(there.all()):
+      _report(q.device, 1022, b)
+    slot = torch.where(there, page, 0) * bs + pos % bs
+    none = ~there.view(-1, 1, 1)
+    k, v = (c.view(-1, Hkv, D)[slot].float().masked_fill(none, 0.0).repeat_interleave(g, dim=1) if num_blocks else
+            torch.zeros(ctx - first, Hq, D, device=q.device) for c in (k_cache, v_cache))             # [m, Hq, D]
     s = torch.einsum("nhd,khd->hnk", q[s0:s0 + n].float(), k) * scale
     at = torch.arange(ctx - n, ctx, device=q.device).unsqueeze(1)
     seen = pos <= at
@@ -314,7 +335,7 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   if out is not None and (out.shape != given.shape or out.dtype != given.dtype or out.device != dev or not out.is_contiguous()):
     raise ValueError("out must be contiguous and like q")
   if not q.is_cuda:
-    return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window, out)
+    return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window, out, max_q_len)
   if out is not None and out.data_ptr() % 16 != 0:
     raise ValueError("out must start on a 16-byte boundary")
   with _on(dev):

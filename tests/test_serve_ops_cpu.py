@@ -212,3 +212,44 @@ def test_a_drafted_token_outside_the_vocabulary_fails(x, dist):
       uni[0] = u
       out, n = S.verify_draft(target, toks, uni, i32([0]), i32([4]), draft)
       assert out.tolist() == [7] * (at - 1) + [new] + [-1] * (4 - at) and n.tolist() == [at]
+
+
+def _reported(where):
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.ops._lib import NativeLibraryError
+  with pytest.raises(NativeLibraryError, match=f"code=2 where={where}"):
+    G.check_status(torch.device("cpu"))
+
+
+def test_paged_extend_plain_skips_and_reports_bad_pages_and_lengths():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  call = lambda t=tables, c=ctx, s=starts, n=lens, k=k, v=v, **kw: S.paged_extend(q, k, v, t, i32(c), i32(s), i32(n), sinks, 0.25, **kw)
+  good = call()
+  # a page outside the cache counts as zeros: what a page of zeros gives
+  bad, zk, zv = tables.clone(), torch.cat((k, torch.zeros_like(k[:1]))), torch.cat((v, torch.zeros_like(v[:1])))
+  bad[3, 1] = len(k)
+  zeros = call(t=bad, k=zk, v=zv)
+  for page in (-1, len(k), -2 ** 31, 2 ** 31 - 1):
+    bad[3, 1] = page
+    assert torch.equal(call(t=bad), zeros)
+    _reported(1022)
+  # a context past its table is cut there
+  assert torch.equal(call(t=tables[:, :4].contiguous(), c=[5, 3, 32, 90]), call(t=tables[:, :4].contiguous(), c=[5, 3, 32, 32]))
+  _reported(1021)
+  # rows outside q, and more of them than announced: the sequence is skipped, the others are not
+  for s, n, kw in (([9, 10, 13, -1], lens, {}), ([9, 10, 13, 7], lens, {}), (starts, [1, 3, 0, -9], {}), (starts, lens, dict(max_q_len=8))):
+    out = call(s=s, n=n, **kw)
+    _reported(1020)
+    assert torch.equal(out[9:], good[9:]) and (out[:9] == 0).all()
+
+
+def test_paged_extend_plain_ignores_what_lies_before_the_window():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case(4)
+  args = (i32(ctx), i32(starts), i32(lens), sinks, 0.25, 4)
+  want = S.paged_extend(q, k, v, tables, *args)
+  for t in range(ctx[3] - lens[3] - 4 + 1):
+    k[tables[3, t // 8].long(), t % 8] = float("nan")
+    v[tables[3, t // 8].long(), t % 8] = float("inf")
+  assert torch.equal(S.paged_extend(q, k, v, tables, *args), want)
+  tables[3, :2] = -1                                # pages that nobody looks at
+  assert torch.equal(S.paged_extend(q, k, v, tables, *args), want)
