@@ -157,7 +157,10 @@ def rope_append_reference(qkv, positions, inv_freq, conc, n_heads, n_kv_heads, k
   qk = torch.cat((x1 * cos - x2 * sin, x2 * cos + x1 * sin), dim=-1).to(qkv.dtype)
   q, k, v = qk[:, :n_heads].contiguous(), qk[:, n_heads:].contiguous(), x[:, n_heads + n_kv_heads:].contiguous()
   if slots is not None:
-    ok = slots >= 0
+    past = (slots >= k_cache.size(0) * k_cache.size(1)).nonzero()
+    if past.numel():
+      _report(qkv.device, 1000, int(past[0]), int(slots[past[0]]))
+    ok = (slots >= 0) & (slots < k_cache.size(0) * k_cache.size(1))
     k_cache.view(-1, n_kv_heads, D)[slots[ok].long()] = k[ok]
     v_cache.view(-1, n_kv_heads, D)[slots[ok].long()] = v[ok]
   return q, k, v

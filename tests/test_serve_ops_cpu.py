@@ -253,3 +253,12 @@ def test_paged_extend_plain_ignores_what_lies_before_the_window():
   assert torch.equal(S.paged_extend(q, k, v, tables, *args), want)
   tables[3, :2] = -1                                # pages that nobody looks at
   assert torch.equal(S.paged_extend(q, k, v, tables, *args), want)
+
+
+def test_rope_append_plain_skips_and_reports_a_slot_past_the_cache():
+  g = torch.Generator().manual_seed(0)
+  qkv, pos, inv = torch.randn(4, 4 * 16, generator=g), torch.arange(4), torch.ones(8)
+  kc, vc = torch.zeros(2, 4, 1, 16), torch.zeros(2, 4, 1, 16)
+  q, k, v = S.rope_append(qkv, pos, inv, 1.0, 2, 1, kc, vc, i32([7, 8, 2 ** 31 - 1, 2]), need_kv=True)
+  _reported(1000)
+  assert int((vc != 0).any(-1).sum()) == 2 and torch.equal(kc.view(8, 16)[[7, 2]], k[[0, 3], 0]) and q.shape == (4, 2, 16)
