@@ -381,14 +381,18 @@ def verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, dra
   out = torch.full((tokens.numel(),), -1, dtype=torch.int32) if out is None else out
   n_out = torch.zeros(q_lens.numel(), dtype=torch.int32)
   u = uniforms.double()
-  V = target_probs.size(1)
+  N, V = target_probs.shape
   for b, (s0, n) in enumerate(zip(q_starts.tolist(), q_lens.tolist())):
+    if s0 < 0 or n < 0 or s0 + n > N:
+      _report(tokens.device, 1010, b, s0)
+      continue
     if n == 0:
       continue
     j = 1
     while j < n:
       x = int(tokens[s0 + j])
       if not 0 <= x < V:
+        _report(tokens.device, 1011, s0 + j, x)
         break
       qx = 1.0 if draft_probs is None else float(draft_probs[s0 + j, x])
       if not float(u[s0 + j]) * qx < float(target_probs[s0 + j - 1, x]):
@@ -431,7 +435,7 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
 
   Returns (out [N] int32: the emitted tokens from row q_starts[b] on, -1 behind them; n_out [B] int32: how many, at least 1
   for a sequence with rows).  Rows of no sequence are -1, or left as they were in a given ``out``.  A drafted token outside
-  the vocabulary fails and shows up in ``check_status``."""
+  the vocabulary fails, a sequence whose rows lie outside the inputs is skipped with a count of 0; both show up in ``check_status``."""
   if target_probs.dim() != 2 or not 0 < target_probs.size(1) <= 2 ** 30:
     raise ValueError("target_probs must be [N, V], V up to 2^30")
   N, V = target_probs.shape

@@ -212,6 +212,7 @@ def test_a_drafted_token_outside_the_vocabulary_fails(x, dist):
       uni[0] = u
       out, n = S.verify_draft(target, toks, uni, i32([0]), i32([4]), draft)
       assert out.tolist() == [7] * (at - 1) + [new] + [-1] * (4 - at) and n.tolist() == [at]
+      _reported(1011)
 
 
 def _reported(where):
@@ -262,3 +263,14 @@ def test_rope_append_plain_skips_and_reports_a_slot_past_the_cache():
   q, k, v = S.rope_append(qkv, pos, inv, 1.0, 2, 1, kc, vc, i32([7, 8, 2 ** 31 - 1, 2]), need_kv=True)
   _reported(1000)
   assert int((vc != 0).any(-1).sum()) == 2 and torch.equal(kc.view(8, 16)[[7, 2]], k[[0, 3], 0]) and q.shape == (4, 2, 16)
+
+
+def test_verify_draft_plain_skips_and_reports():
+  target, u = torch.full((3, 8), 0.125), torch.zeros(3)
+  for s0, n in ((1, 3), (-1, 2), (0, -1), (2, 2 ** 31 - 1), (4, 0)):
+    out, count = S.verify_draft(target, torch.tensor([0, 1, 1]), u, i32([s0, 0]), i32([n, 1]))
+    _reported(1010)
+    assert count.tolist() == [0, 1] and out.tolist() == [0, -1, -1]
+  out, count = S.verify_draft(target, torch.tensor([0, 8, 1]), u, i32([0]), i32([3]))
+  _reported(1011)
+  assert count.tolist() == [1] and out.tolist() == [0, -1, -1]

@@ -651,6 +651,8 @@ def test_verify_draft_tokens_outside_the_vocabulary_fail(dist):
         toks, uni = torch.tensor([0, 7, 7, 7]), torch.zeros(4)
         toks[at], uni[0] = x, u
         want, count = S.verify_draft(target, toks, uni, i32([0]).cpu(), i32([4]).cpu(), draft)
+        with pytest.raises(NativeLibraryError, match="code=2 where=1011"):
+          G.check_status(torch.device("cpu"))
         out, n = S.verify_draft(target.to(DEV), toks.to(DEV), uni.to(DEV), i32([0]), i32([4]), None if draft is None else draft.to(DEV))
         with pytest.raises(NativeLibraryError, match="code=2 where=1011"):
           G.check_status()
