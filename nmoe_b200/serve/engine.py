@@ -14,7 +14,7 @@ sequence by one token.  ``generate`` wraps the loop for greedy / top-k sampling;
 runs prompts through the first layers only (the probe / judge taps of the curation stack).
 
 Two things shorten decoding.  Blocks that every running sequence has in common (a grading rubric, a
-few-shot header) are attended to once per step for the whole batch (steps without drafts).  And with ``draft_tokens`` > 0
+few-shot header) are attended to once per step for the whole batch (steps in which nobody has drafts).  And with ``draft_tokens`` > 0
 ``generate`` lets each sequence propose that many tokens per step by looking its last tokens up in
 its own text (answers that quote their prompt, structured output); one pass scores them all and
 those that fit are kept.  Greedy output is what it would be without drafts (on the GPU as far as the
@@ -27,6 +27,7 @@ raising.
 """
 from __future__ import annotations
 
+import itertools
 from collections import deque
 from typing import Callable, Deque, Dict, Iterable, List, Optional, Sequence as Seq, Tuple
 
@@ -202,7 +203,7 @@ class Engine:
   def _decode_drafts(self, seqs: List[Sequence], k: int) -> Tuple[torch.Tensor, torch.Tensor, CacheView, List[int]]:
     """One pass over the last token of every sequence and up to ``k`` looked-up ones behind it: (logits [N, vocab], the packed
     input tokens [N], the step's cache view, rows per sequence).  A sequence gets fewer where its budget, its context or the
-    free blocks end."""
+    free blocks end; where nobody has any the step is a plain decode step, behind a shared prefix if there is one."""
     dev, bs = self.device, self.block_size
     for s in seqs:
       self.pool.append_slot(s)                        # the step itself comes before anybody's drafts
@@ -218,16 +219,22 @@ class Engine:
       slots += [self.pool.slot(s, p) for p in range(first, first + 1 + len(draft))]
       lens.append(1 + len(draft))
       self.steps["drafted"] += len(draft)
-    starts = [0]
-    for n in lens[:-1]:
-      starts.append(starts[-1] + n)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32).to(dev)
     tokens = torch.tensor(ids, dtype=torch.long).to(dev)
-    cache = CacheView(self.k_cache, self.v_cache, i32(slots), block_tables=torch.from_numpy(self._tables(seqs)).to(dev),
-                      context_lens=i32([len(s) - 1 + n for s, n in zip(seqs, lens)]), block_size=bs, q_starts=i32(starts), q_lens=i32(lens),
-                      max_q_len=max(lens))
+    ctx, tables = [len(s) - 1 + n for s, n in zip(seqs, lens)], self._tables(seqs)
+    if max(lens) == 1:
+      rows = dict(shared_len=self._shared_len(tables, min(ctx)))
+    else:
+      rows = dict(q_starts=i32(self._starts(lens)), q_lens=i32(lens), max_q_len=max(lens))
+    cache = CacheView(self.k_cache, self.v_cache, i32(slots), block_tables=torch.from_numpy(tables).to(dev), context_lens=i32(ctx),
+                      block_size=bs, **rows)
     self.steps["decode"] += 1
     return self.model(tokens, torch.tensor(pos, dtype=torch.long).to(dev), cache=cache, is_prefill=False), tokens, cache, lens
+
+  @staticmethod
+  def _starts(lens: List[int]) -> List[int]:
+    """First row of each sequence where their rows follow one another."""
+    return [0] + list(itertools.accumulate(lens[:-1]))
 
   @torch.inference_mode()
   def step_drafts(self, k: int, *, temperature: float = 0.0, top_k: int = 0, generator: Optional[torch.Generator] = None
@@ -258,7 +265,10 @@ class Engine:
         row += n
     else:
       u = torch.rand(tokens.numel(), device=generator.device if generator is not None else self.device, generator=generator).to(self.device)
-      emitted, count = sops.verify_draft(probs, tokens, u, cache.q_starts, cache.q_lens, out=torch.empty_like(tokens, dtype=torch.int32))
+      rows = cache.q_starts, cache.q_lens
+      if cache.q_lens is None:                        # no drafts: one token each, drawn from its row
+        rows = (torch.tensor(x, dtype=torch.int32).to(self.device) for x in (self._starts(lens), lens))
+      emitted, count = sops.verify_draft(probs, tokens, u, *rows, out=torch.empty_like(tokens, dtype=torch.int32))
       emitted = emitted.tolist()
       for s, n, j in zip(seqs, lens, count.tolist()):
         out.append((s.seq_id, emitted[row:row + j]))

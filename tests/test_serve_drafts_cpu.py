@@ -134,3 +134,35 @@ def test_a_cast_model_keeps_its_rotary_frequencies(model):
     assert cast.embed.dtype == dtype and torch.equal(cast.inv_freq, model.inv_freq) and cast.inv_freq.dtype == torch.float32
     assert torch.equal(cast(ids, pos), want(ids, pos))
   assert torch.equal(copy.deepcopy(model).bfloat16().float().inv_freq, model.inv_freq)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_a_step_in_which_nobody_drafts_is_a_plain_one(model, monkeypatch, temperature):
+  """With nothing proposed, draft_tokens changes neither the steps (a shared prefix is attended to once) nor what they say."""
+  from nmoe_b200.serve import engine as E
+  from nmoe_b200.serve import ops as S
+  calls = {"shared_prefix_decode": 0, "paged_extend": 0}
+  for name in calls:
+    def count(*a, _inner=getattr(S, name), _name=name, **kw):
+      calls[_name] += 1
+      return _inner(*a, **kw)
+    monkeypatch.setattr(S, name, count)
+  monkeypatch.setattr(E, "MIN_SHARED_TOKENS", 4)
+
+  def run(k, propose):
+    monkeypatch.setattr(LookupDraft, "propose", propose)
+    eng = Engine(model, max_seq_len=80, max_batch=3, block_size=4)
+    eng.generate(PROMPTS[:1], max_new_tokens=1)
+    calls.update(shared_prefix_decode=0, paged_extend=0)
+    out = eng.generate(PROMPTS[:3], max_new_tokens=10, draft_tokens=k, temperature=temperature, generator=torch.Generator().manual_seed(1))
+    return out, dict(calls), eng.steps
+
+  none = lambda self, t, k: []
+  plain, plain_calls, plain_steps = run(0, none)
+  out, got, steps = run(4, none)
+  assert got == plain_calls and got["shared_prefix_decode"] == 9 and steps == plain_steps      # one layer of three has no window
+  assert temperature > 0 or out == plain
+  # one drafting sequence is enough to make it a packed step
+  out, got, _ = run(4, lambda self, t, k: [t[-1]][:k] if len(t) == 30 else [])
+  assert got["paged_extend"] > plain_calls["paged_extend"] and 0 < got["shared_prefix_decode"] < 9
+  assert temperature > 0 or out == plain
