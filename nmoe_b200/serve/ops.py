@@ -133,6 +133,15 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tenso
     raise ValueError("the cache must start on a 16-byte boundary")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+  """Whether the stretches of memory from the first to the last element of two non-empty tensors meet."""
+  def span(t):
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+  (a0, a1), (b0, b1) = span(a), span(b)
+  return a0 < b1 and b0 < a1
+
+
 def _check_int32(t: torch.Tensor, device: torch.device, what: str) -> None:
   if t.dtype != torch.int32 or t.device != device:
     raise ValueError(f"{what} must be int32 on {device}")
@@ -320,7 +329,7 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   q [N, Hq, D]: the tokens of sequence b are rows q_starts[b] .. q_starts[b] + q_lens[b] - 1 (sequences do not overlap; gaps
   are fine); its token j stands at position context_lens[b] - q_lens[b] + j and sees the keys at or before it, of those the
   last ``window`` if that is positive.  sinks [Hq]: a logit per head that only enters the denominator.  A token that sees no
-  key gives zeros, a context below 0 counts as 0.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D].  K and V of the
+  key gives zeros, a context below 0 counts as 0.  Rows of no sequence are zero in the result, or left as they were in ``out`` [N, Hq, D] (which may be q itself).  K and V of the
   positions before ``context_lens[b]`` (within the window of the first new token) are finite; what else the pages hold does not matter.
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.
   Sequences whose rows lie outside q or exceed ``max_q_len`` are skipped, contexts longer than their table are cut, pages
@@ -337,6 +346,8 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     raise ValueError("max_q_len must not be negative")
   if out is not None and (out.shape != given.shape or out.dtype != given.dtype or out.device != dev or not out.is_contiguous()):
     raise ValueError("out must be contiguous and like q")
+  if out is not None and N > 0 and (out.data_ptr() != given.data_ptr() or not given.is_contiguous()) and _overlap(out, given):
+    raise ValueError("out must be q itself or not overlap it: rows are written while others are read")
   if not q.is_cuda:
     return paged_extend_reference(q, k_cache, v_cache, block_tables, context_lens, q_starts, q_lens, sinks, scale, window, out, max_q_len)
   if out is not None and out.data_ptr() % 16 != 0:
@@ -456,8 +467,7 @@ def verify_draft(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: tor
     _check_int32(out, dev, "out")
     if out.shape != (N,) or not out.is_contiguous():
       raise ValueError("out must be a contiguous [N]")
-    first, ends = tokens.data_ptr(), ((N - 1) * tokens.stride(0) + 1) * tokens.element_size()
-    if N > 0 and first < out.data_ptr() + 4 * N and out.data_ptr() < first + ends:
+    if N > 0 and _overlap(out, tokens):
       raise ValueError("out must not overlap tokens, which are read while it is written")
   if not target_probs.is_cuda:
     return verify_draft_reference(target_probs, tokens, uniforms, q_starts, q_lens, draft_probs, out)

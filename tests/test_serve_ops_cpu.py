@@ -274,3 +274,20 @@ def test_verify_draft_plain_skips_and_reports():
   out, count = S.verify_draft(target, torch.tensor([0, 8, 1]), u, i32([0]), i32([3]))
   _reported(1011)
   assert count.tolist() == [1] and out.tolist() == [0, -1, -1]
+
+
+def test_paged_extend_writes_over_q_or_beside_it():
+  q, k, v, tables, ctx, starts, lens, sinks = _attention_case()
+  room = torch.zeros(40, 6, 16)
+  call = lambda at, out: S.paged_extend(room[at:at + 15], k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, out=out)
+  want = S.paged_extend(q, k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, out=q.clone())
+  for at, to in ((10, 10), (0, 15), (20, 5)):
+    room[at:at + 15] = q
+    room[to:to + 15] = q                            # rows of no sequence stay
+    assert torch.equal(call(at, room[to:to + 15]), want)
+  for at, to in ((10, 11), (10, 9), (10, 24), (0, 14), (14, 0)):
+    with pytest.raises(ValueError, match="overlap"):
+      call(at, room[to:to + 15])
+  wide = torch.zeros(15, 8, 16)                     # q inside a wider projection, out in the same memory
+  with pytest.raises(ValueError, match="overlap"):
+    S.paged_extend(wide[:, :6], k, v, tables, i32(ctx), i32(starts), i32(lens), sinks, 0.25, out=wide.view(-1)[:15 * 96].view(15, 6, 16))

@@ -657,3 +657,18 @@ def test_verify_draft_tokens_outside_the_vocabulary_fail(dist):
         with pytest.raises(NativeLibraryError, match="code=2 where=1011"):
           G.check_status()
         assert out.tolist() == want.tolist() and n.tolist() == count.tolist() == [at]
+
+
+@pytest.mark.parametrize("lens,ctx,D,hq,hkv", [([1, 3], [300, 70], 64, 8, 2), ([1], [30_000], 64, 8, 1), ([200, 150], [900, 400], 64, 8, 2),
+                                               ([4], [20_000], 128, 32, 4), ([60, 2, 90], [60, 700, 500], 128, 8, 2)])
+def test_paged_extend_in_place(lens, ctx, D, hq, hkv):
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(len(lens))
+  k, v, tables = paged(ctx, 16, hkv, D, g)
+  starts = [sum(lens[:b]) for b in range(len(lens))]
+  q = torch.randn(sum(lens), hq, D, generator=g).bfloat16().to(DEV)
+  args = (k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32(starts), i32(lens), None, D ** -0.5)
+  want = S.paged_extend(q, *args, max_q_len=max(lens))
+  for _ in range(5):
+    x = q.clone()
+    assert S.paged_extend(x, *args, max_q_len=max(lens), out=x) is x and torch.equal(x, want)
