@@ -39,9 +39,13 @@ from .kv import BlockPool, SeqStatus, Sequence
 from .model import CacheView, Transformer
 
 
-# A shared prefix of fewer tokens is left to the per-sequence decode kernel.  With 64 shared tokens two sequences of 64 more take
-# 9.3 us against 13.0; with 32 shared ones two take 9.5 against 10.8 and eight 10.9 against 10.9.
-MIN_SHARED_TOKENS = 64
+# A shared prefix of fewer tokens is left to paged_decode (of twice as many where a KV head's queries are little work).  Measured on
+# 2 to 128 sequences with 16 or 64 tokens of their own, shared form against paged_decode, us.  64/8 heads of 64: 4 sequences, 64
+# shared tokens 12.6 against 10.0, 96 ones 12.7 and 12.3, 128 ones 13.3 and 14.4; 128 sequences, 128 shared ones 17.9 against 95.
+# Little work: 8/2 heads of 64, 8 sequences, 128 tokens 13.4 against 10.0, 192 ones 14.1 and 12.7, 256 ones 14.4 and 15.8;
+# 16/16 heads of 64, 32 sequences, 192 tokens 14.1 against 12.4, 256 ones 14.4 and 14.8.
+MIN_SHARED_TOKENS = 128
+LITTLE_WORK = 448       # query heads of a KV head times head size
 
 
 class LookupDraft:
@@ -197,7 +201,9 @@ class Engine:
     n_blocks = min(tables.shape[1], (shortest - 1) // self.block_size)        # the block being written is nobody else's
     same = (tables[:, :n_blocks] == tables[:1, :n_blocks]).all(0)
     n = (n_blocks if same.all() else int(same.argmin())) * self.block_size
-    return n if n >= MIN_SHARED_TOKENS else 0
+    cfg = self.model.cfg
+    little = cfg.num_attention_heads // cfg.num_key_value_heads * cfg.head_dim < LITTLE_WORK
+    return n if n >= MIN_SHARED_TOKENS * (2 if little else 1) else 0
 
   # ------------------------------------------------------------------ several tokens per step
   def _decode_drafts(self, seqs: List[Sequence], k: int) -> Tuple[torch.Tensor, torch.Tensor, CacheView, List[int]]:

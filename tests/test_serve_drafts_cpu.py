@@ -166,3 +166,15 @@ def test_a_step_in_which_nobody_drafts_is_a_plain_one(model, monkeypatch, temper
   out, got, _ = run(4, lambda self, t, k: [t[-1]][:k] if len(t) == 30 else [])
   assert got["paged_extend"] > plain_calls["paged_extend"] and 0 < got["shared_prefix_decode"] < 9
   assert temperature > 0 or out == plain
+
+
+@pytest.mark.parametrize("hq,hkv,D,least", [(64, 8, 64, 128), (32, 4, 128, 128), (14, 2, 64, 128), (8, 2, 64, 256), (16, 16, 128, 256)])
+def test_a_prefix_is_shared_where_that_is_faster(hq, hkv, D, least):
+  from types import SimpleNamespace
+  import numpy as np
+  cfg = ServeConfig(num_attention_heads=hq, num_key_value_heads=hkv, head_dim=D)
+  eng = SimpleNamespace(block_size=16, model=SimpleNamespace(cfg=cfg))
+  for blocks in range(1, 40):
+    tables = np.concatenate((np.tile(np.arange(blocks), (4, 1)), 100 + np.arange(8).reshape(4, 2)), 1).astype(np.int32)
+    assert Engine._shared_len(eng, tables, blocks * 16 + 20) == (blocks * 16 if blocks * 16 >= least else 0)
+  assert Engine._shared_len(eng, tables[:1], 40 * 16) == 0

@@ -106,3 +106,45 @@ def test_a_model_cast_as_a_whole_still_runs(models):
   finally:
     mg.inv_freq = kept
   assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("draft_tokens", [0, 4])
+def test_attention_forms_of_a_step_agree(models, draft_tokens, monkeypatch):
+  """Every attention call that generation makes behind a shared rubric, with and without drafts, against paged_decode row by row on
+  the same cache: equal up to one rounding of each, on layers with and without a window."""
+  from nmoe_b200.ops import tc_gemm as G
+  from nmoe_b200.serve import Engine
+  from nmoe_b200.serve import ops as S
+  from nmoe_b200.serve.engine import LookupDraft
+  monkeypatch.setattr(LookupDraft, "propose", lambda self, t, k: t[-2:][:k] if len(t) % 3 else [])
+  seen = {"shared_prefix_decode": 0, "paged_extend": 0}
+
+  def check(o, q, kc, vc, tables, ctx, sinks, scale, window):
+    ref = S.paged_decode(q, kc, vc, tables, ctx, sinks, scale, window).double()
+    # two roundings to bf16, 2^-8 of the value each, and what the fp32 sums may leave of values of order one
+    assert ((o.double() - ref).abs() <= 2.0 ** -7 * 1.01 * ref.abs() + 2.0 ** -14).all()
+
+  inner_s, inner_e = S.shared_prefix_decode, S.paged_extend
+  def shared(q, kc, vc, tables, ctx, n, sinks, scale, window=0):
+    o = inner_s(q, kc, vc, tables, ctx, n, sinks, scale, window)
+    check(o, q, kc, vc, tables, ctx, sinks, scale, window)
+    seen["shared_prefix_decode"] += 1
+    return o
+  def extend(q, kc, vc, tables, ctx, starts, lens, sinks, scale, window=0, **kw):
+    o = inner_e(q, kc, vc, tables, ctx, starts, lens, sinks, scale, window, **kw)
+    if kw["max_q_len"] <= 5:                       # a step, not a prompt: each token as a sequence of its own
+      rows = torch.repeat_interleave(torch.arange(len(lens), device=lens.device), lens.long())
+      at = torch.arange(len(rows), device=lens.device) - starts[rows]
+      check(o, q, kc, vc, tables[rows].contiguous(), (ctx[rows] - lens[rows] + 1 + at).int(), sinks, scale, window)
+      seen["paged_extend"] += 1
+    return o
+  monkeypatch.setattr(S, "shared_prefix_decode", shared)
+  monkeypatch.setattr(S, "paged_extend", extend)
+  mg, _ = models
+  g = torch.Generator().manual_seed(4)
+  rubric = torch.randint(0, 512, (300,), generator=g).tolist()
+  eng = Engine(mg, max_seq_len=400, max_batch=8)
+  eng.generate([rubric], max_new_tokens=1)
+  out = eng.generate([rubric + torch.randint(0, 512, (n,), generator=g).tolist() for n in (3, 40, 17, 39)], max_new_tokens=12, draft_tokens=draft_tokens)
+  assert all(len(o) == 12 for o in out) and seen["shared_prefix_decode"] > 0 and (seen["paged_extend"] > 0) == (draft_tokens > 0)
+  G.check_status()
