@@ -120,7 +120,8 @@ def grade_prompts(engine, tok: Tokenizer, texts: Sequence[str], *, is_code: Opti
   ``draft_tokens`` is the engine's: the answers' keys and braces are soon found in the rubric and in the answer itself."""
   code = list(is_code) if is_code is not None else [False] * len(texts)
   prompts = [right_trim(tok, t, is_code=c, max_ctx=max_ctx, max_new=max_new, fmt=fmt) for t, c in zip(texts, code)]
-  outs = engine.generate(prompts, max_new_tokens=max_new, stop_tokens=stop_tokens, draft_tokens=draft_tokens)
+  drafts = {"draft_tokens": draft_tokens} if draft_tokens else {}          # an engine without them need not know the word
+  outs = engine.generate(prompts, max_new_tokens=max_new, stop_tokens=stop_tokens, **drafts)
   rows = []
   for o, c in zip(outs, code):
     raw = tok.decode(o)

@@ -178,3 +178,20 @@ def test_a_prefix_is_shared_where_that_is_faster(hq, hkv, D, least):
     tables = np.concatenate((np.tile(np.arange(blocks), (4, 1)), 100 + np.arange(8).reshape(4, 2)), 1).astype(np.int32)
     assert Engine._shared_len(eng, tables, blocks * 16 + 20) == (blocks * 16 if blocks * 16 >= least else 0)
   assert Engine._shared_len(eng, tables[:1], 40 * 16) == 0
+
+
+def test_grade_prompts_asks_for_drafts_only_where_they_are_wanted():
+  from nmoe_b200.data.score import ByteTokenizer, grade_prompts
+  answer = '{"helpfulness": 3, "correctness": 4, "coherence": 2, "complexity": 1, "density": 0}'
+
+  class Plain:                                      # an engine of one's own, with the arguments that generate has always had
+    def generate(self, prompts, *, max_new_tokens, stop_tokens):
+      return [list(answer.encode()) for _ in prompts]
+
+  class Drafting:
+    def generate(self, prompts, *, max_new_tokens, stop_tokens, draft_tokens):
+      assert draft_tokens == 3
+      return [list(answer.encode()) for _ in prompts]
+  tok = ByteTokenizer()
+  assert grade_prompts(Plain(), tok, ["a", "b"])[1]["scores"]["correctness"] == 4
+  assert grade_prompts(Drafting(), tok, ["a"], draft_tokens=3)[0]["scores"]["helpfulness"] == 3
