@@ -474,6 +474,8 @@ def cmd_hydra_oracle_label(a) -> int:
   from .score import grade_prompts
   if not a.output:
     raise SystemExit("hydra-oracle-label needs --output")
+  if a.draft_tokens < 0:
+    raise SystemExit("--draft-tokens must not be negative")
   model, _ = _grading_model(a)
   tok = _tokenizer(a.tokenizer)
   ids, docs, n_done = _grading_inputs(a, tok)

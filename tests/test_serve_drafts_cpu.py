@@ -195,3 +195,13 @@ def test_grade_prompts_asks_for_drafts_only_where_they_are_wanted():
   tok = ByteTokenizer()
   assert grade_prompts(Plain(), tok, ["a", "b"])[1]["scores"]["correctness"] == 4
   assert grade_prompts(Drafting(), tok, ["a"], draft_tokens=3)[0]["scores"]["helpfulness"] == 3
+
+
+def test_a_refused_draft_count_leaves_earlier_labels(tmp_path):
+  from nmoe_b200.data.cli import main
+  out, docs = tmp_path / "labels.jsonl", tmp_path / "docs.jsonl"
+  out.write_text("earlier labels\n")
+  docs.write_text('{"id": "a", "text": "x"}\n')
+  with pytest.raises(SystemExit, match="draft-tokens"):
+    main(["hydra-oracle-label", "--checkpoint", str(tmp_path / "none"), "--input", str(docs), "--output", str(out), "--draft-tokens", "-1"])
+  assert out.read_text() == "earlier labels\n"
