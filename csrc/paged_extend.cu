@@ -23,9 +23,10 @@
 // chains: four CTAs for D = 64, whose S has a single buffer to fit tensor memory, two for D = 128.  Code that is run once or
 // seldom stays rolled: with the softmax of 64 keys in one piece, 55 % of the instruction cache's request rate was the bound and
 // the fourth CTA gained nothing (699 us; loops over 32 keys: 625; loaders and start of a CTA rolled too: 597; three CTAs: 700).
-// 8 prompts of 200..1750 new tokens behind 1300..3500 cached ones, 64/8 heads of 64: 597 us, 670 TFLOP/s (issue slots 56 %,
-// special function unit 62 %, tensor cores 31 %).  What did not help: part of the exponentials by polynomial, two warps for 32
-// rows, two tiles a CTA, 16 keys at a time (631 us), keeping half of the scores between maximum and exponentials (679 us).
+// 8 prompts of 200..1750 new tokens behind 1300..3500 cached ones, 64/8 heads of 64: 597 us, 670 TFLOP/s (over a long run, at
+// lower clocks, 632 us; issue slots 55 %, special function unit 64 %, tensor cores 32 %).  What did not help: part of the
+// exponentials by polynomial, two warps for 32 rows, two tiles a CTA, 16 keys at a time (631 us), keeping half of the scores
+// between maximum and exponentials (679 us).
 //
 // Few rows (k_paged_few, below): decode steps and drafts, bound by the bytes of K and V.
 //
@@ -864,9 +865,10 @@ k_paged_extend(const ExtendParams p, const __grid_constant__ CUtensorMap tm_k, c
 // barrier is needed.  Each of four warps streams its own tiles of 16 or 32 keys through a ring of its own,
 // with its own running maximum, sum and O; they meet once at the end.  P^T turns from accumulator to operand layout with
 // movmatrix, in its two parts; the maximum is raised only when some key beats it by 2^8, which one vote a tile finds out.
-// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 69 us, 3.7 TB/s (62 with P in one part, when the stream
-// itself ran at 5.5 TB/s; 73 with 40 rows for every list; the rest is 5 us of start-up latencies a CTA and the last wave).  Equal shares of all keys for 296 CTAs, with pieces joined
-// afterwards, took 95 us: a start-up for every piece, and heads of one page no longer read together.
+// 64 sequences with 1..5 tokens over 300..4096 keys, 64/8 heads of 64: 70 us, 3.7 TB/s (62 with P in one part, when the stream
+// itself ran at 5.5 TB/s; 73 with 40 rows for every list; the rest is 5 us of start-up latencies a CTA and the last wave).  Equal
+// shares of all keys for 296 CTAs, with pieces joined afterwards, took 95 us: a start-up for every piece, and heads of one page no
+// longer read together.
 template <int D, int NT>
 struct PxFew {
   static constexpr int kWarps = 4, kThreads = 128;
@@ -1228,6 +1230,7 @@ struct PxPlan {
 };
 
 // `lists` row lists of up to `rows` rows that see at most `keys` keys each; groups only where partial sets may be written.
+// (Times: those of few_most with P in two parts, the others as they were with one, on both sides of each choice.)
 static PxPlan px_plan(int D, int hkv, long long rows, int lists, long long keys, bool may_group) {
   PxPlan q;
   // 64 sequences over 300..4096 keys, D = 64: 40 rows 84 us against 100 in the kernel for many rows, 24 rows 62 against 91 (one

@@ -672,3 +672,24 @@ def test_paged_extend_in_place(lens, ctx, D, hq, hkv):
   for _ in range(5):
     x = q.clone()
     assert S.paged_extend(x, *args, max_q_len=max(lens), out=x) is x and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("ctx", [[50, 900, 17, 300, 9, 128], [3000, 6000, 200, 5000, 9, 4100]])
+@pytest.mark.parametrize("hq,hkv,window", [(64, 8, 0), (8, 1, 0), (16, 2, 100)])
+def test_lists_of_few_rows_beside_longer_ones(ctx, hq, hkv, window):
+  """1 to 5 tokens in one call: lists of 8 to 40 rows, on their own, split over a cluster, and in sets that are joined."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(hq)
+  lens = [5, 1, 3, 2, 0, 4]
+  k, v, tables = paged(ctx, 16, hkv, 64, g)
+  starts = [sum(lens[:b]) for b in range(6)]
+  q, sinks = torch.randn(sum(lens), hq, 64, generator=g).bfloat16(), torch.randn(hq, generator=g)
+  want, bound, _ = _once_rounded(q, k, v, tables, ctx, starts, lens, sinks, 0.125, window)
+  kd, vd = k.to(DEV), v.to(DEV)
+  out = S.paged_extend(q.to(DEV), kd, vd, tables.to(DEV), i32(ctx), i32(starts), i32(lens), sinks.to(DEV), 0.125, window, max_q_len=5)
+  within(out, want, bound)
+  for b in (1, 2, 5):                               # one list at a time: other splits, sets
+    one = S.paged_extend(q.to(DEV), kd, vd, tables[b:b + 1].to(DEV), i32(ctx[b:b + 1]), i32(starts[b:b + 1]), i32(lens[b:b + 1]), sinks.to(DEV), 0.125,
+                         window, max_q_len=5)
+    rows = slice(starts[b], starts[b] + lens[b])
+    within(one[rows], want[rows], bound[rows])
