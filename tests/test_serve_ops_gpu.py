@@ -693,3 +693,35 @@ def test_lists_of_few_rows_beside_longer_ones(ctx, hq, hkv, window):
                          window, max_q_len=5)
     rows = slice(starts[b], starts[b] + lens[b])
     within(one[rows], want[rows], bound[rows])
+
+
+@pytest.mark.parametrize("D,hq,hkv,n", [(64, 8, 1, 1), (128, 32, 4, 4)])
+def test_captured_calls_with_workspaces_share_nothing(D, hq, hkv, n):
+  """Two graphs whose calls split their keys into sets, replayed in turn and on two streams at once, with new contents."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(n)
+  states, graphs, outs = [], [], []
+  for ctx in ([30_000], [21_000, 9000]):
+    B = len(ctx)
+    k, v, tables = paged(ctx, 16, hkv, D, g)
+    args = (torch.randn(n * B, hq, D, generator=g).bfloat16().to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx), i32([n * b for b in range(B)]),
+            i32([n] * B), None, D ** -0.5)
+    S.paged_extend(*args, max_q_len=n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      outs.append(S.paged_extend(*args, max_q_len=n))
+    states.append(args)
+    graphs.append(graph)
+  streams = [torch.cuda.Stream() for _ in graphs]
+  for turn in range(3):
+    for args in states:
+      args[0].copy_(torch.randn(args[0].shape, generator=g).bfloat16())
+    want = [S.paged_extend(*args, max_q_len=n) for args in states]
+    torch.cuda.synchronize()
+    for _ in range(10):
+      for graph, st in zip(graphs, streams):
+        with torch.cuda.stream(st):
+          graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
