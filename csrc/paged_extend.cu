@@ -14,7 +14,7 @@
 // after the final division.  The sum l takes the unrounded p.
 //
 // Roundings of P.  The tensor core multiplies it with bf16 values, so it has to be bf16 too.  Steps of a few tokens (the kernel for
-// few rows, lists of one tile, a shared prefix) take it in two parts, its bf16 value and the bf16 value of what that leaves, at
+// few rows, lists of one tile or one token, a shared prefix) take it in two parts, its bf16 value and the bf16 value of what that leaves, at
 // twice the products of P V: what comes out is rounded once, as paged_decode's results are (which has P in fp32), whichever kernel a
 // sequence's step happens to run on.  Error of the result relative to its norm 1.7e-3, with one part 2.4e-3.  Prompts of several
 // tiles take one part, as the dense attention of a prompt without a cached prefix does (8 prompts: 597 us, in two parts 795).
@@ -1343,7 +1343,7 @@ static int px_run(ExtendParams& p, const PxPlan& q, int D, int lists, cudaStream
   p.sorted = !p.flat && lists > 1 && lists <= PX_SORT_MOST && q.tiles * q.splits * q.groups * p.hkv * lists > q.slots;
   const dim3 grid(static_cast<unsigned>(q.tiles) * q.splits * q.groups, p.hkv, lists);
   // steps of a few tokens: P in two parts, see the head of this file
-  const bool fine = p.flat || q.tiles == 1;
+  const bool fine = p.flat || q.tiles == 1 || p.max_q_len == 1;
   cudaError_t e;
   if (D == 64) {
     switch (q.nt) {

@@ -332,7 +332,7 @@ def paged_extend(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
   key gives zeros, a context below 0 counts as 0.  Rows of no sequence are zero in the result, or left as they were in ``out``
   [N, Hq, D] (which may be q itself).  K and V of the positions before ``context_lens[b]`` (within the window of the first new token) are finite; what else the pages hold does not matter.
   ``max_q_len``: an upper bound of q_lens known to the host (default N); with a tight one fewer empty blocks are launched.  Where it
-  is at most 128 rows of a KV head (max_q_len * Hq / Hkv) the result is rounded once, as that of ``paged_decode``; beyond, in prompts,
+  is one token, or at most 128 rows of a KV head (max_q_len * Hq / Hkv), the result is rounded once, as that of ``paged_decode``; beyond, in prompts,
   the probabilities are rounded to bf16 before they meet the values, as in dense attention.
   Sequences whose rows lie outside q or exceed ``max_q_len`` are skipped, contexts longer than their table are cut, pages
   outside the cache count as zeros: all three show up in ``check_status``."""

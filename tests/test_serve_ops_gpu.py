@@ -725,3 +725,18 @@ def test_captured_calls_with_workspaces_share_nothing(D, hq, hkv, n):
           graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("hq,D", [(129, 64), (200, 64), (130, 128)])
+def test_one_token_of_many_heads_is_rounded_once(hq, D):
+  """More query heads of a KV head than a tile holds: still decode steps."""
+  from nmoe_b200.serve import ops as S
+  g = torch.Generator().manual_seed(hq)
+  ctx = [180, 90, 161]
+  k, v, tables = paged(ctx, 16, 1, D, g, shared=80)
+  q, sinks = torch.randn(3, hq, D, generator=g).bfloat16(), torch.randn(hq, generator=g)
+  want, bound, _ = _once_rounded(q, k, v, tables, ctx, [0, 1, 2], [1] * 3, sinks, D ** -0.5, 0)
+  args = q.to(DEV), k.to(DEV), v.to(DEV), tables.to(DEV), i32(ctx)
+  within(S.paged_extend(*args, i32([0, 1, 2]), i32([1] * 3), sinks.to(DEV), D ** -0.5, max_q_len=1), want, bound)
+  for prefix in (0, 80):
+    within(S.shared_prefix_decode(*args, prefix, sinks.to(DEV), D ** -0.5), want, bound, f"prefix {prefix}")
